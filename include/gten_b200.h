@@ -114,6 +114,91 @@ int gtn_bias_add_inplace(gtn_tensor* inp, const gtn_tensor* bias, int start_pos,
 int gtn_token_embed(const gtn_tensor* weight, const gtn_tensor* tokens, gtn_tensor* out, int start_pos,
                     void* stream);
 
+/* ---- paged serving operators --------------------------------------------------------------- */
+/* No counterpart in the reference, whose cache is one contiguous buffer per sequence (modules.cpp:78-104).
+ * A pool of fixed-size pages holds the keys and values of many requests; a block table names each
+ * request's pages in order, so that token j of request b lies in page block_table[b][j / page_size], row
+ * j % page_size. A step of a server over ragged requests calls, in this order,
+ *   gtn_paged_plan     pages for the new tokens, block tables, slot map and positions, on the device;
+ *   gtn_paged_append   per layer: rotary at each token's own position, K and V rows into their pages;
+ *   gtn_paged_attn     per layer: attention of the new tokens over the pages.
+ * The token-wise tensors hold the new tokens of all requests back to back: request b's are rows
+ * q_start[b] .. q_start[b + 1]; rows behind the last request are padding and stay as they were.
+ * Lengths, tables and slots are read on the device, so a captured graph follows them. Every index
+ * read there is bounds-checked: a bad one touches no memory and raises GTN_ERR_DEVICE at the next
+ * gtn_check (the rows that it concerns are unspecified). Numerics: fp32 (not the reference's order). */
+
+/* Descriptor of a paged cache. k and v are two pools of n_pages pages each, page_stride bytes apart
+ * (0: page after page), 16-byte aligned, page_stride a multiple of 16. Inside a page:
+ *   GTN_F16  fp16 [kv_heads][page_size][d_head];
+ *   GTN_Q8   int8 [kv_heads][page_size][d_head], then the fp16 deltas [kv_heads][page_size][d_head / 32]
+ *            (the values of Q8 blocks, values and deltas apart so that rows are 16-byte aligned).
+ * page_size: 16, 32, 64, 128 or 256; d_head: 64 or 128; n_pages * page_size < 2^31. */
+typedef struct gtn_paged_cache {
+    void* k;
+    void* v;
+    int32_t dtype;
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t d_head;
+    int64_t page_stride;
+} gtn_paged_cache;
+
+/* Bytes of one page of the pool of k or v (the smallest page_stride); 0 for arguments outside the above. */
+int64_t gtn_paged_page_bytes(int dtype, int page_size, int kv_heads, int d_head);
+
+/* Plans one step for n requests (1 to 4096). All tensors int32 on the device:
+ *   ctx_lens [n], new_lens [n]   tokens already in the cache, tokens of this step (0 allowed);
+ *   free_pages [f], n_free [1]   page ids to hand out, in order; how many of them are free (<= f);
+ *   block_table [n, max_pages]   in and out: the first ceil(ctx / page_size) entries of a row are its
+ *                                pages; the pages for the new tokens are written behind them;
+ *   q_start [n + 1]              prefix sum of new_lens;
+ *   kv_lens [n]                  ctx + new where granted, else 0;
+ *   pos [rows], slots [rows]     position of each row in its request (-1: padding); page * page_size +
+ *                                offset (-1: padding, or not granted);
+ *   n_used [1]                   pages taken from the front of free_pages.
+ * Requests are served in order. One is not granted when its lengths are negative, its tokens fit
+ * neither the table's row nor the `rows` rows, or when it needs pages and those of the requests up to
+ * it exceed n_free; the caller plans it again in a later step. The free list itself is not changed. */
+int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const gtn_tensor* free_pages,
+                   const gtn_tensor* n_free, int page_size, gtn_tensor* block_table, gtn_tensor* q_start,
+                   gtn_tensor* kv_lens, gtn_tensor* pos, gtn_tensor* slots, gtn_tensor* n_used, void* stream);
+
+/* Rotary embedding at pos[r] (rotate-half on the first rope_pct of each head, as gtn_rotary_emb, with
+ * angles pos * rope_base^(-2j/rd) formed in 64 bits) of the query and key rows, and the key and value
+ * rows into the pages of slots[r]. q [rows, heads * d_head], k and v [rows, kv_heads * d_head]: fp32, fp16
+ * or Q8, one type, row strides as in their descriptors (they may be column ranges of one stacked
+ * projection); q_out [rows, heads * d_head]: fp16 or Q8; pos and slots: int32 [rows]. q_out may be q's own
+ * memory when type and strides agree. Q8 results use the activation quantizer (gtn_quantize_q8_rows), but
+ * Q8 value rows go to a Q8 cache unchanged. Rows with pos < 0 are skipped, rows with slot < 0 write no
+ * cache row; two rows must not share a slot. */
+int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor* v, const gtn_tensor* pos,
+                     const gtn_tensor* slots, const gtn_paged_cache* cache, gtn_tensor* q_out, float rope_pct,
+                     float rope_base, void* stream);
+
+/* Attention of the new tokens over the pages, with GQA (query head h reads kv head h / (heads /
+ * kv_heads)). Row q_start[b] + i of request b is the token at position p = kv_lens[b] - new_b + i
+ * (new_b = q_start[b + 1] - q_start[b]) and sees the keys j <= p; with window > 0 only those with
+ * j > p - window or j < n_sink. out = sum_j softmax_j(scale q.k_j) v_j; zeros for a row that sees no key
+ * (kv_lens[b] = 0: a request that was not granted). Keys that a row does not see never reach it,
+ * whatever they hold, and table entries whose page no row of the request sees may be anything.
+ *   q, out [rows, heads * d_head]: fp16 (16-byte aligned rows) or Q8, the same type and shape, rows < 2^20;
+ *   block_table int32 [n, max_pages], q_start int32 [n + 1], kv_lens int32 [n], n <= 4096;
+ *   scale: 0 means 1 / sqrt(d_head); max_new: a bound on the new tokens of one request where the caller
+ *   knows one (1 for a decode step), else 0: it chooses the kernels, not the result;
+ *   workspace: device memory of gtn_paged_attn_workspace(...) bytes, 16-byte aligned; its contents are
+ *   scratch, and calls that may run at the same time need one each.
+ * Q8 caches and activations enter the products as fp16, so |value| must stay below 65504. */
+int64_t gtn_paged_attn_workspace(int heads, int d_head);
+int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_tensor* block_table,
+                   const gtn_tensor* q_start, const gtn_tensor* kv_lens, gtn_tensor* out, float scale, int window,
+                   int n_sink, int max_new, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Waits for `stream` and returns GTN_ERR_DEVICE if a kernel on the current device flagged an error
+ * since the last check (gtn_model_check for callers without a model). */
+int gtn_check(void* stream);
+
 /* ---- quantization (src/gten/quants.cpp, src/<model>/<model>_to_gten.py) ------------------- */
 
 /* Weight packer, bit-exact with the reference converters' q8_quantize / q4_quantize

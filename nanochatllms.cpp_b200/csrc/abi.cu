@@ -7,6 +7,7 @@
 #include <mutex>
 #include <tuple>
 
+#include "abi.cuh"
 #include "launch.cuh"
 
 namespace gtn {
@@ -23,11 +24,6 @@ int fail(int code, const char* fmt, ...) {
     va_end(ap);
     g_last_error = buf;
     return code;
-}
-
-static int cuda_status(cudaError_t e, const char* what) {
-    if (e == cudaSuccess) return GTN_OK;
-    return fail(e == cudaErrorMemoryAllocation ? GTN_ERR_OOM : GTN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
 static std::atomic<unsigned long long> g_launches{0};
@@ -517,58 +513,6 @@ static cudaError_t matmul_tma(const uint8_t* X, long xs, int M, const uint8_t* W
 }  // namespace gtn
 
 using namespace gtn;
-
-// ---- tensor helpers (tensor.h:96-116 bstride) -------------------------------------------------
-static bool valid_dtype(int dt) { return dt >= GTN_I32 && dt <= GTN_Q4; }
-
-static long bstride(const gtn_tensor* t, int i) {
-    const long s = t->strides[i];
-    switch (t->dtype) {
-        case GTN_Q4: return s == 1 ? 1 : (s / GTN_QBLK) * GTN_Q4_BYTES;
-        case GTN_Q8: return s == 1 ? 1 : (s / GTN_QBLK) * GTN_Q8_BYTES;
-        case GTN_F16: return s * 2;
-        default: return s * 4;
-    }
-}
-
-static int check_tensor(const gtn_tensor* t, const char* name) {
-    if (!t) return fail(GTN_ERR_ARG, "%s is NULL", name);
-    if (!t->data) return fail(GTN_ERR_ARG, "%s has no data", name);
-    if (!valid_dtype(t->dtype)) return fail(GTN_ERR_ARG, "%s has invalid dtype %d", name, t->dtype);
-    if (t->ndim < 1 || t->ndim > 3) return fail(GTN_ERR_ARG, "%s has %d dims", name, t->ndim);
-    for (int i = 0; i < t->ndim; ++i)
-        if (t->shape[i] <= 0) return fail(GTN_ERR_ARG, "%s dim %d is %d", name, i, t->shape[i]);
-    // Quantized rows of a partial last block: the reference allocates ceil(n/32) blocks per row
-    // (tensor.cpp:43-45) but steps rows by floor(n/32) blocks (tensor.h:196-200), so rows beyond
-    // the first overlap. Only single-row use is well defined.
-    if ((t->dtype == GTN_Q8 || t->dtype == GTN_Q4) && t->ndim >= 2 && t->shape[t->ndim - 1] % GTN_QBLK != 0) {
-        long rows = 1;
-        for (int i = 0; i < t->ndim - 1; ++i) rows *= t->shape[i];
-        if (rows > 1)
-            return fail(GTN_ERR_ARG, "%s: quantized rows of %d elements (not a multiple of 32) overlap", name,
-                        t->shape[t->ndim - 1]);
-    }
-    return GTN_OK;
-}
-
-static bool shape_eq(const gtn_tensor* a, const gtn_tensor* b) {
-    if (a->ndim != b->ndim) return false;
-    for (int i = 0; i < a->ndim; ++i)
-        if (a->shape[i] != b->shape[i]) return false;
-    return true;
-}
-
-static cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
-
-#define GTN_CHECK(expr)                 \
-    do {                                \
-        const int rc_ = (expr);         \
-        if (rc_ != GTN_OK) return rc_;  \
-    } while (0)
-#define GTN_REQUIRE(cond, ...)                              \
-    do {                                                    \
-        if (!(cond)) return fail(GTN_ERR_ARG, __VA_ARGS__); \
-    } while (0)
 
 static int launched(const char* what) { return cuda_status(cudaGetLastError(), what); }
 

@@ -23,8 +23,8 @@
 #include <thread>
 #include <vector>
 
+#include "abi.cuh"
 #include "fused.cuh"
-#include "launch.cuh"
 
 namespace gtn {
 
@@ -701,14 +701,6 @@ static int forward(gtn_model* m, int seq, int n, int sp) {
     GK(matmul_f32(m->a, rd_, adt, 1, m->lm_head, m->emb_rs, m->wdt, m->n_vocab, d, lg, m->n_vocab, st));
     GK(launch_pdl(k_argmax, dim3(1), dim3(1024), 0, st, (const float*)lg, m->n_vocab, m->next + seq, 0L, 0L));
 #undef GK
-    return GTN_OK;
-}
-
-static int check_dev_err() {
-    const unsigned int v = take_device_error();
-    if (v)
-        return fail(GTN_ERR_DEVICE, "device-side error code %u (1: a bounded wait expired, 2: token id out of range)",
-                    v);
     return GTN_OK;
 }
 

@@ -1,0 +1,403 @@
+// Paged serving operators: the step planner (gtn_paged_plan) and the cache append with rotary positions
+// (gtn_paged_append). The attention over the pages is in paged_attn.cu.
+#include "paged.cuh"
+
+#include <cmath>
+
+namespace gtn {
+
+int paged_cache_args(const gtn_paged_cache* c, const char* who, PagedCache* out) {
+    GTN_REQUIRE(c, "%s: cache is NULL", who);
+    GTN_REQUIRE(c->k && c->v, "%s: cache has no data", who);
+    GTN_REQUIRE(c->dtype == GTN_F16 || c->dtype == GTN_Q8, "%s: cache dtype %d (F16 or Q8)", who, c->dtype);
+    const long need = gtn_paged_page_bytes(c->dtype, c->page_size, c->kv_heads, c->d_head);
+    GTN_REQUIRE(need > 0, "%s: page_size %d, kv_heads %d, d_head %d unsupported", who, c->page_size, c->kv_heads,
+                c->d_head);
+    GTN_REQUIRE(c->n_pages > 0 && (long)c->n_pages * c->page_size < (1L << 31), "%s: n_pages %d", who, c->n_pages);
+    const long stride = c->page_stride ? c->page_stride : need;
+    GTN_REQUIRE(stride >= need && stride % 16 == 0 && stride < (1L << 40), "%s: page_stride %ld (pages of %ld bytes)",
+                who, (long)c->page_stride, need);
+    GTN_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, "%s: pools must be 16-byte aligned", who);
+    out->k = (uint8_t*)c->k;
+    out->v = (uint8_t*)c->v;
+    out->page_stride = stride;
+    out->dt = c->dtype;
+    out->n_pages = c->n_pages;
+    out->ps = c->page_size;
+    out->ps_shift = __builtin_ctz((unsigned)c->page_size);
+    out->kv_heads = c->kv_heads;
+    out->d = c->d_head;
+    return GTN_OK;
+}
+
+int paged_int_arg(const gtn_tensor* t, int ndim, const char* who, const char* name) {
+    GTN_CHECK(check_tensor(t, name));
+    GTN_REQUIRE(t->dtype == GTN_I32 && t->ndim == ndim, "%s: %s must be int32, %d-D", who, name, ndim);
+    GTN_REQUIRE(t->shape[ndim - 1] == 1 || t->strides[ndim - 1] == 1, "%s: %s must be contiguous", who, name);
+    GTN_REQUIRE(ndim == 1 || t->strides[0] >= t->shape[1], "%s: %s rows overlap", who, name);
+    return GTN_OK;
+}
+
+int paged_on_device(const void* const* p, int n, const char* who) {
+    int dev = 0;
+    GTN_CHECK(cuda_status(cudaGetDevice(&dev), who));
+    for (int i = 0; i < n; ++i) {
+        cudaPointerAttributes a;
+        GTN_CHECK(cuda_status(cudaPointerGetAttributes(&a, p[i]), who));
+        GTN_REQUIRE(a.type == cudaMemoryTypeManaged || (a.type == cudaMemoryTypeDevice && a.device == dev),
+                    "%s: tensor data %p is not memory of the current device %d", who, p[i], dev);
+    }
+    return GTN_OK;
+}
+
+// ---- planner -----------------------------------------------------------------------------------
+// need_b = ceil((ctx + new) / ps) - ceil(ctx / ps) pages, granted while the inclusive prefix of need
+// stays within n_free; q_start = prefix of new. Every CTA runs both prefix sums over all requests itself
+// (at most 8 requests a thread; a second kernel for them would cost more than the few microseconds of
+// one CTA) and then writes its share of the table entries and of the rows.
+constexpr int PLAN_THREADS = 512;
+constexpr int PLAN_ROWS = 1024;  // rows per CTA
+
+struct PlanArgs {
+    const int32_t *ctx, *nw, *free_pages, *n_free;
+    int32_t *table, *q_start, *kv_lens, *pos, *slots, *n_used;
+    long table_stride;
+    int n, n_cap, max_pages, rows, ps_shift;
+};
+
+// Exclusive prefix over the CTA's threads of one value each; *total receives the sum. red: 17 values of
+// shared memory.
+__device__ __forceinline__ long long plan_scan(long long x, long long* red, long long* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long s = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+    }
+    __syncthreads();  // red may still be read from an earlier scan
+    if (lane == 31) red[warp] = s;
+    __syncthreads();
+    if (warp == 0) {
+        long long w = lane < PLAN_THREADS / 32 ? red[lane] : 0;
+        const long long own = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        if (lane < PLAN_THREADS / 32) red[lane] = w - own;
+        if (lane == 31) red[16] = w;
+    }
+    __syncthreads();
+    *total = red[16];
+    return red[warp] + s - x;
+}
+
+static __global__ void __launch_bounds__(PLAN_THREADS) k_paged_plan(PlanArgs a) {
+    __shared__ int s_qend[PAGED_MAX_REQ];  // end row of each request
+    __shared__ int s_off[PAGED_MAX_REQ];   // pages of the granted requests before it; -1 - that if not granted
+    __shared__ long long red[17];
+    __shared__ int s_used;
+    pdl_wait();
+    const int tid = threadIdx.x, per = (a.n + PLAN_THREADS - 1) / PLAN_THREADS, b0 = tid * per;
+    const int psm = (1 << a.ps_shift) - 1;
+    int ctx[8], nw[8];
+    long long rows = 0, rows_all;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool in = i < per && b0 + i < a.n;
+        ctx[i] = in ? a.ctx[b0 + i] : 0;
+        nw[i] = in ? a.nw[b0 + i] : 0;
+        rows += nw[i] > 0 ? nw[i] : 0;
+    }
+    const int n_free = min(a.n_cap, *a.n_free);
+    long long end = plan_scan(rows, red, &rows_all);
+    int need[8];
+    bool fits[8];
+    long long pages = 0, pages_all;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        end += nw[i] > 0 ? nw[i] : 0;
+        const long long kv = (long long)ctx[i] + nw[i];
+        fits[i] = ctx[i] >= 0 && nw[i] >= 0 && kv <= ((long long)a.max_pages << a.ps_shift) && end <= a.rows;
+        need[i] = fits[i] ? (int)((kv + psm) >> a.ps_shift) - (int)(((long long)ctx[i] + psm) >> a.ps_shift) : 0;
+        pages += need[i];
+        if (i < per && b0 + i < a.n) {
+            const int e = (int)(end < 0x7fffffffLL ? end : 0x7fffffffLL);
+            s_qend[b0 + i] = e;
+            if (blockIdx.x == 0) a.q_start[b0 + i + 1] = e;
+        }
+    }
+    if (blockIdx.x == 0 && tid == 0) a.q_start[0] = 0;
+    long long off = plan_scan(pages, red, &pages_all);
+    if (tid == 0) s_used = 0;
+    __syncthreads();
+    int used = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool grant = fits[i] && (need[i] == 0 || off + need[i] <= n_free);
+        if (i < per && b0 + i < a.n) {
+            s_off[b0 + i] = grant ? (int)min(off, 0x7ffffffeLL) : -1;
+            if (blockIdx.x == 0) a.kv_lens[b0 + i] = grant ? ctx[i] + nw[i] : 0;
+            if (grant) used += need[i];
+        }
+        off += need[i];
+    }
+    if (blockIdx.x == 0 && used) atomicAdd(&s_used, used);
+    __syncthreads();
+    if (blockIdx.x == 0 && tid == 0) *a.n_used = s_used;
+    // new table entries: request b by CTA b mod grid, one warp each
+    const int lane = tid & 31, warp = tid >> 5;
+    for (int b = blockIdx.x * (PLAN_THREADS / 32) + warp; b < a.n; b += gridDim.x * (PLAN_THREADS / 32)) {
+        const int o = s_off[b];
+        if (o < 0) continue;
+        const int c = a.ctx[b], have = (c + psm) >> a.ps_shift;
+        const int nd = (int)(((long long)c + a.nw[b] + psm) >> a.ps_shift) - have;
+        for (int i = lane; i < nd; i += 32) a.table[b * a.table_stride + have + i] = a.free_pages[o + i];
+    }
+    // rows: the request by binary search in the row ends, the page from the old table entries or, for a
+    // page that this step hands out, from the free list
+    for (int t = blockIdx.x * PLAN_ROWS + tid; t < min(a.rows, (int)(blockIdx.x + 1) * PLAN_ROWS); t += PLAN_THREADS) {
+        int pos = -1, slot = -1;
+        if (t < rows_all) {
+            int lo = 0, hi = a.n - 1;  // the first b with s_qend[b] > t
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (s_qend[mid] > t) hi = mid;
+                else lo = mid + 1;
+            }
+            const int c = a.ctx[lo];
+            pos = c + (t - (lo > 0 ? s_qend[lo - 1] : 0));
+            const int o = s_off[lo];
+            if (o >= 0) {
+                const int have = (c + psm) >> a.ps_shift, col = pos >> a.ps_shift;
+                const int page = col < have ? a.table[lo * a.table_stride + col] : a.free_pages[o + col - have];
+                slot = page < 0 ? -1 : (page << a.ps_shift) + (pos & psm);
+            }
+        }
+        a.pos[t] = pos;
+        a.slots[t] = slot;
+    }
+}
+
+// ---- append ------------------------------------------------------------------------------------
+struct AppendArgs {
+    const uint8_t *q, *k, *v;
+    long qs, ks, vs, os;  // row strides, bytes
+    const int32_t *pos, *slots;
+    uint8_t* out;
+    PagedCache c;
+    int heads, sdt, odt, half;
+    unsigned int* err;
+};
+struct RopeFreq {
+    double f[64];  // base^(-2j / rd)
+};
+
+constexpr int APP_THREADS = 256;
+
+// One CTA per row, one warp per head; lane l holds elements l, l + 32, ... of its head, so that a 32-element
+// block is one element per lane (the activation quantizer's layout).
+template <int D>
+static __global__ void __launch_bounds__(APP_THREADS) k_paged_append(AppendArgs a, const __grid_constant__ RopeFreq fr) {
+    constexpr int NB = D / GTN_QBLK;
+    __shared__ float2 cs[64];
+    __shared__ float buf[APP_THREADS / 32][D];
+    pdl_wait();
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int pos = a.pos[t], slot = a.slots[t];
+    if (pos < 0) return;
+    if (tid < a.half) {
+        // the angle in 64 bits, reduced to [-pi, pi] before the fp32 sine: an fp32 angle is off by
+        // pos * 2^-24 radians
+        const double x = (double)pos * fr.f[tid];
+        const double r = fma(-rint(x * 0.15915494309189535), 6.283185307179586, x);
+        float sn, cn;
+        sincosf((float)r, &sn, &cn);
+        cs[tid] = make_float2(cn, sn);
+    }
+    __syncthreads();
+    const int kvh = a.c.kv_heads, page = slot >> a.c.ps_shift, r = slot & (a.c.ps - 1);
+    const bool store = slot >= 0 && page < a.c.n_pages;
+    if (slot >= 0 && !store && tid == 0 && a.err) atomicOr(a.err, GTN_DEVERR_PAGE);
+    const long hb = row_bytes(a.sdt, D);
+    for (int hh = warp; hh < a.heads + 2 * kvh; hh += APP_THREADS / 32) {
+        const bool is_q = hh < a.heads, is_k = !is_q && hh < a.heads + kvh;
+        if (!is_q && !store) continue;
+        const int h = is_q ? hh : (is_k ? hh - a.heads : hh - a.heads - kvh);
+        const uint8_t* src = (is_q ? a.q + (long)t * a.qs : is_k ? a.k + (long)t * a.ks : a.v + (long)t * a.vs) + h * hb;
+        float x[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) x[i] = load_elem(src, a.sdt, i * GTN_QBLK + lane);
+        if ((is_q || is_k) && a.half > 0) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < NB; ++i) buf[warp][i * GTN_QBLK + lane] = x[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int e = i * GTN_QBLK + lane;
+                if (e < a.half) {
+                    const float2 w = cs[e];
+                    x[i] = fmaf(x[i], w.x, -(buf[warp][e + a.half] * w.y));
+                } else if (e < 2 * a.half) {
+                    const float2 w = cs[e - a.half];
+                    x[i] = fmaf(buf[warp][e - a.half], w.y, x[i] * w.x);
+                }
+            }
+        }
+        if (is_q) {
+            uint8_t* dst = a.out + (long)t * a.os + h * row_bytes(a.odt, D);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) store_row_elem(dst, a.odt, i, lane, D, x[i]);
+            continue;
+        }
+        uint8_t* pg = (is_k ? a.c.k : a.c.v) + (long)page * a.c.page_stride;
+        uint8_t* dst = pg + paged_row(a.c, h, r);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            if (a.c.dt == GTN_F16) {
+                reinterpret_cast<uint16_t*>(dst)[i * GTN_QBLK + lane] = f2h(x[i]);
+                continue;
+            }
+            uint16_t dh;
+            int8_t qv;
+            if (!is_k && a.sdt == GTN_Q8) {  // V blocks pass unchanged
+                dh = ld_u16(src + i * GTN_Q8_BYTES);
+                qv = (int8_t)src[i * GTN_Q8_BYTES + 2 + lane];
+            } else {
+                qv = warp_quant_block(x[i], lane, GTN_QBLK, &dh);
+            }
+            dst[i * GTN_QBLK + lane] = (uint8_t)qv;
+            if (lane == 0) reinterpret_cast<uint16_t*>(pg + paged_delta(a.c, h, r))[i] = dh;
+        }
+    }
+}
+
+}  // namespace gtn
+
+using namespace gtn;
+
+extern "C" {
+
+int64_t gtn_paged_page_bytes(int dtype, int page_size, int kv_heads, int d_head) {
+    if (dtype != GTN_F16 && dtype != GTN_Q8) return 0;
+    if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1))) return 0;
+    if ((d_head != 64 && d_head != 128) || kv_heads < 1 || kv_heads > 1024) return 0;
+    return paged_page_bytes(dtype, page_size, kv_heads, d_head);
+}
+
+int gtn_check(void* stream) {
+    GTN_CHECK(cuda_status(cudaStreamSynchronize(S(stream)), "check"));
+    return check_dev_err();
+}
+
+int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const gtn_tensor* free_pages,
+                   const gtn_tensor* n_free, int page_size, gtn_tensor* block_table, gtn_tensor* q_start,
+                   gtn_tensor* kv_lens, gtn_tensor* pos, gtn_tensor* slots, gtn_tensor* n_used, void* stream) {
+    const char* who = "paged_plan";
+    GTN_CHECK(paged_int_arg(ctx_lens, 1, who, "ctx_lens"));
+    GTN_CHECK(paged_int_arg(new_lens, 1, who, "new_lens"));
+    GTN_CHECK(paged_int_arg(free_pages, 1, who, "free_pages"));
+    GTN_CHECK(paged_int_arg(n_free, 1, who, "n_free"));
+    GTN_CHECK(paged_int_arg(block_table, 2, who, "block_table"));
+    GTN_CHECK(paged_int_arg(q_start, 1, who, "q_start"));
+    GTN_CHECK(paged_int_arg(kv_lens, 1, who, "kv_lens"));
+    GTN_CHECK(paged_int_arg(pos, 1, who, "pos"));
+    GTN_CHECK(paged_int_arg(slots, 1, who, "slots"));
+    GTN_CHECK(paged_int_arg(n_used, 1, who, "n_used"));
+    const int n = ctx_lens->shape[0];
+    GTN_REQUIRE(n <= PAGED_MAX_REQ, "%s: %d requests (at most %d)", who, n, PAGED_MAX_REQ);
+    GTN_REQUIRE(new_lens->shape[0] == n && kv_lens->shape[0] == n && block_table->shape[0] == n &&
+                    q_start->shape[0] == n + 1,
+                "%s: shapes do not agree on %d requests", who, n);
+    GTN_REQUIRE(pos->shape[0] == slots->shape[0], "%s: pos and slots differ in rows", who);
+    GTN_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0, "%s: page_size %d", who,
+                page_size);
+    const void* ptrs[] = {ctx_lens->data, new_lens->data, free_pages->data, n_free->data, block_table->data,
+                          q_start->data,  kv_lens->data,  pos->data,        slots->data,  n_used->data};
+    GTN_CHECK(paged_on_device(ptrs, 10, who));
+    PlanArgs a;
+    a.ctx = (const int32_t*)ctx_lens->data;
+    a.nw = (const int32_t*)new_lens->data;
+    a.free_pages = (const int32_t*)free_pages->data;
+    a.n_free = (const int32_t*)n_free->data;
+    a.table = (int32_t*)block_table->data;
+    a.q_start = (int32_t*)q_start->data;
+    a.kv_lens = (int32_t*)kv_lens->data;
+    a.pos = (int32_t*)pos->data;
+    a.slots = (int32_t*)slots->data;
+    a.n_used = (int32_t*)n_used->data;
+    a.table_stride = block_table->strides[0];
+    a.n = n;
+    a.n_cap = free_pages->shape[0];
+    a.max_pages = block_table->shape[1];
+    a.rows = pos->shape[0];
+    a.ps_shift = __builtin_ctz((unsigned)page_size);
+    return cuda_status(launch_pdl(k_paged_plan, dim3((a.rows + PLAN_ROWS - 1) / PLAN_ROWS), dim3(PLAN_THREADS), 0,
+                                  S(stream), a),
+                       who);
+}
+
+int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor* v, const gtn_tensor* pos,
+                     const gtn_tensor* slots, const gtn_paged_cache* cache, gtn_tensor* q_out, float rope_pct,
+                     float rope_base, void* stream) {
+    const char* who = "paged_append";
+    AppendArgs a;
+    GTN_CHECK(paged_cache_args(cache, who, &a.c));
+    GTN_CHECK(check_tensor(q, "q"));
+    GTN_CHECK(check_tensor(k, "k"));
+    GTN_CHECK(check_tensor(v, "v"));
+    GTN_CHECK(check_tensor(q_out, "q_out"));
+    GTN_CHECK(paged_int_arg(pos, 1, who, "pos"));
+    GTN_CHECK(paged_int_arg(slots, 1, who, "slots"));
+    GTN_REQUIRE(q->ndim == 2 && k->ndim == 2 && v->ndim == 2 && q_out->ndim == 2, "%s: 2-D rows", who);
+    const int rows = q->shape[0], d = a.c.d, kvd = a.c.kv_heads * d;
+    GTN_REQUIRE(q->shape[1] % d == 0, "%s: q of %d columns, d_head %d", who, q->shape[1], d);
+    GTN_REQUIRE(k->shape[0] == rows && k->shape[1] == kvd && v->shape[0] == rows && v->shape[1] == kvd,
+                "%s: k / v must be [%d, %d]", who, rows, kvd);
+    GTN_REQUIRE(q_out->shape[0] == rows && q_out->shape[1] == q->shape[1], "%s: q_out shape", who);
+    GTN_REQUIRE(pos->shape[0] == rows && slots->shape[0] == rows, "%s: pos / slots must have %d entries", who, rows);
+    GTN_REQUIRE(q->dtype == k->dtype && k->dtype == v->dtype, "%s: q, k, v dtypes differ", who);
+    GTN_REQUIRE(q->dtype == GTN_F16 || q->dtype == GTN_F32 || q->dtype == GTN_Q8, "%s: q dtype %d", who, q->dtype);
+    GTN_REQUIRE(q_out->dtype == GTN_F16 || q_out->dtype == GTN_Q8, "%s: q_out dtype %d", who, q_out->dtype);
+    const gtn_tensor* rt[] = {q, k, v, q_out};
+    for (const gtn_tensor* t : rt) {
+        GTN_REQUIRE(t->strides[1] == 1 && t->strides[0] >= t->shape[1], "%s: row strides", who);
+        GTN_REQUIRE(t->dtype != GTN_Q8 || t->strides[0] % GTN_QBLK == 0, "%s: Q8 row stride %d", who, t->strides[0]);
+        GTN_REQUIRE((uintptr_t)t->data % (t->dtype == GTN_F32 ? 4 : 2) == 0, "%s: row alignment", who);
+    }
+    const uint8_t *qb = (const uint8_t*)q->data, *ob = (const uint8_t*)q_out->data;
+    const bool same = qb == ob && q->dtype == q_out->dtype && bstride(q, 0) == bstride(q_out, 0);
+    const long qe = (long)(rows - 1) * bstride(q, 0) + row_bytes(q->dtype, q->shape[1]);
+    const long oe = (long)(rows - 1) * bstride(q_out, 0) + row_bytes(q_out->dtype, q->shape[1]);
+    GTN_REQUIRE(same || ob >= qb + qe || qb >= ob + oe, "%s: q_out overlaps q", who);
+    GTN_REQUIRE(rope_pct >= 0.0f && rope_pct <= 1.0f, "%s: rope_pct", who);
+    GTN_REQUIRE(rope_base > 0.0f && std::isfinite(rope_base), "%s: rope_base", who);
+    const void* ptrs[] = {q->data, k->data, v->data, q_out->data, pos->data, slots->data, a.c.k, a.c.v};
+    GTN_CHECK(paged_on_device(ptrs, 8, who));
+    a.q = qb;
+    a.k = (const uint8_t*)k->data;
+    a.v = (const uint8_t*)v->data;
+    a.out = (uint8_t*)q_out->data;
+    a.qs = bstride(q, 0);
+    a.ks = bstride(k, 0);
+    a.vs = bstride(v, 0);
+    a.os = bstride(q_out, 0);
+    a.pos = (const int32_t*)pos->data;
+    a.slots = (const int32_t*)slots->data;
+    a.heads = q->shape[1] / d;
+    a.sdt = q->dtype;
+    a.odt = q_out->dtype;
+    const int rd = (int)((float)d * rope_pct);
+    a.half = rd / 2;
+    a.err = device_error_word();
+    RopeFreq fr;
+    for (int j = 0; j < 64; ++j) fr.f[j] = j < a.half ? std::pow((double)rope_base, -2.0 * j / (2 * a.half)) : 0.0;
+    const cudaError_t e = d == 64 ? launch_pdl(k_paged_append<64>, dim3(rows), dim3(APP_THREADS), 0, S(stream), a, fr)
+                                  : launch_pdl(k_paged_append<128>, dim3(rows), dim3(APP_THREADS), 0, S(stream), a, fr);
+    return cuda_status(e, who);
+}
+
+}  // extern "C"

@@ -38,6 +38,11 @@ class gtn_tensor(C.Structure):
                 ("shape", C.c_int32 * 3), ("strides", C.c_int32 * 3)]
 
 
+class gtn_paged_cache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("d_head", C.c_int32), ("page_stride", C.c_int64)]
+
+
 _lib = None
 
 
@@ -73,6 +78,15 @@ def lib() -> C.CDLL:
         L.gtn_sample_topk.argtypes = [C.c_void_p, C.c_int, C.c_float, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]
         L.gtn_model_generate_topk.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_int,
                                               C.c_void_p, C.c_void_p]
+        P = C.c_void_p
+        L.gtn_paged_page_bytes.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int]
+        L.gtn_paged_page_bytes.restype = C.c_int64
+        L.gtn_paged_plan.argtypes = [P, P, P, P, C.c_int, P, P, P, P, P, P, P]
+        L.gtn_paged_append.argtypes = [P, P, P, P, P, P, P, C.c_float, C.c_float, P]
+        L.gtn_paged_attn_workspace.argtypes = [C.c_int, C.c_int]
+        L.gtn_paged_attn_workspace.restype = C.c_int64
+        L.gtn_paged_attn.argtypes = [P, P, P, P, P, P, C.c_float, C.c_int, C.c_int, C.c_int, P, C.c_int64, P]
+        L.gtn_check.argtypes = [P]
         _lib = L
     return _lib
 
@@ -127,10 +141,12 @@ def _stream(stream):
 
 @dataclass
 class GT:
-    """A gten tensor view: device buffer + dtype + logical shape (elements), contiguous rows."""
+    """A gten tensor view: device buffer + dtype + logical shape (elements), contiguous rows unless
+    ``strides`` (elements, one per dim) says otherwise."""
     buf: object
     dtype: int
     shape: tuple
+    strides: tuple | None = None
 
     def desc(self) -> gtn_tensor:
         t = gtn_tensor()
@@ -140,6 +156,8 @@ class GT:
         st = [1] * len(self.shape)
         for i in range(len(self.shape) - 2, -1, -1):
             st[i] = st[i + 1] * self.shape[i + 1]
+        if self.strides is not None:
+            st = list(self.strides)
         for i, s in enumerate(self.shape):
             t.shape[i] = s
             t.strides[i] = st[i]
@@ -202,6 +220,70 @@ def bias_add_inplace(inp: GT, bias: GT, start_pos: int = 0, stream=None):
 
 def token_embed(weight: GT, tokens: GT, out: GT, start_pos: int = 0, stream=None):
     _check(lib().gtn_token_embed(_d(weight), _d(tokens), _d(out), start_pos, _stream(stream)), "token_embed")
+
+
+# ---- paged serving operators ----------------------------------------------------------------
+class PagedCache:
+    """A paged K/V cache: two pools of ``n_pages`` pages of ``page_size`` tokens (gtn_paged_cache has the
+    page layout; ``page_bytes`` the bytes of one page). k, v: device buffers (torch tensors or pointers)."""
+
+    def __init__(self, k, v, dtype: int, n_pages: int, page_size: int, kv_heads: int, d_head: int, page_stride: int = 0):
+        self.k, self.v = k, v  # keeps the buffers alive
+        self.d_head, self.kv_heads = d_head, kv_heads
+        self._desc = gtn_paged_cache(_ptr(k), _ptr(v), dtype, n_pages, page_size, kv_heads, d_head, page_stride)
+
+    @staticmethod
+    def page_bytes(dtype: int, page_size: int, kv_heads: int, d_head: int) -> int:
+        n = int(lib().gtn_paged_page_bytes(dtype, page_size, kv_heads, d_head))
+        if n == 0:
+            raise GtenError(f"no paged cache of dtype {dtype}, page_size {page_size}, kv_heads {kv_heads}, d_head {d_head}")
+        return n
+
+    def desc(self) -> gtn_paged_cache:
+        return self._desc
+
+
+def paged_plan(ctx_lens: GT, new_lens: GT, free_pages: GT, n_free: GT, page_size: int, block_table: GT, q_start: GT,
+               kv_lens: GT, pos: GT, slots: GT, n_used: GT, stream=None):
+    """Block tables, slot map and positions of one step from the requests' lengths (all int32, on the
+    device). A request that was not granted has kv_lens 0 and slots -1."""
+    _check(lib().gtn_paged_plan(_d(ctx_lens), _d(new_lens), _d(free_pages), _d(n_free), page_size, _d(block_table),
+                                _d(q_start), _d(kv_lens), _d(pos), _d(slots), _d(n_used), _stream(stream)), "paged_plan")
+
+
+def paged_append(q: GT, k: GT, v: GT, pos: GT, slots: GT, cache: PagedCache, q_out: GT, rope_pct: float = 1.0,
+                 rope_base: float = 10000.0, stream=None):
+    """Rotary at each row's own position, K and V rows into their pages, rotated queries to q_out."""
+    _check(lib().gtn_paged_append(_d(q), _d(k), _d(v), _d(pos), _d(slots), _d(cache), _d(q_out), rope_pct, rope_base,
+                                  _stream(stream)), "paged_append")
+
+
+def paged_attn_workspace(heads: int, d_head: int) -> int:
+    """Bytes of scratch that one paged_attn call needs on the current device."""
+    return int(lib().gtn_paged_attn_workspace(heads, d_head))
+
+
+def paged_attn(q: GT, cache: PagedCache, block_table: GT, q_start: GT, kv_lens: GT, out: GT, scale: float = 0.0,
+               window: int = 0, n_sink: int = 0, max_new: int = 0, workspace=None, stream=None):
+    """Attention of the new tokens over the pages (causal; window > 0: the last ``window`` keys and the
+    first ``n_sink``). ``workspace``: a device buffer (uint8 tensor) of paged_attn_workspace bytes; without
+    one, a tensor is taken from torch's allocator for this call, on the call's stream."""
+    d = cache.d_head
+    if workspace is None:
+        import torch
+        st = stream
+        if st is not None and not hasattr(st, "cuda_stream"):
+            st = torch.cuda.ExternalStream(int(st))
+        n = paged_attn_workspace(max(1, q.shape[-1] // d), d)
+        with torch.cuda.stream(st):
+            workspace = torch.empty(n, dtype=torch.uint8, device="cuda")
+    _check(lib().gtn_paged_attn(_d(q), _d(cache), _d(block_table), _d(q_start), _d(kv_lens), _d(out), scale, window,
+                                n_sink, max_new, _ptr(workspace), workspace.numel(), _stream(stream)), "paged_attn")
+
+
+def check(stream=None) -> None:
+    """Waits for the stream; raises if a kernel on the current device flagged an error since the last check."""
+    _check(lib().gtn_check(_stream(stream)), "check")
 
 
 # ---- quantization -------------------------------------------------------------------------
