@@ -158,7 +158,7 @@ cudaError_t matmul_f32(const uint8_t* X, long xs, int xdt, int M, const uint8_t*
     return matmul_tma(X, xs, M, W, ws, wdt, N, K, Y, ldy, st, tc);
 }
 
-static int sm_count() {
+int sm_count() {
     static thread_local int dev_cached = -1, n = 148;
     int dev = 0;
     cudaGetDevice(&dev);

@@ -9,6 +9,9 @@ inline int cuda_status(cudaError_t e, const char* what) {
     return fail(e == cudaErrorMemoryAllocation ? GTN_ERR_OOM : GTN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// Multiprocessors of the current device.
+int sm_count();
+
 // Reads and clears the device error word; the stream whose kernels are meant has been waited for.
 inline int check_dev_err() {
     const unsigned int v = take_device_error();

@@ -1,82 +1,33 @@
 // gtn_paged_attn: attention of new tokens over a paged cache (causal; or a sliding window and first
 // tokens that stay visible), GQA, ragged requests.
-#include "paged.cuh"
+#include "paged_decode.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 namespace gtn {
 
-struct PagedAttnArgs {
-    const uint8_t* q;
-    uint8_t* out;
-    long qs, os;  // row strides, bytes
-    int io;       // dtype of q and out
-    PagedCache c;
-    const int32_t *table, *q_start, *kv_lens;
-    long table_stride;
-    int n_req, rows, heads, group, max_pages, window, n_sink;
-    float scale_log2;  // scale * log2(e): the softmax runs in base 2
-    unsigned int* err;
-};
+// CTAs of the decode kernel: as many as are resident at once.
+static int decode_ctas(int d) { return sm_count() * (d == 64 ? 3 : 2); }
 
-// One warp per (row, query head), the keys in order with a running maximum and sum; lane l holds elements
-// l, l + 32, ... of the head.
-template <int D>
-static __global__ void __launch_bounds__(128) k_paged_attn_rows(PagedAttnArgs a) {
-    constexpr int NB = D / GTN_QBLK;
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long u = (long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int t = (int)(u / a.heads), h = (int)(u % a.heads), g = h / a.group;
-    if (t >= a.rows || t >= a.q_start[a.n_req]) return;
-    int lo = 0, hi = a.n_req - 1;  // the first b with q_start[b + 1] > t
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_start[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
-    }
-    int kv = a.kv_lens[lo];
-    if (kv < 0 || kv > (a.max_pages << a.c.ps_shift)) {
-        kv = 0;
-        if (lane == 0) atomicOr(a.err, GTN_DEVERR_PAGE);
-    }
-    const int p = kv - (a.q_start[lo + 1] - t);
-    const long hb = row_bytes(a.io, D);
-    float q[NB], o[NB], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        q[i] = load_elem(a.q + (long)t * a.qs + h * hb, a.io, i * GTN_QBLK + lane);
-        o[i] = 0.0f;
-    }
-    for (int j = 0; j <= p; ++j) {
-        if (a.window > 0 && j <= p - a.window && j >= a.n_sink) {
-            j = max(j, p - a.window);
-            continue;
-        }
-        const int page = a.table[lo * a.table_stride + (j >> a.c.ps_shift)];
-        if (page < 0 || page >= a.c.n_pages) {
-            if (lane == 0) atomicOr(a.err, GTN_DEVERR_PAGE);
-            continue;
-        }
-        const int r = j & (a.c.ps - 1);
-        const uint8_t* kp = a.c.k + (long)page * a.c.page_stride;
-        const uint8_t* vp = a.c.v + (long)page * a.c.page_stride;
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) s = fmaf(q[i], paged_elem(a.c, kp, g, r, i * GTN_QBLK + lane), s);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= a.scale_log2;
-        const float mn = fmaxf(m, s);
-        const float f = exp2f(m - mn), e = exp2f(s - mn);
-        l = fmaf(l, f, e);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) o[i] = fmaf(o[i], f, e * paged_elem(a.c, vp, g, r, i * GTN_QBLK + lane));
-        m = mn;
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-        store_row_elem(a.out + (long)t * a.os + h * hb, a.io, i, lane, D, l > 0.0f || l != l ? o[i] / l : 0.0f);
+static int64_t decode_part_floats(int d) { return 2L * decode_ctas(d) * 16 * (d + 2); }
+
+template <int DT, int D, int ROWS>
+static cudaError_t launch_decode(const PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
+    const int ctas = decode_ctas(D);
+    const size_t smem = paged_decode_smem<D, ROWS>();
+    cudaError_t e = ensure_smem(k_paged_decode<DT, D, ROWS>, smem);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(k_paged_decode<DT, D, ROWS>, dim3(ctas), dim3(PD_THREADS), smem, st, a, p);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_paged_join<ROWS, PD_KEYS, D>, dim3(ctas - 1, ROWS / 4), dim3(128), 0, st, a, p, ctas);
+}
+
+template <int ROWS>
+static cudaError_t decode(const PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
+    if (a.c.d == 64)
+        return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 64, ROWS>(a, p, st) : launch_decode<GTN_Q8, 64, ROWS>(a, p, st);
+    return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 128, ROWS>(a, p, st) : launch_decode<GTN_Q8, 128, ROWS>(a, p, st);
 }
 
 }  // namespace gtn
@@ -87,7 +38,7 @@ extern "C" {
 
 int64_t gtn_paged_attn_workspace(int heads, int d_head) {
     if (heads < 1 || (d_head != 64 && d_head != 128)) return 0;
-    return 16;
+    return decode_part_floats(d_head) * (int64_t)sizeof(float);
 }
 
 int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_tensor* block_table,
@@ -145,14 +96,17 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     a.rows = q->shape[0];
     a.heads = heads;
     a.group = heads / a.c.kv_heads;
-    a.max_pages = block_table->shape[1];
+    a.cap = (long)block_table->shape[1] * a.c.ps;
     a.window = window;
     a.n_sink = n_sink;
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)d)) * 1.4426950408889634f;
+    a.part = (float*)workspace;
     a.err = device_error_word();
-    const unsigned grid = (unsigned)(((long)a.rows * heads + 3) / 4);
-    const cudaError_t e = d == 64 ? launch_pdl(k_paged_attn_rows<64>, dim3(grid), dim3(128), 0, S(stream), a)
-                                  : launch_pdl(k_paged_attn_rows<128>, dim3(grid), dim3(128), 0, S(stream), a);
+    PagedPick p;
+    p.cut = 0x7fffffff;
+    p.below = true;
+    const long most = max_new > 0 ? (long)max_new * a.group : 16;
+    const cudaError_t e = most <= 8 ? decode<8>(a, p, S(stream)) : decode<16>(a, p, S(stream));
     return cuda_status(e, who);
 }
 

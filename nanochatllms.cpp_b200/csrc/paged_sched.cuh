@@ -1,0 +1,287 @@
+// Work distribution of the paged attention kernels.
+//
+// An item is one tile of ROWS query rows (token-major, the `group` query heads of one kv head per token)
+// of one request and kv head; a unit is KEYS consecutive keys of an item. The units of all items form one
+// line, ordered by request, kv head, row tile and key, and CTA c takes units [c * share, (c + 1) * share)
+// of it, share = ceil(units / CTAs): every CTA does the same work whatever the lengths are, and a single long
+// request spreads over the whole GPU. An item that lies in one CTA's range is finished there; of an item
+// that crosses a border, each CTA leaves its unnormalised sums in its own scratch slots (slot 0: the item
+// began before the range; slot 1: it begins in it), and k_paged_join adds them up in CTA order.
+// Everything is computed from the lengths on the device, the same in every CTA and kernel of a call.
+#pragma once
+#include "paged.cuh"
+
+namespace gtn {
+
+struct PagedAttnArgs {
+    const uint8_t* q;
+    uint8_t* out;
+    long qs, os;  // row strides, bytes
+    int io;       // dtype of q and out
+    PagedCache c;
+    const int32_t *table, *q_start, *kv_lens;
+    long table_stride;
+    int n_req, rows, heads, group, window, n_sink;
+    long cap;          // keys that a row of the table can hold
+    float scale_log2;  // scale * log2(e): the softmax runs in base 2
+    float* part;       // scratch slots: [CTA][2] of ROWS * (D + 2) floats
+    unsigned int* err;
+};
+
+// A request's rows as the kernels take them: row i of [0, n) sits at position base + i; lengths that the
+// table or the row tensor cannot hold are flagged and cut.
+struct PagedReq {
+    int first;  // row of token 0 in q and out
+    int n;      // tokens
+    int base;   // position of token 0 (negative: tokens before the first key see nothing)
+};
+__device__ __forceinline__ PagedReq paged_req(const PagedAttnArgs& a, int b, bool flag) {
+    const int s = a.q_start[b], e = a.q_start[b + 1];
+    int kv = a.kv_lens[b];
+    bool bad = kv < 0 || kv > a.cap || s < 0 || e < s;
+    if (kv < 0 || kv > a.cap) kv = 0;
+    PagedReq r;
+    r.first = s;
+    r.n = s < 0 || s >= a.rows || e <= s ? 0 : min(e, a.rows) - s;
+    r.base = e > s ? kv - (e - s) : 0;
+    if (bad && flag) atomicOr(a.err, GTN_DEVERR_PAGE);
+    return r;
+}
+
+// The keys of one row tile: sink units [0, ns), then units w0, w0 + 1, ...
+struct PagedTile {
+    int plo, phi;  // positions of the tile's first and last token
+    int ns, w0, units;
+};
+template <int ROWS, int KEYS>
+__device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs& a, const PagedReq& r, int tile) {
+    PagedTile t;
+    t.plo = r.base + tile * ROWS / a.group;
+    t.phi = r.base + min(r.n - 1, (tile * ROWS + ROWS - 1) / a.group);
+    t.ns = t.w0 = 0;
+    t.units = 1;  // a tile that sees nothing still writes its zeros
+    if (t.phi >= 0) {
+        const int lo = a.window > 0 ? max(0, t.plo - a.window + 1) : 0;
+        t.w0 = lo / KEYS;
+        t.ns = min((min(a.n_sink, t.phi + 1) + KEYS - 1) / KEYS, t.w0);
+        t.units = t.ns + t.phi / KEYS - t.w0 + 1;
+    }
+    return t;
+}
+template <int KEYS>
+__device__ __forceinline__ int paged_unit_key(const PagedTile& t, int u) {
+    return (u < t.ns ? u : t.w0 + u - t.ns) * KEYS;
+}
+
+// Which requests a kernel takes: those of at most `cut` rows per kv head, or the others.
+struct PagedPick {
+    int cut;
+    bool below;
+};
+template <int ROWS>
+__device__ __forceinline__ int paged_tiles(const PagedAttnArgs& a, const PagedPick& p, const PagedReq& r) {
+    const int m = r.n * a.group;
+    return r.n > 0 && (m <= p.cut) == p.below ? (m + ROWS - 1) / ROWS : 0;
+}
+template <int ROWS, int KEYS>
+__device__ __forceinline__ long long paged_req_units(const PagedAttnArgs& a, const PagedPick& p, const PagedReq& r) {
+    const int nt = paged_tiles<ROWS>(a, p, r);
+    long long s = 0;
+    for (int t = 0; t < nt; ++t) s += paged_tile<ROWS, KEYS>(a, r, t).units;
+    return s;
+}
+
+// A position on the line of units: item (b, h, tile), unit u of it, the item's first position.
+struct PagedPos {
+    int b, h, tile, u;
+    PagedReq r;
+    PagedTile t;
+    long long start;
+};
+struct PagedSched {
+    long long total, share;
+    PagedPos pos;
+};
+struct PagedSchedSmem {
+    long long warp[33];
+    PagedPos pos;
+};
+
+// Total units, the share of one of `ctas` CTAs, and the item at position `cta` * share (its b is -1 at
+// or past the end). Called by all THREADS threads of the CTA; ends with a barrier.
+template <int ROWS, int KEYS, int THREADS>
+__device__ __forceinline__ PagedSched paged_sched(const PagedAttnArgs& a, const PagedPick& p, int ctas, int cta,
+                                                  bool flag, PagedSchedSmem& sm) {
+    constexpr int NW = THREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (a.n_req + THREADS - 1) / THREADS, b0 = min(a.n_req, tid * per), b1 = min(a.n_req, b0 + per);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += paged_req_units<ROWS, KEYS>(a, p, paged_req(a, b, flag)) * a.c.kv_heads;
+    long long s = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+    }
+    if (lane == 31) sm.warp[warp] = s;
+    if (tid == 0) sm.pos.b = -1;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        before += w < warp ? sm.warp[w] : 0;
+        total += sm.warp[w];
+    }
+    before += s - mine;
+    PagedSched r;
+    r.total = total;
+    r.share = (total + ctas - 1) / ctas;
+    const long long at = r.share * cta;
+    if (at < total && at >= before && at < before + mine) {
+        long long left = at - before, start = before;
+        for (int b = b0; b < b1; ++b) {
+            const PagedReq q = paged_req(a, b, false);
+            const long long one = paged_req_units<ROWS, KEYS>(a, p, q), all = one * a.c.kv_heads;
+            if (left >= all) {
+                left -= all;
+                start += all;
+                continue;
+            }
+            PagedPos x;
+            x.b = b;
+            x.r = q;
+            x.h = (int)(left / one);
+            left -= x.h * one;
+            start += x.h * one;
+            for (x.tile = 0;; ++x.tile) {
+                x.t = paged_tile<ROWS, KEYS>(a, q, x.tile);
+                if (left < x.t.units) break;
+                left -= x.t.units;
+                start += x.t.units;
+            }
+            x.u = (int)left;
+            x.start = start;
+            sm.pos = x;
+            break;
+        }
+    }
+    __syncthreads();
+    r.pos = sm.pos;
+    return r;
+}
+
+// The next item on the line (b >= n_req behind the last one).
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void paged_next(const PagedAttnArgs& a, const PagedPick& p, PagedPos& x) {
+    x.start += x.t.units;
+    x.u = 0;
+    if (++x.tile < paged_tiles<ROWS>(a, p, x.r)) {
+        x.t = paged_tile<ROWS, KEYS>(a, x.r, x.tile);
+        return;
+    }
+    x.tile = 0;
+    if (++x.h == a.c.kv_heads) {
+        x.h = 0;
+        while (++x.b < a.n_req) {
+            x.r = paged_req(a, x.b, false);
+            if (paged_tiles<ROWS>(a, p, x.r) > 0) break;
+        }
+        if (x.b >= a.n_req) return;
+    }
+    x.t = paged_tile<ROWS, KEYS>(a, x.r, 0);
+}
+
+// ---- scratch slots ------------------------------------------------------------------------------
+// One slot: ROWS * D sums, ROWS running maxima, ROWS sums of weights.
+template <int ROWS, int D>
+__host__ __device__ constexpr long paged_slot() {
+    return (long)ROWS * (D + 2);
+}
+
+// Writes 32 / T consecutive outputs per lane, T lanes per 32-element block: columns [c0, c0 + N) of one
+// head's row in dtype io. Lanes of a block are adjacent; every lane of the warp takes part.
+template <int N>
+__device__ __forceinline__ void paged_store(uint8_t* head, int io, int c0, const float (&y)[N], bool live) {
+    constexpr int T = GTN_QBLK / N;
+    static_assert(GTN_QBLK % N == 0 && N % 4 == 0, "whole blocks");
+    if (io == GTN_F16) {
+        if (!live) return;
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) w[i] = (uint32_t)f2h(y[2 * i]) | ((uint32_t)f2h(y[2 * i + 1]) << 16);
+        uint2* dst = reinterpret_cast<uint2*>(head + 2 * c0);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) dst[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+        return;
+    }
+    // the activation quantizer (warp_quant_block): absmax without NaN, delta, 1 / delta unrounded, roundf
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(y[i]));
+#pragma unroll
+    for (int o = 1; o < T; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (!live) return;
+    const float delta = m / 127.0f, inv = delta != 0.0f ? 1.0f / delta : 0.0f;
+    uint8_t* blk = head + c0 / GTN_QBLK * GTN_Q8_BYTES;
+    if (c0 % GTN_QBLK == 0) *reinterpret_cast<uint16_t*>(blk) = f2h(delta);
+    uint16_t* dst = reinterpret_cast<uint16_t*>(blk + 2 + c0 % GTN_QBLK);  // blocks start at even addresses
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const uint32_t lo = (uint8_t)(int8_t)roundf(y[2 * i] * inv), hi = (uint8_t)(int8_t)roundf(y[2 * i + 1] * inv);
+        dst[i] = (uint16_t)(lo | (hi << 8));
+    }
+}
+
+// Address of (row of the item) in q / out: token, head.
+__device__ __forceinline__ long paged_row_at(const PagedAttnArgs& a, const PagedPos& x, int row, int rows_per_tile,
+                                             long stride, long head_bytes) {
+    const int m = x.tile * rows_per_tile + row, tok = m / a.group;
+    return (long)(x.r.first + tok) * stride + (long)(x.h * a.group + m - tok * a.group) * head_bytes;
+}
+
+// Joins the items that cross CTA borders: CTA (c - 1, y) takes the item over border c if that is the first
+// border in it, one warp per row.
+template <int ROWS, int KEYS, int D>
+__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, PagedPick p, int ctas) {
+    __shared__ PagedSchedSmem sm;
+    pdl_wait();
+    const int c = blockIdx.x + 1;
+    const PagedSched s = paged_sched<ROWS, KEYS, 128>(a, p, ctas, c, false, sm);
+    const PagedPos& x = s.pos;
+    if (x.b < 0 || x.u == 0 || x.start < (c - 1) * s.share) return;
+    const int last = (int)((x.start + x.t.units - 1) / s.share);
+    const int lane = threadIdx.x & 31, row = blockIdx.y * 4 + (threadIdx.x >> 5);
+    const bool live = x.tile * ROWS + row < x.r.n * a.group;
+    constexpr int N = D / 32 < 4 ? 4 : D / 32, LANES = D / N;  // columns per lane, lanes that hold some
+    if (!live) return;
+    const long S = paged_slot<ROWS, D>();
+    float m = -INFINITY;
+    for (int i = c - 1 + lane; i <= last; i += 32) m = fmaxf(m, a.part[(2L * i + (i == c - 1)) * S + ROWS * D + row]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float mm = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, y[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) y[j] = 0.0f;
+    const int c0 = (lane % LANES) * N;
+#pragma unroll 4
+    for (int i = c - 1; i <= last; ++i) {
+        const float* ps = a.part + (2L * i + (i == c - 1)) * S;
+        const float f = exp2f(ps[ROWS * D + row] - mm);
+        l = fmaf(ps[ROWS * (D + 1) + row], f, l);
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(ps + row * D + c0 + j);
+            y[j] = fmaf(v.x, f, y[j]);
+            y[j + 1] = fmaf(v.y, f, y[j + 1]);
+            y[j + 2] = fmaf(v.z, f, y[j + 2]);
+            y[j + 3] = fmaf(v.w, f, y[j + 3]);
+        }
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) y[j] = l != 0.0f ? y[j] * inv : 0.0f;
+    paged_store<N>(a.out + paged_row_at(a, x, row, ROWS, a.os, row_bytes(a.io, D)), a.io, c0, y, lane < LANES);
+}
+
+}  // namespace gtn
