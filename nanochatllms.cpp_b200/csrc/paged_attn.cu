@@ -7,27 +7,31 @@
 
 namespace gtn {
 
-// CTAs of the decode kernel: as many as are resident at once.
-static int decode_ctas(int d) { return sm_count() * (d == 64 ? 3 : 2); }
-
-static int64_t decode_part_floats(int d) { return 2L * decode_ctas(d) * 16 * (d + 2); }
+// Workers of the decode kernel: the warps that are resident at once.
+constexpr int DECODE_CTAS = 3;  // per SM, at most
+static int64_t decode_ws_bytes(int d) {
+    const int64_t workers = (int64_t)sm_count() * DECODE_CTAS * PD_WARPS;
+    return workers * (2 * 16 * (d + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(PagedJoin) + 16);
+}
 
 template <int DT, int D, int ROWS>
-static cudaError_t launch_decode(const PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
-    const int ctas = decode_ctas(D);
-    const size_t smem = paged_decode_smem<D, ROWS>();
-    cudaError_t e = ensure_smem(k_paged_decode<DT, D, ROWS>, smem);
+static cudaError_t launch_decode(PagedAttnArgs a, const PagedPick& p, int most_rows, cudaStream_t st) {
+    using C = DecodeCfg<DT, D, ROWS>;
+    static_assert(C::OCC <= DECODE_CTAS, "workspace");
+    const int ctas = sm_count() * C::OCC, workers = ctas * PD_WARPS;
+    a.join = reinterpret_cast<PagedJoin*>(a.part + (long)workers * 2 * paged_slot<ROWS, D>());
+    cudaError_t e = ensure_smem(k_paged_decode<DT, D, ROWS>, C::SMEM);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(k_paged_decode<DT, D, ROWS>, dim3(ctas), dim3(PD_THREADS), smem, st, a, p);
+    e = launch_pdl(k_paged_decode<DT, D, ROWS>, dim3(ctas), dim3(32 * PD_WARPS), C::SMEM, st, a, p);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_join<ROWS, PD_KEYS, D>, dim3(ctas - 1, ROWS / 4), dim3(128), 0, st, a, p, ctas);
+    return launch_pdl(k_paged_join<ROWS, D>, dim3((workers + 3) / 4, most_rows), dim3(128), 0, st, a, workers);
 }
 
 template <int ROWS>
-static cudaError_t decode(const PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
+static cudaError_t decode(const PagedAttnArgs& a, const PagedPick& p, int most, cudaStream_t st) {
     if (a.c.d == 64)
-        return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 64, ROWS>(a, p, st) : launch_decode<GTN_Q8, 64, ROWS>(a, p, st);
-    return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 128, ROWS>(a, p, st) : launch_decode<GTN_Q8, 128, ROWS>(a, p, st);
+        return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 64, ROWS>(a, p, most, st) : launch_decode<GTN_Q8, 64, ROWS>(a, p, most, st);
+    return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 128, ROWS>(a, p, most, st) : launch_decode<GTN_Q8, 128, ROWS>(a, p, most, st);
 }
 
 }  // namespace gtn
@@ -38,7 +42,7 @@ extern "C" {
 
 int64_t gtn_paged_attn_workspace(int heads, int d_head) {
     if (heads < 1 || (d_head != 64 && d_head != 128)) return 0;
-    return decode_part_floats(d_head) * (int64_t)sizeof(float);
+    return decode_ws_bytes(d_head);
 }
 
 int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_tensor* block_table,
@@ -106,7 +110,7 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     p.cut = 0x7fffffff;
     p.below = true;
     const long most = max_new > 0 ? (long)max_new * a.group : 16;
-    const cudaError_t e = most <= 8 ? decode<8>(a, p, S(stream)) : decode<16>(a, p, S(stream));
+    const cudaError_t e = most <= 8 ? decode<8>(a, p, (int)most, S(stream)) : decode<16>(a, p, 16, S(stream));
     return cuda_status(e, who);
 }
 

@@ -2,16 +2,23 @@
 //
 // An item is one tile of ROWS query rows (token-major, the `group` query heads of one kv head per token)
 // of one request and kv head; a unit is KEYS consecutive keys of an item. The units of all items form one
-// line, ordered by request, kv head, row tile and key, and CTA c takes units [c * share, (c + 1) * share)
-// of it, share = ceil(units / CTAs): every CTA does the same work whatever the lengths are, and a single long
-// request spreads over the whole GPU. An item that lies in one CTA's range is finished there; of an item
-// that crosses a border, each CTA leaves its unnormalised sums in its own scratch slots (slot 0: the item
-// began before the range; slot 1: it begins in it), and k_paged_join adds them up in CTA order.
-// Everything is computed from the lengths on the device, the same in every CTA and kernel of a call.
+// line, ordered by request, kv head, row tile and key, and worker c (a warp or a CTA) takes units
+// [c * share, (c + 1) * share) of it, share = ceil(units / workers): every worker does the same work whatever
+// the lengths are, and a single long request spreads over the whole GPU. An item that lies in one worker's
+// range is finished there; of an item that crosses a border, each worker leaves its unnormalised sums in
+// its own scratch slots (slot 0: the item began before the range; slot 1: it begins in it), and
+// k_paged_join adds them up in the order of the workers. Everything is computed from the lengths on the
+// device, the same for every worker of a call.
 #pragma once
 #include "paged.cuh"
 
 namespace gtn {
+
+// What a worker says of the item that begins in its range and goes on behind it.
+struct PagedJoin {
+    int last;                   // the last worker of the item; -1: there is no such item
+    int first, h, tile, nrow;   // the item: first row of its request, kv head, row tile, query rows
+};
 
 struct PagedAttnArgs {
     const uint8_t* q;
@@ -24,7 +31,8 @@ struct PagedAttnArgs {
     int n_req, rows, heads, group, window, n_sink;
     long cap;          // keys that a row of the table can hold
     float scale_log2;  // scale * log2(e): the softmax runs in base 2
-    float* part;       // scratch slots: [CTA][2] of ROWS * (D + 2) floats
+    float* part;       // scratch slots: [worker][2] of ROWS * (D + 2) floats
+    PagedJoin* join;   // [worker]
     unsigned int* err;
 };
 
@@ -98,20 +106,18 @@ struct PagedPos {
     PagedTile t;
     long long start;
 };
-struct PagedSched {
-    long long total, share;
-    PagedPos pos;
-};
+template <int W>
 struct PagedSchedSmem {
     long long warp[33];
-    PagedPos pos;
+    PagedPos pos[W];
 };
 
-// Total units, the share of one of `ctas` CTAs, and the item at position `cta` * share (its b is -1 at
-// or past the end). Called by all THREADS threads of the CTA; ends with a barrier.
-template <int ROWS, int KEYS, int THREADS>
-__device__ __forceinline__ PagedSched paged_sched(const PagedAttnArgs& a, const PagedPick& p, int ctas, int cta,
-                                                  bool flag, PagedSchedSmem& sm) {
+// Total units (returned), and in sm.pos[i] the item at position (first + i) * share of workers first ..
+// first + W - 1 of `workers` (its b is -1 at or past the end). Called by all THREADS threads of the CTA; ends
+// with a barrier.
+template <int ROWS, int KEYS, int THREADS, int W>
+__device__ __forceinline__ long long paged_sched(const PagedAttnArgs& a, const PagedPick& p, int workers, int first,
+                                                 bool flag, PagedSchedSmem<W>& sm) {
     constexpr int NW = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.n_req + THREADS - 1) / THREADS, b0 = min(a.n_req, tid * per), b1 = min(a.n_req, b0 + per);
@@ -124,7 +130,7 @@ __device__ __forceinline__ PagedSched paged_sched(const PagedAttnArgs& a, const 
         if (lane >= o) s += y;
     }
     if (lane == 31) sm.warp[warp] = s;
-    if (tid == 0) sm.pos.b = -1;
+    if (tid < W) sm.pos[tid].b = -1;
     __syncthreads();
     long long before = 0, total = 0;
 #pragma unroll
@@ -133,11 +139,10 @@ __device__ __forceinline__ PagedSched paged_sched(const PagedAttnArgs& a, const 
         total += sm.warp[w];
     }
     before += s - mine;
-    PagedSched r;
-    r.total = total;
-    r.share = (total + ctas - 1) / ctas;
-    const long long at = r.share * cta;
-    if (at < total && at >= before && at < before + mine) {
+    const long long share = (total + workers - 1) / workers;
+    for (int i = 0; i < W; ++i) {
+        const long long at = share * (first + i);
+        if (at >= total || at < before || at >= before + mine) continue;
         long long left = at - before, start = before;
         for (int b = b0; b < b1; ++b) {
             const PagedReq q = paged_req(a, b, false);
@@ -161,13 +166,12 @@ __device__ __forceinline__ PagedSched paged_sched(const PagedAttnArgs& a, const 
             }
             x.u = (int)left;
             x.start = start;
-            sm.pos = x;
+            sm.pos[i] = x;
             break;
         }
     }
     __syncthreads();
-    r.pos = sm.pos;
-    return r;
+    return total;
 }
 
 // The next item on the line (b >= n_req behind the last one).
@@ -198,8 +202,8 @@ __host__ __device__ constexpr long paged_slot() {
     return (long)ROWS * (D + 2);
 }
 
-// Writes 32 / T consecutive outputs per lane, T lanes per 32-element block: columns [c0, c0 + N) of one
-// head's row in dtype io. Lanes of a block are adjacent; every lane of the warp takes part.
+// Writes columns [c0, c0 + N) of one head's row in dtype io, 32 / N adjacent lanes per 32-element block;
+// every lane of the warp takes part, those with `live` write.
 template <int N>
 __device__ __forceinline__ void paged_store(uint8_t* head, int io, int c0, const float (&y)[N], bool live) {
     constexpr int T = GTN_QBLK / N;
@@ -232,56 +236,56 @@ __device__ __forceinline__ void paged_store(uint8_t* head, int io, int c0, const
     }
 }
 
-// Address of (row of the item) in q / out: token, head.
-__device__ __forceinline__ long paged_row_at(const PagedAttnArgs& a, const PagedPos& x, int row, int rows_per_tile,
+// Offset of an item's row in q or out: token, head.
+__device__ __forceinline__ long paged_row_at(const PagedAttnArgs& a, int first, int h, int tile, int row, int rows_per_tile,
                                              long stride, long head_bytes) {
-    const int m = x.tile * rows_per_tile + row, tok = m / a.group;
-    return (long)(x.r.first + tok) * stride + (long)(x.h * a.group + m - tok * a.group) * head_bytes;
+    const int m = tile * rows_per_tile + row, tok = m / a.group;
+    return (long)(first + tok) * stride + (long)(h * a.group + m - tok * a.group) * head_bytes;
 }
 
-// Joins the items that cross CTA borders: CTA (c - 1, y) takes the item over border c if that is the first
-// border in it, one warp per row.
-template <int ROWS, int KEYS, int D>
-__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, PagedPick p, int ctas) {
-    __shared__ PagedSchedSmem sm;
+// Joins the items that cross borders: warp (worker w, row y, y + gridDim.y, ...) the one that begins in w's range.
+template <int ROWS, int D>
+__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, int workers) {
     pdl_wait();
-    const int c = blockIdx.x + 1;
-    const PagedSched s = paged_sched<ROWS, KEYS, 128>(a, p, ctas, c, false, sm);
-    const PagedPos& x = s.pos;
-    if (x.b < 0 || x.u == 0 || x.start < (c - 1) * s.share) return;
-    const int last = (int)((x.start + x.t.units - 1) / s.share);
-    const int lane = threadIdx.x & 31, row = blockIdx.y * 4 + (threadIdx.x >> 5);
-    const bool live = x.tile * ROWS + row < x.r.n * a.group;
-    constexpr int N = D / 32 < 4 ? 4 : D / 32, LANES = D / N;  // columns per lane, lanes that hold some
-    if (!live) return;
+    const int lane = threadIdx.x & 31, w = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (w >= workers) return;
+    const PagedJoin x = a.join[w];
+    if (x.last < 0) return;
+    constexpr int LANES = D / 4, WAYS = D == 64 ? 2 : 1;  // four columns per lane; parts taken side by side
     const long S = paged_slot<ROWS, D>();
-    float m = -INFINITY;
-    for (int i = c - 1 + lane; i <= last; i += 32) m = fmaxf(m, a.part[(2L * i + (i == c - 1)) * S + ROWS * D + row]);
+    const float* part = a.part + 2L * w * S;
+    const int n = x.last - w + 1;  // part 0: slot 1 of worker w; part i: slot 0 of worker w + i
+    auto slot = [&](int i) { return part + (i == 0 ? S : 2L * i * S); };
+    for (int row = blockIdx.y; row < x.nrow; row += gridDim.y) {
+        float m = -INFINITY;
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, slot(i)[ROWS * D + row]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float mm = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, y[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) y[j] = 0.0f;
-    const int c0 = (lane % LANES) * N;
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float mm = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int c0 = lane % LANES * 4;
 #pragma unroll 4
-    for (int i = c - 1; i <= last; ++i) {
-        const float* ps = a.part + (2L * i + (i == c - 1)) * S;
-        const float f = exp2f(ps[ROWS * D + row] - mm);
-        l = fmaf(ps[ROWS * (D + 1) + row], f, l);
-#pragma unroll
-        for (int j = 0; j < N; j += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(ps + row * D + c0 + j);
-            y[j] = fmaf(v.x, f, y[j]);
-            y[j + 1] = fmaf(v.y, f, y[j + 1]);
-            y[j + 2] = fmaf(v.z, f, y[j + 2]);
-            y[j + 3] = fmaf(v.w, f, y[j + 3]);
+        for (int i = lane / LANES; i < n; i += WAYS) {
+            const float* ps = slot(i);
+            const float f = exp2f(ps[ROWS * D + row] - mm);
+            const float4 v = *reinterpret_cast<const float4*>(ps + row * D + c0);
+            l = fmaf(ps[ROWS * (D + 1) + row], f, l);
+            y[0] = fmaf(v.x, f, y[0]);
+            y[1] = fmaf(v.y, f, y[1]);
+            y[2] = fmaf(v.z, f, y[2]);
+            y[3] = fmaf(v.w, f, y[3]);
         }
-    }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        if (WAYS == 2) {
+            l += __shfl_xor_sync(0xffffffffu, l, 16);
 #pragma unroll
-    for (int j = 0; j < N; ++j) y[j] = l != 0.0f ? y[j] * inv : 0.0f;
-    paged_store<N>(a.out + paged_row_at(a, x, row, ROWS, a.os, row_bytes(a.io, D)), a.io, c0, y, lane < LANES);
+            for (int j = 0; j < 4; ++j) y[j] += __shfl_xor_sync(0xffffffffu, y[j], 16);
+        }
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = l != 0.0f ? y[j] * inv : 0.0f;
+        paged_store<4>(a.out + paged_row_at(a, x.first, x.h, x.tile, row, ROWS, a.os, row_bytes(a.io, D)), a.io, c0, y,
+                       lane < LANES);
+    }
 }
 
 }  // namespace gtn
