@@ -349,10 +349,7 @@ static cudaError_t cc_gemm(const uint8_t* X, long xs, int M, const uint8_t* W, l
 
 // ---- tensor-core GEMM (k_gemm_tc) -----------------------------------------------------------
 // cuTensorMapEncodeTiled, reached through the runtime's driver entry point.
-typedef CUresult (*TmapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static TmapEncodeFn tmap_encode_fn() {
+TmapEncodeFn tmap_encode_fn() {
     static TmapEncodeFn fn = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {

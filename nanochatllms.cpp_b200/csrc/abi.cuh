@@ -9,6 +9,12 @@ inline int cuda_status(cudaError_t e, const char* what) {
     return fail(e == cudaErrorMemoryAllocation ? GTN_ERR_OOM : GTN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// cuTensorMapEncodeTiled, reached through the runtime's driver entry point (nullptr: not available).
+typedef CUresult (*TmapEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+TmapEncodeFn tmap_encode_fn();
+
 // Multiprocessors of the current device.
 int sm_count();
 

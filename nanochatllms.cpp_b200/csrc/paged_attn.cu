@@ -1,17 +1,21 @@
 // gtn_paged_attn: attention of new tokens over a paged cache (causal; or a sliding window and first
 // tokens that stay visible), GQA, ragged requests.
-#include "paged_decode.cuh"
+#include "paged_chunk.cuh"
 
 #include <algorithm>
 #include <cmath>
 
 namespace gtn {
 
-// Workers of the decode kernel: the warps that are resident at once.
+// Workers of the decode kernel: the warps that are resident at once; of the chunk kernel: one CTA per SM.
 constexpr int DECODE_CTAS = 3;  // per SM, at most
+static long decode_workers() { return (long)sm_count() * DECODE_CTAS * PD_WARPS; }
+static int64_t join_bytes(long workers) { return (workers * (int64_t)sizeof(PagedJoin) + 15) / 16 * 16; }
 static int64_t decode_ws_bytes(int d) {
-    const int64_t workers = (int64_t)sm_count() * DECODE_CTAS * PD_WARPS;
-    return workers * (2 * 16 * (d + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(PagedJoin) + 16);
+    return decode_workers() * 2 * 16 * (d + 2) * (int64_t)sizeof(float) + join_bytes(decode_workers());
+}
+static int64_t chunk_ws_bytes(int d) {
+    return (int64_t)sm_count() * 2 * CH_ROWS * (d + 2) * (int64_t)sizeof(float) + join_bytes(sm_count());
 }
 
 template <int DT, int D, int ROWS>
@@ -34,6 +38,44 @@ static cudaError_t decode(const PagedAttnArgs& a, const PagedPick& p, int most, 
     return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 128, ROWS>(a, p, most, st) : launch_decode<GTN_Q8, 128, ROWS>(a, p, most, st);
 }
 
+// A pool of fp16 pages as [page][kv head and row][d] for boxes of `box` rows x 64 columns.
+static bool page_map(const PagedCache& c, uint8_t* pool, int box, CUtensorMap* m) {
+    const TmapEncodeFn fn = tmap_encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)c.d, (cuuint64_t)c.kv_heads * c.ps, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.d * 2, (cuuint64_t)c.page_stride};
+    const cuuint32_t bx[3] = {64, (cuuint32_t)box, 1}, es[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, pool, dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DT, int D>
+static cudaError_t launch_chunk(PagedAttnArgs a, const PagedPick& p, cudaStream_t st) {
+    using C = ChunkCfg<D>;
+    const int ctas = sm_count();
+    a.join = reinterpret_cast<PagedJoin*>(a.part + (long)ctas * 2 * paged_slot<CH_ROWS, D>());
+    cudaError_t e = ensure_smem(k_paged_chunk<DT, D>, C::SMEM);
+    if (e != cudaSuccess) return e;
+    // the register split (2 x 208 + 88 per three warps) has to fit what the CTA is launched with
+    static const int regs = [] {
+        cudaFuncAttributes f;
+        return cudaFuncGetAttributes(&f, k_paged_chunk<DT, D>) == cudaSuccess ? f.numRegs : 0;
+    }();
+    if (regs < 168) return cudaErrorInvalidConfiguration;
+    CUtensorMap km{}, vm{};
+    const int box = std::min(a.c.ps, CH_KEYS);
+    if (DT == GTN_F16 && (!page_map(a.c, a.c.k, box, &km) || !page_map(a.c, a.c.v, box, &vm))) return cudaErrorInvalidValue;
+    e = launch_pdl(k_paged_chunk<DT, D>, dim3(ctas), dim3(CH_THREADS), C::SMEM, st, a, p, km, vm, box);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_paged_join<CH_ROWS, D>, dim3((ctas + 3) / 4, 64), dim3(128), 0, st, a, ctas);
+}
+
+static cudaError_t chunk(const PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
+    if (a.c.d == 64) return a.c.dt == GTN_F16 ? launch_chunk<GTN_F16, 64>(a, p, st) : launch_chunk<GTN_Q8, 64>(a, p, st);
+    return a.c.dt == GTN_F16 ? launch_chunk<GTN_F16, 128>(a, p, st) : launch_chunk<GTN_Q8, 128>(a, p, st);
+}
+
 }  // namespace gtn
 
 using namespace gtn;
@@ -42,7 +84,7 @@ extern "C" {
 
 int64_t gtn_paged_attn_workspace(int heads, int d_head) {
     if (heads < 1 || (d_head != 64 && d_head != 128)) return 0;
-    return decode_ws_bytes(d_head);
+    return decode_ws_bytes(d_head) + chunk_ws_bytes(d_head);
 }
 
 int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_tensor* block_table,
@@ -106,11 +148,26 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)d)) * 1.4426950408889634f;
     a.part = (float*)workspace;
     a.err = device_error_word();
+    // Requests of at most `cut` rows per kv head (tokens x query heads of it) go to the decode kernel, the
+    // others to the chunk kernel. With a bound on the new tokens that says so, only the one is launched; so
+    // is it for a single request, where the other's empty launch would cost more than its choice gives.
     PagedPick p;
-    p.cut = 0x7fffffff;
     p.below = true;
-    const long most = max_new > 0 ? (long)max_new * a.group : 16;
-    const cudaError_t e = most <= 8 ? decode<8>(a, p, (int)most, S(stream)) : decode<16>(a, p, 16, S(stream));
+    p.cut = a.group <= 8 ? 8 : a.group <= 16 ? 16 : 0;
+    const long most = max_new > 0 ? (long)max_new * a.group : 0x7fffffffL;
+    cudaError_t e = cudaSuccess;
+    if (most <= 16) {
+        p.cut = 0x7fffffff;
+        e = most <= 8 ? decode<8>(a, p, (int)most, S(stream)) : decode<16>(a, p, (int)most, S(stream));
+    } else {
+        PagedAttnArgs c = a;
+        c.part = (float*)((uint8_t*)workspace + decode_ws_bytes(d));
+        if (n == 1) p.cut = 0;
+        PagedPick rest = p;
+        rest.below = false;
+        e = chunk(c, rest, S(stream));
+        if (e == cudaSuccess && p.cut > 0) e = p.cut == 8 ? decode<8>(a, p, 8, S(stream)) : decode<16>(a, p, 16, S(stream));
+    }
     return cuda_status(e, who);
 }
 

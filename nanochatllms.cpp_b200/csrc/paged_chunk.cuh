@@ -1,0 +1,600 @@
+// Paged attention for chunks of new tokens: bound by the matrix products and the exponentials.
+//
+// A worker (paged_sched.cuh) is a CTA, one per SM; an item is 256 query rows (two tiles of 128, the rows of
+// one kv head's query heads packed token by token, so that K and V are read once for all of them), a unit 128
+// keys. S = Q K^T and O += P V run on tcgen05 with S (128 columns per tile), P (fp16, in S's place) and O in
+// TMEM; one thread owns a query row, so that the softmax needs no exchange between threads. The two tiles
+// alternate: while one tile's scores are turned into weights, the tensor cores work for the other.
+//
+// Roles, which meet only at mbarriers:
+//   warps 0-3, 4-7  softmax of tile 0, 1: read S, running maximum and sum, write P; rescale O when the maximum
+//                   has grown by more than 2^CH_GROW (until then the old one serves, the weights stay below
+//                   2^(CH_BIAS + CH_GROW) < 65504); load Q before an item and write O behind it;
+//   warp 8          issues the MMAs (one thread): P V of unit u, then Q K^T of unit u + 1, tile by tile;
+//   warps 9-11      K and V. fp16 cache: warp 9 fetches pages with TMA (128-byte swizzle), warps 10 and 11
+//                   look at the V tiles that not every row sees whole (below). Q8 cache: all three read the
+//                   pages' 8-bit values and write the tiles as fp16, q * delta rounded once (2^-11
+//                   relative, like the weights).
+// Keys that a row does not see get weight 0, but 0 times NaN or infinity would reach the row all the same. So
+// in the tiles that not every row sees whole, values that no row sees are zeroed in shared memory, and
+// non-finite ones that some row sees are too, with a flag on which the epilogue adds them, read from the
+// pages again, to the rows that see them.
+// Every wait is bounded as in gemm_tc.cuh.
+#pragma once
+#include "paged_decode.cuh"
+
+namespace gtn {
+
+constexpr int CH_THREADS = 384;
+constexpr int CH_ROWS = 256;
+constexpr int CH_KEYS = 128;
+constexpr float CH_BIAS = 7.0f;
+constexpr float CH_GROW = 8.0f;
+
+template <int D>
+struct ChunkCfg {
+    static constexpr int TILE = 128 * D * 2;  // bytes of a Q, K or V tile
+    static constexpr int KS = D == 64 ? 3 : 2, VS = D == 64 ? 3 : 2;
+    static constexpr int SMEM = 1024 + (2 + KS + VS) * TILE + 512;
+    static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
+    // kind::f16, A = B = fp16, D = fp32; scores: both K-major, N = 128; output: B (V) MN-major, N = D
+    static constexpr uint32_t IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    static constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+};
+
+// Matrix descriptors of tiles of 128-byte rows in the 128-byte swizzle (8-row groups of 1024 bytes). K-major
+// (Q, K: a row holds 64 elements of d): stride between row groups. MN-major (V: a row holds 64 columns of one
+// key): stride between groups of 8 keys, and between 64-column halves.
+__device__ __forceinline__ uint64_t ch_desc(uint32_t saddr, uint32_t lbo) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// D (+)= A B with A in TMEM.
+__device__ __forceinline__ void ch_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+#define CH_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
+#define CH_U8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
+#define CH_W8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
+// 32 consecutive TMEM columns of the thread's lane; valid after ch_wait_ld, which names the registers.
+__device__ __forceinline__ void ch_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : CH_R8(r, 0), CH_R8(r, 8), CH_R8(r, 16), CH_R8(r, 24)
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void ch_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" : CH_W8(r, 0), CH_W8(r, 8), CH_W8(r, 16), CH_W8(r, 24) : : "memory");
+}
+__device__ __forceinline__ void ch_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+        CH_U8(r, 0), CH_U8(r, 8), CH_U8(r, 16), CH_U8(r, 24)
+        : "memory");
+}
+__device__ __forceinline__ void ch_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};\n" ::"r"(taddr),
+        CH_U8(r, 0), CH_U8(r, 8)
+        : "memory");
+}
+__device__ __forceinline__ void ch_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 3-D TMA tile load (no multicast): box (x, y, z) of a pool of pages; boxes outside it read as zeros.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+struct ChunkSmem {
+    uint64_t k_full[3], k_empty[3], v_load[3], v_full[3], v_empty[3];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+    uint32_t tmem;
+    volatile int abort;
+    volatile int odd;  // a non-finite value was set aside (stays set)
+    PagedSchedSmem<1> sched;
+};
+
+template <int DT, int D>
+__global__ void __launch_bounds__(CH_THREADS, 1)
+    k_paged_chunk(PagedAttnArgs a, PagedPick p, const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap, int box) {
+    using C = ChunkCfg<D>;
+    constexpr bool Q8 = DT == GTN_Q8;
+    constexpr int HALVES = D / 64, HALF = 128 * 128;  // 64-column halves of a tile, bytes of one
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ ChunkSmem sm;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sq = base, sk = sq + 2 * C::TILE, sv = sk + C::KS * C::TILE;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
+                     "r"(TC_TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        for (int s = 0; s < 3; ++s) {
+            mbar_init(&sm.k_full[s], Q8 ? 3 : 1);
+            mbar_init(&sm.k_empty[s], 1);
+            mbar_init(&sm.v_load[s], 1);
+            mbar_init(&sm.v_full[s], Q8 ? 3 : 2);
+            mbar_init(&sm.v_empty[s], 1);
+        }
+        for (int r = 0; r < 2; ++r) {
+            mbar_init(&sm.q_full[r], 128);
+            mbar_init(&sm.s_full[r], 1);
+            mbar_init(&sm.p_full[r], 128);
+            mbar_init(&sm.o_full[r], 1);
+        }
+        mbar_init(&sm.drain, 1);
+        sm.abort = 0;
+        sm.odd = 0;
+        fence_mbar_init();
+    }
+    pdl_wait();
+    pdl_trigger();
+    const int me = blockIdx.x, workers = gridDim.x;
+    tc_fence_before();
+    const long long total = paged_sched<CH_ROWS, CH_KEYS, CH_THREADS>(a, p, workers, me, me == 0, sm.sched);
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    const long long share = (total + workers - 1) / workers;
+    PagedPos x = sm.sched.pos[0];
+    int left = x.b < 0 ? 0 : (int)min(total - share * me, share);
+    if (tid == 0) a.join[me].last = -1;
+
+    // units of row tile r in [u0, u1) that any of its rows sees to the causal limit: the first n_r
+    auto tile_units = [&](int r, int u0, int u1) {
+        const int m1 = min(x.r.n * a.group, x.tile * CH_ROWS + (r + 1) * 128) - 1;  // the tile's last row
+        if (m1 < x.tile * CH_ROWS + r * 128) return 0;
+        const int phi = x.r.base + m1 / a.group;
+        int n = 0;
+        if (phi < 0) return 0;
+        // keys ascend with u: sink units u < ns hold keys u * 128, the others (w0 + u - ns) * 128
+        n = min(x.t.ns, phi / CH_KEYS + 1);
+        if (n == x.t.ns) n += max(0, phi / CH_KEYS - x.t.w0 + 1);
+        return max(0, min(u1, n) - u0);
+    };
+    auto wait1 = [&](uint64_t* bar, uint32_t ph) {
+        if (sm.abort == 0 && tc_wait(bar, ph, a.err)) return true;
+        sm.abort = 1;
+        return false;
+    };
+    auto wait = [&](uint64_t* bar, uint32_t ph) { return __all_sync(0xffffffffu, wait1(bar, ph)) != 0; };  // a whole warp
+    // a unit that every row of the item sees whole
+    auto seen_whole = [&](int kb) {
+        const int lo = a.window > 0 ? max(0, x.t.phi - a.window + 1) : 0;
+        return kb + CH_KEYS - 1 <= x.t.plo && (kb >= lo || kb + CH_KEYS <= a.n_sink);
+    };
+    auto next_item = [&](int done) {
+        left -= done;
+        if (left > 0) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
+    };
+
+    if (warp < 8) {
+        // ---- softmax of tile r
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int r = warp >> 2, row = tid & 127;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t ts = lanes + r * 128, to = lanes + C::COL_O + r * D;
+        const uint32_t qs = sq + r * C::TILE;
+        const long hb = row_bytes(a.io, D);
+        uint32_t s_ph = 0, o_ph = 0;
+        bool ok = true;
+        auto load_q = [&]() {  // the row's query into the swizzled tile
+            const int m = x.tile * CH_ROWS + r * 128 + row;
+            if (x.r.n * a.group <= x.tile * CH_ROWS + r * 128) return;
+            const bool in = m < x.r.n * a.group;
+            const uint8_t* qh =
+                a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, r * 128 + row, CH_ROWS, a.qs, hb) : 0);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                const uint4 v = in ? paged_q8x(qh, a.io, 8 * c) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t dst = qs + (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                             : "memory");
+            }
+            fence_async_smem();
+            mbar_arrive(&sm.q_full[r]);
+        };
+        if (left > 0) load_q();
+        while (left > 0 && ok) {
+            const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = tile_units(r, u0, u1);
+            const int m_row = x.tile * CH_ROWS + r * 128 + row;
+            const bool live = m_row < x.r.n * a.group;
+            const int pos = live ? x.r.base + m_row / a.group : -1;
+            const int wlo = a.window > 0 ? pos - a.window + 1 : 0;
+            float mu = -INFINITY, l = 0.0f;  // the maximum in use (base 2), the sum of weights
+            for (int u = 0; u < n; ++u) {
+                if (!(ok = wait(&sm.s_full[r], s_ph))) break;
+                s_ph ^= 1u;
+                tc_fence_after();
+                const int kb = paged_unit_key<CH_KEYS>(x.t, u0 + u);
+                uint32_t s[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ch_ld32(ts + 32 * i, s[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ch_wait_ld(s[i]);
+                const bool whole = seen_whole(kb);
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int key = kb + 32 * i + j;
+                            if (key > pos || (key < wlo && key >= a.n_sink)) s[i][j] = 0xff800000u;
+                        }
+                }
+                float mx = __uint_as_float(s[0][0]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2)
+                        mx = fmaxf(mx, fmaxf(__uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1])));
+                mx *= a.scale_log2;
+                float f = 1.0f;
+                if (mx > mu + CH_GROW || (mu == -INFINITY && mx > mu)) {
+                    f = ex2(mu - mx);  // 0 when nothing was seen yet
+                    mu = mx;
+                    l *= f;
+                }
+                if (u > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+                    // P V of the unit before is done (its commit came before this unit's scores')
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        ch_ld32(to + 32 * c, o);
+                        ch_wait_ld(o);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        ch_st32(to + 32 * c, o);
+                    }
+                }
+                const float sub = CH_BIAS - (mu == -INFINITY ? 0.0f : mu);
+                float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float e0 = ex2(fmaf(__uint_as_float(s[i][2 * j]), a.scale_log2, sub));
+                        const float e1 = ex2(fmaf(__uint_as_float(s[i][2 * j + 1]), a.scale_log2, sub));
+                        sum0 += e0;
+                        sum1 += e1;
+                        w[j] = pack_f16(e0, e1);
+                    }
+                    ch_st16(ts + 16 * i, w);
+                }
+                l += sum0 + sum1;
+                ch_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sm.p_full[r]);
+            }
+            // the next item's queries go in before this item's output comes out: all products with this item's
+            // are done (its last scores were seen)
+            const PagedPos was = x;
+            next_item(u1 - u0);
+            if (ok && left > 0) load_q();
+            if (ok && n > 0) {
+                ok = wait(&sm.o_full[r], o_ph);
+                o_ph ^= 1u;
+                tc_fence_after();
+            }
+            if (ok && was.r.n * a.group > was.tile * CH_ROWS + r * 128) {
+                const bool done = u0 == 0 && u1 == was.t.units;
+                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+                const int prow = r * 128 + row;
+                float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<CH_ROWS, D>();
+                uint8_t* dst =
+                    a.out + (live ? paged_row_at(a, was.r.first, was.h, was.tile, prow, CH_ROWS, a.os, hb) : 0);
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    float v[32];
+                    if (n > 0) {
+                        ch_ld32(to + 32 * c, o);
+                        ch_wait_ld(o);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = n > 0 ? __uint_as_float(o[j]) : 0.0f;
+                    if (n > 0 && sm.odd != 0) {
+                        // values set aside: the non-finite ones that this row sees
+                        for (int u = u0; u < u1; ++u) {
+                            const int kb = paged_unit_key<CH_KEYS>(was.t, u);
+                            for (int key = kb; key < kb + CH_KEYS && key <= pos; ++key) {
+                                if (key < wlo && key >= a.n_sink) continue;
+                                const int page = a.table[was.b * a.table_stride + (key >> a.c.ps_shift)];
+                                if ((unsigned)page >= (unsigned)a.c.n_pages) continue;
+                                const uint8_t* pg = a.c.v + (long)page * a.c.page_stride;
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    const float y = paged_elem(a.c, pg, was.h, key & (a.c.ps - 1), 32 * c + j);
+                                    if (!(fabsf(y) < INFINITY)) v[j] += y;
+                                }
+                            }
+                        }
+                    }
+                    if (done) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = l != 0.0f ? v[j] * inv : 0.0f;
+                        paged_store<32>(dst, a.io, 32 * c, v, live);
+                    } else if (live) {
+                        float4* q4 = reinterpret_cast<float4*>(ps + (long)prow * D + 32 * c);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) q4[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    }
+                }
+                if (!done && live) {
+                    ps[CH_ROWS * D + prow] = mu;
+                    ps[CH_ROWS * (D + 1) + prow] = l;
+                }
+                if (tid == 0 && u0 == 0 && u1 < was.t.units)
+                    a.join[me] = PagedJoin{(int)((was.start + was.t.units - 1) / share), was.r.first, was.h, was.tile,
+                                           min(CH_ROWS, was.r.n * a.group - was.tile * CH_ROWS)};
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 8) {
+            // ---- MMA issue
+            if (lane == 0) {
+                int ks = 0, vs = 0;
+                uint32_t k_ph = 0, v_ph = 0, q_ph = 0, p_ph[2] = {0, 0};
+                bool ok = true;
+                auto qk = [&](int r) {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t off = (i >> 2) * HALF + (i & 3) * 32;
+                        tc_mma(tmem + r * 128, ch_desc(sq + r * C::TILE + off, 16), ch_desc(sk + ks * C::TILE + off, 16),
+                               C::IDESC_S, i > 0);
+                    }
+                    tc_commit(&sm.s_full[r]);
+                };
+                while (left > 0 && ok) {
+                    const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = u1 - u0;
+                    const int nr[2] = {tile_units(0, u0, u1), tile_units(1, u0, u1)};
+                    const bool two = x.r.n * a.group > x.tile * CH_ROWS + 128;
+                    ok = wait1(&sm.k_full[ks], k_ph);
+                    for (int r = 0; r < (two ? 2 : 1) && ok; ++r) {
+                        ok = wait1(&sm.q_full[r], (q_ph >> r) & 1u);
+                        q_ph ^= 1u << r;
+                        tc_fence_after();
+                        if (ok && nr[r] > 0) qk(r);
+                    }
+                    for (int u = 0; u < n && ok; ++u) {
+                        tc_commit(&sm.k_empty[ks]);  // the scores of unit u are issued
+                        if (++ks == C::KS) {
+                            ks = 0;
+                            k_ph ^= 1u;
+                        }
+                        if (u + 1 < n) ok = wait1(&sm.k_full[ks], k_ph);
+                        if (ok) ok = wait1(&sm.v_full[vs], v_ph);
+                        for (int r = 0; r < 2 && ok; ++r) {
+                            if (u >= nr[r]) continue;
+                            if (!(ok = wait1(&sm.p_full[r], p_ph[r]))) break;
+                            p_ph[r] ^= 1u;
+                            tc_fence_after();
+#pragma unroll
+                            for (int i = 0; i < CH_KEYS / 16; ++i)
+                                ch_mma_ts(tmem + C::COL_O + r * D, tmem + r * 128 + i * 8,
+                                          ch_desc(sv + vs * C::TILE + i * 2048, HALF), C::IDESC_O, u > 0 || i > 0);
+                            if (u + 1 < nr[r]) qk(r);
+                            else tc_commit(&sm.o_full[r]);
+                        }
+                        if (!ok) break;
+                        tc_commit(&sm.v_empty[vs]);
+                        if (++vs == C::VS) {
+                            vs = 0;
+                            v_ph ^= 1u;
+                        }
+                    }
+                    next_item(n);
+                }
+                tc_commit(&sm.drain);  // nothing of this CTA is in flight behind this
+                tc_wait(&sm.drain, 0, a.err);
+            }
+            __syncwarp();
+        } else if (!Q8 && warp == 9) {
+            // ---- fetch of fp16 pages: lane i issues the boxes of piece i (`box` rows) of a unit
+            int ks = 0, vs = 0, k_issued = 0, v_issued = 0;
+            uint32_t k_ph = 1, v_ph = 1;  // the first use of a stage waits for nothing
+            bool ok = true;
+            const int pieces = CH_KEYS / box;
+            while (left > 0 && ok) {
+                const int u0 = x.u, u1 = min(x.t.units, u0 + left);
+                for (int u = u0; u < u1; ++u) {
+                    const int kb = paged_unit_key<CH_KEYS>(x.t, u), k0 = kb + lane * box;
+                    const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
+                    int page = a.c.n_pages;  // outside the pool: zeros
+                    if (lane < pieces && k0 <= x.t.phi && (k0 + box - 1 >= lo || k0 < a.n_sink)) {
+                        page = a.table[x.b * a.table_stride + (k0 >> a.c.ps_shift)];
+                        if ((unsigned)page >= (unsigned)a.c.n_pages) {
+                            page = a.c.n_pages;
+                            atomicOr(a.err, GTN_DEVERR_PAGE);
+                        }
+                    }
+                    const int yrow = x.h * a.c.ps + (k0 & (a.c.ps - 1));
+                    if (!(ok = wait(&sm.k_empty[ks], k_ph))) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&sm.k_full[ks], C::TILE);
+                    __syncwarp();
+                    if (lane < pieces)
+                        for (int h = 0; h < HALVES; ++h)
+                            tma_load_3d(sk + ks * C::TILE + h * HALF + lane * box * 128, &kmap, 64 * h, yrow, page,
+                                        &sm.k_full[ks]);
+                    ++k_issued;
+                    if (++ks == C::KS) {
+                        ks = 0;
+                        k_ph ^= 1u;
+                    }
+                    if (!(ok = wait(&sm.v_empty[vs], v_ph))) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&sm.v_load[vs], C::TILE);
+                    __syncwarp();
+                    if (lane < pieces)
+                        for (int h = 0; h < HALVES; ++h)
+                            tma_load_3d(sv + vs * C::TILE + h * HALF + lane * box * 128, &vmap, 64 * h, yrow, page,
+                                        &sm.v_load[vs]);
+                    ++v_issued;
+                    if (++vs == C::VS) {
+                        vs = 0;
+                        v_ph ^= 1u;
+                    }
+                }
+                next_item(u1 - u0);
+            }
+            // a wait has run out somewhere: the copies in flight end before the shared memory goes
+            if (sm.abort != 0 && lane == 0) {
+                for (int i = max(0, k_issued - C::KS); i < k_issued; ++i)
+                    tc_wait(&sm.k_full[i % C::KS], (uint32_t)(i / C::KS) & 1u, a.err);
+                for (int i = max(0, v_issued - C::VS); i < v_issued; ++i)
+                    tc_wait(&sm.v_load[i % C::VS], (uint32_t)(i / C::VS) & 1u, a.err);
+            }
+            __syncwarp();
+        } else if (!Q8) {
+            // ---- V tiles that not every row sees whole
+            int vs = 0;
+            uint32_t v_ph = 0;
+            bool ok = true;
+            const int ct = tid - 320;
+            while (left > 0 && ok) {
+                const int u0 = x.u, u1 = min(x.t.units, u0 + left);
+                for (int u = u0; u < u1; ++u) {
+                    if (!(ok = wait(&sm.v_load[vs], v_ph))) break;
+                    const int kb = paged_unit_key<CH_KEYS>(x.t, u);
+                    if (!seen_whole(kb)) {
+                        const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
+                        for (int i = ct; i < HALVES * 1024; i += 64) {
+                            const int key = kb + ((i >> 3) & 127);
+                            const uint32_t at = sv + vs * C::TILE + i * 16;
+                            const bool seen = key <= x.t.phi && (key >= lo || key < a.n_sink);
+                            uint4 v = lds16(at);
+                            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                            bool change = !seen, bad = false;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (!seen) w[j] = 0u;
+                                if ((w[j] & 0x7c00u) == 0x7c00u) { w[j] &= 0xffff0000u; bad = true; }
+                                if ((w[j] & 0x7c000000u) == 0x7c000000u) { w[j] &= 0x0000ffffu; bad = true; }
+                            }
+                            if (change || bad)
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
+                                             "r"(w[2]), "r"(w[3])
+                                             : "memory");
+                            if (bad) sm.odd = 1;
+                        }
+                        fence_async_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.v_full[vs]);
+                    if (++vs == C::VS) {
+                        vs = 0;
+                        v_ph ^= 1u;
+                    }
+                }
+                next_item(u1 - u0);
+            }
+        } else {
+            // ---- Q8 pages to fp16 tiles: 96 threads, 16 elements of a row at a time
+            int ks = 0, vs = 0;
+            uint32_t k_ph = 1, v_ph = 1;
+            bool ok = true;
+            const int ct = tid - 288;
+            constexpr int CPR = D / 16, CHUNKS = 128 * CPR;  // 16-element chunks of a row, of a tile
+            constexpr int PER = (CHUNKS + 95) / 96;
+            while (left > 0 && ok) {
+                const int u0 = x.u, u1 = min(x.t.units, u0 + left);
+                const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
+                for (int u = u0; u < u1 && ok; ++u) {
+                    const int kb = paged_unit_key<CH_KEYS>(x.t, u);
+                    const bool whole = seen_whole(kb);
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const uint8_t* pool = kv ? a.c.v : a.c.k;
+                        uint4 raw[PER];
+                        uint16_t dl[PER];
+#pragma unroll
+                        for (int i = 0; i < PER; ++i) {
+                            const int ch = ct + 96 * i, row = ch / CPR, key = kb + row;
+                            raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                            dl[i] = 0;
+                            if (ch < CHUNKS && key <= x.t.phi && (key >= lo || key < a.n_sink)) {
+                                const int page = a.table[x.b * a.table_stride + (key >> a.c.ps_shift)];
+                                if ((unsigned)page < (unsigned)a.c.n_pages) {
+                                    const uint8_t* pg = pool + (long)page * a.c.page_stride;
+                                    const int pr = key & (a.c.ps - 1), e = ch % CPR * 16;
+                                    raw[i] = *reinterpret_cast<const uint4*>(pg + paged_row(a.c, x.h, pr) + e);
+                                    dl[i] = reinterpret_cast<const uint16_t*>(pg + paged_delta(a.c, x.h, pr))[e / GTN_QBLK];
+                                } else {
+                                    atomicOr(a.err, GTN_DEVERR_PAGE);
+                                }
+                            }
+                        }
+                        if (!(ok = kv ? wait(&sm.v_empty[vs], v_ph) : wait(&sm.k_empty[ks], k_ph))) break;
+                        const uint32_t tile = kv ? sv + vs * C::TILE : sk + ks * C::TILE;
+#pragma unroll
+                        for (int i = 0; i < PER; ++i) {
+                            const int ch = ct + 96 * i, row = ch / CPR, c16 = ch % CPR;
+                            if (ch >= CHUNKS) continue;
+                            const __half2 d2 = __half2half2(__ushort_as_half(dl[i]));
+                            const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                            uint32_t w[8];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint2 b = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
+                                const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&b.x), d2);
+                                const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&b.y), d2);
+                                w[2 * j] = *reinterpret_cast<const uint32_t*>(&h0);
+                                w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                            }
+                            if (kv && !whole) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    if ((w[j] & 0x7c00u) == 0x7c00u) { w[j] &= 0xffff0000u; sm.odd = 1; }
+                                    if ((w[j] & 0x7c000000u) == 0x7c000000u) { w[j] &= 0x0000ffffu; sm.odd = 1; }
+                                }
+                            }
+                            const uint32_t at = tile + (c16 >> 2) * HALF + row * 128;
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                                 at + ((((2 * c16 + j) & 7) ^ (row & 7)) << 4)),
+                                             "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                                             : "memory");
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(kv ? &sm.v_full[vs] : &sm.k_full[ks]);
+                    }
+                    if (!ok) break;
+                    if (++ks == C::KS) {
+                        ks = 0;
+                        k_ph ^= 1u;
+                    }
+                    if (++vs == C::VS) {
+                        vs = 0;
+                        v_ph ^= 1u;
+                    }
+                }
+                next_item(u1 - u0);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC_TMEM_COLS) : "memory");
+    }
+}
+
+}  // namespace gtn

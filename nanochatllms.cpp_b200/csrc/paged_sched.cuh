@@ -213,9 +213,15 @@ __device__ __forceinline__ void paged_store(uint8_t* head, int io, int c0, const
         uint32_t w[N / 2];
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) w[i] = (uint32_t)f2h(y[2 * i]) | ((uint32_t)f2h(y[2 * i + 1]) << 16);
-        uint2* dst = reinterpret_cast<uint2*>(head + 2 * c0);
+        if constexpr (N % 8 == 0) {
+            uint4* dst = reinterpret_cast<uint4*>(head + 2 * c0);
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i) dst[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+            for (int i = 0; i < N / 8; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else {
+            uint2* dst = reinterpret_cast<uint2*>(head + 2 * c0);
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) dst[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+        }
         return;
     }
     // the activation quantizer (warp_quant_block): absmax without NaN, delta, 1 / delta unrounded, roundf
