@@ -192,9 +192,11 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         const long hb = row_bytes(a.io, D);
         uint32_t s_ph = 0, o_ph = 0;
         bool ok = true;
-        auto load_q = [&]() {  // the row's query into the swizzled tile
+        // The row's query into the swizzled tile. Not for a tile without units: its softmax waits for nothing
+        // and could pass q_full twice before the MMA warp looks.
+        auto load_q = [&]() {
             const int m = x.tile * CH_ROWS + r * 128 + row;
-            if (x.r.n * a.group <= x.tile * CH_ROWS + r * 128) return;
+            if (tile_units(r, x.u, min(x.t.units, x.u + left)) == 0) return;
             const bool in = m < x.r.n * a.group;
             const uint8_t* qh =
                 a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, r * 128 + row, CH_ROWS, a.qs, hb) : 0);
@@ -364,13 +366,13 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 while (left > 0 && ok) {
                     const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = u1 - u0;
                     const int nr[2] = {tile_units(0, u0, u1), tile_units(1, u0, u1)};
-                    const bool two = x.r.n * a.group > x.tile * CH_ROWS + 128;
                     ok = wait1(&sm.k_full[ks], k_ph);
-                    for (int r = 0; r < (two ? 2 : 1) && ok; ++r) {
+                    for (int r = 0; r < 2 && ok; ++r) {
+                        if (nr[r] == 0) continue;
                         ok = wait1(&sm.q_full[r], (q_ph >> r) & 1u);
                         q_ph ^= 1u << r;
                         tc_fence_after();
-                        if (ok && nr[r] > 0) qk(r);
+                        if (ok) qk(r);
                     }
                     for (int u = 0; u < n && ok; ++u) {
                         tc_commit(&sm.k_empty[ks]);  // the scores of unit u are issued

@@ -309,6 +309,16 @@ def test_attn_long_axis(gpu, lens, cache):
     b.run().compare()
 
 
+@pytest.mark.parametrize("cache", [F16, Q8])
+@pytest.mark.parametrize("heads,kvh,d,n", [(32, 32, 64, 3), (24, 24, 128, 2)])
+def test_attn_many_items_per_worker(gpu, cache, heads, kvh, d, n):
+    """Several items and many units for every worker: the rings wrap, and ranges end on units that only one
+    of an item's two row tiles needs."""
+    b = Batch(gpu, n, [(700 + 31 * i, 500 - 17 * i) for i in range(n)], heads, kvh, d, 32, cache, F16)
+    b.run().compare()
+    G.check()
+
+
 @pytest.mark.parametrize("scale", [0.02, 1.0])
 def test_attn_scale_and_peaked_scores(gpu, scale):
     """Scores up to about +-100: weights that underflow, and a running maximum that moves."""
