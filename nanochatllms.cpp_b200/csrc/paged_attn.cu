@@ -57,12 +57,6 @@ static cudaError_t launch_chunk(PagedAttnArgs a, const PagedPick& p, cudaStream_
     a.join = reinterpret_cast<PagedJoin*>(a.part + (long)ctas * 2 * paged_slot<CH_ROWS, D>());
     cudaError_t e = ensure_smem(k_paged_chunk<DT, D>, C::SMEM);
     if (e != cudaSuccess) return e;
-    // the register split (2 x 208 + 88 per three warps) has to fit what the CTA is launched with
-    static const int regs = [] {
-        cudaFuncAttributes f;
-        return cudaFuncGetAttributes(&f, k_paged_chunk<DT, D>) == cudaSuccess ? f.numRegs : 0;
-    }();
-    if (regs < 168) return cudaErrorInvalidConfiguration;
     CUtensorMap km{}, vm{};
     const int box = std::min(a.c.ps, CH_KEYS);
     if (DT == GTN_F16 && (!page_map(a.c, a.c.k, box, &km) || !page_map(a.c, a.c.v, box, &vm))) return cudaErrorInvalidValue;

@@ -36,6 +36,7 @@ struct ChunkCfg {
     static constexpr int TILE = 128 * D * 2;  // bytes of a Q, K or V tile
     static constexpr int KS = D == 64 ? 3 : 2, VS = D == 64 ? 3 : 2;
     static constexpr int SMEM = 1024 + (2 + KS + VS) * TILE + 512;
+    static constexpr int POLY = D == 64 ? 3 : 4;  // every POLY-th pair of exponentials on the multiply-add pipe
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
     // kind::f16, A = B = fp16, D = fp32; scores: both K-major, N = 128; output: B (V) MN-major, N = D
     static constexpr uint32_t IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -94,6 +95,53 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
             dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
         : "memory");
+}
+
+// Pairs of fp32 in one 64-bit register (packed multiply-add and add).
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 f2_get(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair on the multiply-add pipe: x = n + f with n the nearest integer (by adding 1.5 * 2^23, which
+// leaves n in the low bits), 2^f by a polynomial of degree 4, 2^n by an integer add to the exponent. The
+// coefficients minimise the largest relative error on [-1/2, 1/2] (Remez exchange): 2.6e-6, a hundredth of
+// the rounding to fp16 that follows. x below -126 gives about 2^-126; NaN is not kept (the caller looks).
+__device__ __forceinline__ float2 f2_exp2(uint64_t x) {
+    float2 v = f2_get(x);
+    x = f2_pack(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+    const uint64_t magic = f2_pack(12582912.0f, 12582912.0f), back = f2_pack(-12582912.0f, -12582912.0f);
+    const uint64_t t = f2_add(x, magic), n = f2_add(t, back), f = f2_fma(n, f2_pack(-1.0f, -1.0f), x);
+    uint64_t q = f2_fma(f2_pack(0.009570102207362652f, 0.009570102207362652f), f,
+                        f2_pack(0.05591785907745361f, 0.05591785907745361f));
+    q = f2_fma(q, f, f2_pack(0.240247443318367f, 0.240247443318367f));
+    q = f2_fma(q, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+    q = f2_fma(q, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+    v = f2_get(q);
+    const float2 e = f2_get(t);
+    v.x = __int_as_float(__float_as_int(v.x) + (__float_as_int(e.x) << 23));
+    v.y = __int_as_float(__float_as_int(v.y) + (__float_as_int(e.y) << 23));
+    return v;
 }
 
 struct ChunkSmem {
@@ -184,7 +232,6 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
 
     if (warp < 8) {
         // ---- softmax of tile r
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int r = warp >> 2, row = tid & 127;
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t ts = lanes + r * 128, to = lanes + C::COL_O + r * D;
@@ -217,43 +264,37 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             const bool live = m_row < x.r.n * a.group;
             const int pos = live ? x.r.base + m_row / a.group : -1;
             const int wlo = a.window > 0 ? pos - a.window + 1 : 0;
-            float mu = -INFINITY, l = 0.0f;  // the maximum in use (base 2), the sum of weights
+            // the maximum in use (base 2; a row behind the item's last needs none), the sum of weights
+            float mu = live ? -INFINITY : 0.0f, l = 0.0f;
             for (int u = 0; u < n; ++u) {
                 if (!(ok = wait(&sm.s_full[r], s_ph))) break;
                 s_ph ^= 1u;
                 tc_fence_after();
                 const int kb = paged_unit_key<CH_KEYS>(x.t, u0 + u);
-                uint32_t s[4][32];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ch_ld32(ts + 32 * i, s[i]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ch_wait_ld(s[i]);
                 const bool whole = seen_whole(kb);
-                if (!whole) {
+                // the keys of chunk i (32) that this row sees, as bits
+                auto seen_bits = [&](int i) -> uint32_t {
+                    const int k0 = kb + 32 * i;
+                    auto below = [](int n) -> uint32_t { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+                    uint32_t v = below(pos - k0 + 1);
+                    if (a.window > 0) v &= ~below(wlo - k0) | below(a.n_sink - k0);
+                    return v;
+                };
+                auto hide = [](uint32_t (&v)[32], uint32_t bits) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int key = kb + 32 * i + j;
-                            if (key > pos || (key < wlo && key >= a.n_sink)) s[i][j] = 0xff800000u;
-                        }
-                }
-                float mx = __uint_as_float(s[0][0]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2)
-                        mx = fmaxf(mx, fmaxf(__uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1])));
-                mx *= a.scale_log2;
-                float f = 1.0f;
-                if (mx > mu + CH_GROW || (mu == -INFINITY && mx > mu)) {
-                    f = ex2(mu - mx);  // 0 when nothing was seen yet
-                    mu = mx;
-                    l *= f;
-                }
-                if (u > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
+                    for (int j = 0; j < 32; ++j)
+                        if (!((bits >> j) & 1u)) v[j] = 0xff800000u;
+                };
+                auto grown = [&](float mx) {  // moves the maximum in use; the rows' sums so far follow
+                    float f = 1.0f;
+                    if (mx > mu + CH_GROW || (mu == -INFINITY && mx > mu)) {
+                        f = ex2(mu - mx);  // 0 when nothing was seen yet
+                        mu = mx;
+                        l *= f;
+                    }
+                    if (u == 0 || !__any_sync(0xffffffffu, f != 1.0f)) return;
                     // P V of the unit before is done (its commit came before this unit's scores')
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
                         uint32_t o[32];
                         ch_ld32(to + 32 * c, o);
@@ -262,23 +303,94 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                         for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
                         ch_st32(to + 32 * c, o);
                     }
-                }
-                const float sub = CH_BIAS - (mu == -INFINITY ? 0.0f : mu);
-                float sum0 = 0.0f, sum1 = 0.0f;
+                };
+                // A unit that every row sees whole: weights by the maximum in use, its own maximum on the way; in
+                // place only if that does not lie too far above.
+                const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2);
+                bool fast = whole && !__any_sync(0xffffffffu, mu == -INFINITY);
+                if (fast) {
+                    const uint64_t sub2 = f2_pack(CH_BIAS - mu, CH_BIAS - mu);
+                    uint64_t acc0 = 0, acc1 = 0;
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
+                    uint32_t v[2][32], w[4][16];
+                    ch_ld32(ts, v[0]);
+                    ch_wait_ld(v[0]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t w[16];
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t(&cur)[32] = v[i & 1];
+                        if (i < 3) ch_ld32(ts + 32 * (i + 1), v[(i + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float e0 = ex2(fmaf(__uint_as_float(s[i][2 * j]), a.scale_log2, sub));
-                        const float e1 = ex2(fmaf(__uint_as_float(s[i][2 * j + 1]), a.scale_log2, sub));
-                        sum0 += e0;
-                        sum1 += e1;
-                        w[j] = pack_f16(e0, e1);
+                        for (int j = 0; j < 16; ++j) {
+                            const float s0 = __uint_as_float(cur[2 * j]), s1 = __uint_as_float(cur[2 * j + 1]);
+                            if (j & 1) mx1 = max3_nan(mx1, s0, s1);
+                            else mx0 = max3_nan(mx0, s0, s1);
+                            const uint64_t t = f2_fma(f2_pack(s0, s1), sc2, sub2);
+                            float2 e;
+                            if (j % C::POLY == C::POLY - 1) {
+                                e = f2_exp2(t);
+                            } else {
+                                e = f2_get(t);
+                                e = make_float2(ex2(e.x), ex2(e.y));
+                            }
+                            if (j & 1) acc1 = f2_add(acc1, f2_pack(e.x, e.y));
+                            else acc0 = f2_add(acc0, f2_pack(e.x, e.y));
+                            w[i][j] = pack_f16(e.x, e.y);
+                        }
+                        if (i < 3) ch_wait_ld(v[(i + 1) & 1]);
                     }
-                    ch_st16(ts + 16 * i, w);
+                    const float mx = max3_nan(mx0, mx1, mx1) * a.scale_log2;
+                    fast = !__any_sync(0xffffffffu, mx > mu + CH_GROW);
+                    if (fast) {
+                        const float2 h = f2_get(f2_add(acc0, acc1));
+                        l += h.x + h.y;
+                        if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);  // NaN or +infinity: the row has no softmax
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ch_st16(ts + 16 * i, w[i]);
+                    }
                 }
-                l += sum0 + sum1;
+                if (!fast) {  // first the maximum, then the weights
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t bits = whole ? ~0u : seen_bits(i);
+                        if (__all_sync(0xffffffffu, bits == 0u)) continue;
+                        uint32_t v[32];
+                        ch_ld32(ts + 32 * i, v);
+                        ch_wait_ld(v);
+                        if (__any_sync(0xffffffffu, bits != ~0u)) hide(v, bits);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) mx = max3_nan(mx, __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+                    }
+                    mx *= a.scale_log2;
+                    if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);
+                    grown(mx);
+                    const float sub = CH_BIAS - (mu == -INFINITY ? 0.0f : mu);
+                    uint64_t acc = 0;
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t bits = whole ? ~0u : seen_bits(i);
+                        uint32_t w[16];
+                        if (__all_sync(0xffffffffu, bits == 0u)) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = 0u;
+                        } else {
+                            uint32_t v[32];
+                            ch_ld32(ts + 32 * i, v);
+                            ch_wait_ld(v);
+                            if (__any_sync(0xffffffffu, bits != ~0u)) hide(v, bits);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const float e0 = ex2(fmaf(__uint_as_float(v[2 * j]), a.scale_log2, sub));
+                                const float e1 = ex2(fmaf(__uint_as_float(v[2 * j + 1]), a.scale_log2, sub));
+                                acc = f2_add(acc, f2_pack(e0, e1));
+                                w[j] = pack_f16(e0, e1);
+                            }
+                        }
+                        ch_st16(ts + 16 * i, w);  // over scores that are read
+                    }
+                    const float2 h = f2_get(acc);
+                    l += h.x + h.y;
+                }
                 ch_wait_st();
                 tc_fence_before();
                 mbar_arrive(&sm.p_full[r]);
@@ -347,7 +459,6 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 8) {
             // ---- MMA issue
             if (lane == 0) {
