@@ -62,7 +62,7 @@ static cudaError_t launch_chunk(PagedAttnArgs a, const PagedPick& p, cudaStream_
     if (DT == GTN_F16 && (!page_map(a.c, a.c.k, box, &km) || !page_map(a.c, a.c.v, box, &vm))) return cudaErrorInvalidValue;
     e = launch_pdl(k_paged_chunk<DT, D>, dim3(ctas), dim3(CH_THREADS), C::SMEM, st, a, p, km, vm, box);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_join<CH_ROWS, D>, dim3((ctas + 3) / 4, 64), dim3(128), 0, st, a, ctas);
+    return launch_pdl(k_paged_join_cols<CH_ROWS, D>, dim3(ctas, CH_ROWS / 128, D / 32), dim3(128), 0, st, a);
 }
 
 static cudaError_t chunk(const PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {

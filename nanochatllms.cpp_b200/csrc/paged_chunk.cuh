@@ -35,7 +35,8 @@ template <int D>
 struct ChunkCfg {
     static constexpr int TILE = 128 * D * 2;  // bytes of a Q, K or V tile
     static constexpr int KS = D == 64 ? 3 : 2, VS = D == 64 ? 3 : 2;
-    static constexpr int SMEM = 1024 + (2 + KS + VS) * TILE + 512;
+    static constexpr int STAGE = 32 * 64;  // bytes per softmax warp: 32 rows x 32 fp16 outputs on their way out
+    static constexpr int SMEM = 1024 + (2 + KS + VS) * TILE + 8 * STAGE;
     static constexpr int POLY = D == 64 ? 3 : 4;  // every POLY-th pair of exponentials on the multiply-add pipe
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
     // kind::f16, A = B = fp16, D = fp32; scores: both K-major, N = 128; output: B (V) MN-major, N = D
@@ -50,13 +51,37 @@ __device__ __forceinline__ uint64_t ch_desc(uint32_t saddr, uint32_t lbo) {
     return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024u >> 4) << 32) |
            (1ull << 46) | (2ull << 61);
 }
-// D (+)= A B with A in TMEM.
-__device__ __forceinline__ void ch_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Called by a whole converged warp, done by its `leader` lane: so all operands are warp-uniform and stay in
+// uniform registers (issued from a divergent lane, each MMA cost some 85 cycles of register moves, more than it
+// runs).
+__device__ __forceinline__ void ch_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
+}
+// A in TMEM.
+__device__ __forceinline__ void ch_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
+                                          uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void ch_commit(uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+        "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t ch_elect() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}\n" : "=r"(r));
+    return r;
 }
 #define CH_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
 #define CH_U8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
@@ -146,12 +171,30 @@ __device__ __forceinline__ float2 f2_exp2(uint64_t x) {
 
 struct ChunkSmem {
     uint64_t k_full[3], k_empty[3], v_load[3], v_full[3], v_empty[3];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drain;  // p_full: per tile, 64 keys each
     uint32_t tmem;
     volatile int abort;
     volatile int odd;  // a non-finite value was set aside (stays set)
     PagedSchedSmem<1> sched;
 };
+
+// Adds the values that were set aside (non-finite) to a row's columns c0 .. c0 + 31, as far as it sees them.
+static __device__ __noinline__ void ch_add_odd(const PagedAttnArgs& a, const PagedPos& x, int u0, int u1, int pos, int wlo,
+                                               int c0, float (&v)[32]) {
+    for (int u = u0; u < u1; ++u) {
+        const int kb = paged_unit_key<CH_KEYS>(x.t, u);
+        for (int key = kb; key < kb + CH_KEYS && key <= pos; ++key) {
+            if (key < wlo && key >= a.n_sink) continue;
+            const int page = a.table[x.b * a.table_stride + (key >> a.c.ps_shift)];
+            if ((unsigned)page >= (unsigned)a.c.n_pages) continue;
+            const uint8_t* pg = a.c.v + (long)page * a.c.page_stride;
+            for (int j = 0; j < 32; ++j) {
+                const float y = paged_elem(a.c, pg, x.h, key & (a.c.ps - 1), c0 + j);
+                if (!(fabsf(y) < INFINITY)) v[j] += y;
+            }
+        }
+    }
+}
 
 template <int DT, int D>
 __global__ void __launch_bounds__(CH_THREADS, 1)
@@ -182,7 +225,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         for (int r = 0; r < 2; ++r) {
             mbar_init(&sm.q_full[r], 128);
             mbar_init(&sm.s_full[r], 1);
-            mbar_init(&sm.p_full[r], 128);
+            mbar_init(&sm.p_full[r][0], 128);
+            mbar_init(&sm.p_full[r][1], 128);
             mbar_init(&sm.o_full[r], 1);
         }
         mbar_init(&sm.drain, 1);
@@ -214,17 +258,24 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         if (n == x.t.ns) n += max(0, phi / CH_KEYS - x.t.w0 + 1);
         return max(0, min(u1, n) - u0);
     };
-    auto wait1 = [&](uint64_t* bar, uint32_t ph) {
-        if (sm.abort == 0 && tc_wait(bar, ph, a.err)) return true;
-        sm.abort = 1;
-        return false;
+    // by a whole warp; false once a wait of the CTA has run out
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+        bool got = mbar_try_wait(bar, ph);
+        if (!__all_sync(0xffffffffu, got)) {
+            got = got || (sm.abort == 0 && tc_wait(bar, ph, a.err));
+            if (!__all_sync(0xffffffffu, got)) {
+                sm.abort = 1;
+                return false;
+            }
+        }
+        return true;
     };
-    auto wait = [&](uint64_t* bar, uint32_t ph) { return __all_sync(0xffffffffu, wait1(bar, ph)) != 0; };  // a whole warp
-    // a unit that every row of the item sees whole
-    auto seen_whole = [&](int kb) {
-        const int lo = a.window > 0 ? max(0, x.t.phi - a.window + 1) : 0;
-        return kb + CH_KEYS - 1 <= x.t.plo && (kb >= lo || kb + CH_KEYS <= a.n_sink);
+    // a unit that every row of the item (of the positions plo .. phi) sees whole
+    auto whole_for = [&](int kb, int plo, int phi) {
+        const int lo = a.window > 0 ? max(0, phi - a.window + 1) : 0;
+        return kb + CH_KEYS - 1 <= plo && (kb >= lo || kb + CH_KEYS <= a.n_sink);
     };
+    auto seen_whole = [&](int kb) { return whole_for(kb, x.t.plo, x.t.phi); };
     auto next_item = [&](int done) {
         left -= done;
         if (left > 0) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
@@ -242,16 +293,25 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         // The row's query into the swizzled tile. Not for a tile without units: its softmax waits for nothing
         // and could pass q_full twice before the MMA warp looks.
         auto load_q = [&]() {
-            const int m = x.tile * CH_ROWS + r * 128 + row;
             if (tile_units(r, x.u, min(x.t.units, x.u + left)) == 0) return;
-            const bool in = m < x.r.n * a.group;
-            const uint8_t* qh =
-                a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, r * 128 + row, CH_ROWS, a.qs, hb) : 0);
+            // D / 8 adjacent lanes per row
+            constexpr int CPR = D / 8;
+            const int c = lane % CPR;
+            uint4 v[CPR];
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                const uint4 v = in ? paged_q8x(qh, a.io, 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t dst = qs + (c >> 3) * HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+            for (int i = 0; i < CPR; ++i) {
+                const int rw = r * 128 + (warp & 3) * 32 + i * (32 / CPR) + lane / CPR;
+                const bool in = x.tile * CH_ROWS + rw < x.r.n * a.group;
+                const uint8_t* qh = a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, rw, CH_ROWS, a.qs, hb) : 0);
+                v[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (in) v[i] = paged_q8x(qh, a.io, 8 * c);
+            }
+#pragma unroll
+            for (int i = 0; i < CPR; ++i) {
+                const int rw = (warp & 3) * 32 + i * (32 / CPR) + lane / CPR;
+                const uint32_t dst = qs + (c >> 3) * HALF + rw * 128 + (((c & 7) ^ (rw & 7)) << 4);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z),
+                             "r"(v[i].w)
                              : "memory");
             }
             fence_async_smem();
@@ -264,6 +324,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             const bool live = m_row < x.r.n * a.group;
             const int pos = live ? x.r.base + m_row / a.group : -1;
             const int wlo = a.window > 0 ? pos - a.window + 1 : 0;
+            // positions of this tile's first and last row
+            const int t0 = x.tile * CH_ROWS + r * 128;
+            const int tlo = x.r.base + t0 / a.group, thi = x.r.base + min(x.r.n - 1, (t0 + 127) / a.group);
             // the maximum in use (base 2; a row behind the item's last needs none), the sum of weights
             float mu = live ? -INFINITY : 0.0f, l = 0.0f;
             for (int u = 0; u < n; ++u) {
@@ -271,7 +334,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 s_ph ^= 1u;
                 tc_fence_after();
                 const int kb = paged_unit_key<CH_KEYS>(x.t, u0 + u);
-                const bool whole = seen_whole(kb);
+                const bool whole = whole_for(kb, tlo, thi);
                 // the keys of chunk i (32) that this row sees, as bits
                 auto seen_bits = [&](int i) -> uint32_t {
                     const int k0 = kb + 32 * i;
@@ -304,27 +367,50 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                         ch_st32(to + 32 * c, o);
                     }
                 };
-                // A unit that every row sees whole: weights by the maximum in use, its own maximum on the way; in
-                // place only if that does not lie too far above.
-                const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2);
-                bool fast = whole && !__any_sync(0xffffffffu, mu == -INFINITY);
-                if (fast) {
-                    const uint64_t sub2 = f2_pack(CH_BIAS - mu, CH_BIAS - mu);
-                    uint64_t acc0 = 0, acc1 = 0;
-                    float mx0 = -INFINITY, mx1 = -INFINITY;
-                    uint32_t v[2][32], w[4][16];
-                    ch_ld32(ts, v[0]);
+                // first the maximum, then the weights, 64 keys at a time
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll 1
+                for (int i = 0; i < 4; i += 2) {
+                    uint32_t v[2][32];
+                    ch_ld32(ts + 32 * i, v[0]);
+                    ch_ld32(ts + 32 * i + 32, v[1]);
                     ch_wait_ld(v[0]);
+                    ch_wait_ld(v[1]);
+                    if (!whole) {
+                        const uint32_t b0 = seen_bits(i), b1 = seen_bits(i + 1);
+                        if (__any_sync(0xffffffffu, b0 != ~0u)) hide(v[0], b0);
+                        if (__any_sync(0xffffffffu, b1 != ~0u)) hide(v[1], b1);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t(&cur)[32] = v[i & 1];
-                        if (i < 3) ch_ld32(ts + 32 * (i + 1), v[(i + 1) & 1]);
+                    for (int j = 0; j < 32; j += 2) {
+                        mx0 = max3_nan(mx0, __uint_as_float(v[0][j]), __uint_as_float(v[0][j + 1]));
+                        mx1 = max3_nan(mx1, __uint_as_float(v[1][j]), __uint_as_float(v[1][j + 1]));
+                    }
+                }
+                const float mx = max3_nan(mx0, mx1, mx1) * a.scale_log2;
+                if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);  // NaN or +infinity: the row has no softmax
+                grown(mx);
+                const float sub = CH_BIAS - (mu == -INFINITY ? 0.0f : mu);
+                const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), sub2 = f2_pack(sub, sub);
+                uint64_t acc0 = 0, acc1 = 0;
+#pragma unroll 1
+                for (int i = 0; i < 4; i += 2) {
+                    uint32_t v[2][32], w[32];
+                    ch_ld32(ts + 32 * i, v[0]);
+                    ch_ld32(ts + 32 * i + 32, v[1]);
+                    ch_wait_ld(v[0]);
+                    ch_wait_ld(v[1]);
+                    if (!whole) {
+                        const uint32_t b0 = seen_bits(i), b1 = seen_bits(i + 1);
+                        if (__any_sync(0xffffffffu, b0 != ~0u)) hide(v[0], b0);
+                        if (__any_sync(0xffffffffu, b1 != ~0u)) hide(v[1], b1);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            const float s0 = __uint_as_float(cur[2 * j]), s1 = __uint_as_float(cur[2 * j + 1]);
-                            if (j & 1) mx1 = max3_nan(mx1, s0, s1);
-                            else mx0 = max3_nan(mx0, s0, s1);
-                            const uint64_t t = f2_fma(f2_pack(s0, s1), sc2, sub2);
+                            const uint64_t t =
+                                f2_fma(f2_pack(__uint_as_float(v[h][2 * j]), __uint_as_float(v[h][2 * j + 1])), sc2, sub2);
                             float2 e;
                             if (j % C::POLY == C::POLY - 1) {
                                 e = f2_exp2(t);
@@ -334,66 +420,15 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                             }
                             if (j & 1) acc1 = f2_add(acc1, f2_pack(e.x, e.y));
                             else acc0 = f2_add(acc0, f2_pack(e.x, e.y));
-                            w[i][j] = pack_f16(e.x, e.y);
+                            w[16 * h + j] = pack_f16(e.x, e.y);
                         }
-                        if (i < 3) ch_wait_ld(v[(i + 1) & 1]);
-                    }
-                    const float mx = max3_nan(mx0, mx1, mx1) * a.scale_log2;
-                    fast = !__any_sync(0xffffffffu, mx > mu + CH_GROW);
-                    if (fast) {
-                        const float2 h = f2_get(f2_add(acc0, acc1));
-                        l += h.x + h.y;
-                        if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);  // NaN or +infinity: the row has no softmax
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ch_st16(ts + 16 * i, w[i]);
-                    }
+                    ch_st32(ts + 16 * i, w);  // over scores that are read
+                    ch_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&sm.p_full[r][i >> 1]);
                 }
-                if (!fast) {  // first the maximum, then the weights
-                    float mx = -INFINITY;
-#pragma unroll 1
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t bits = whole ? ~0u : seen_bits(i);
-                        if (__all_sync(0xffffffffu, bits == 0u)) continue;
-                        uint32_t v[32];
-                        ch_ld32(ts + 32 * i, v);
-                        ch_wait_ld(v);
-                        if (__any_sync(0xffffffffu, bits != ~0u)) hide(v, bits);
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) mx = max3_nan(mx, __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
-                    }
-                    mx *= a.scale_log2;
-                    if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);
-                    grown(mx);
-                    const float sub = CH_BIAS - (mu == -INFINITY ? 0.0f : mu);
-                    uint64_t acc = 0;
-#pragma unroll 1
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t bits = whole ? ~0u : seen_bits(i);
-                        uint32_t w[16];
-                        if (__all_sync(0xffffffffu, bits == 0u)) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) w[j] = 0u;
-                        } else {
-                            uint32_t v[32];
-                            ch_ld32(ts + 32 * i, v);
-                            ch_wait_ld(v);
-                            if (__any_sync(0xffffffffu, bits != ~0u)) hide(v, bits);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const float e0 = ex2(fmaf(__uint_as_float(v[2 * j]), a.scale_log2, sub));
-                                const float e1 = ex2(fmaf(__uint_as_float(v[2 * j + 1]), a.scale_log2, sub));
-                                acc = f2_add(acc, f2_pack(e0, e1));
-                                w[j] = pack_f16(e0, e1);
-                            }
-                        }
-                        ch_st16(ts + 16 * i, w);  // over scores that are read
-                    }
-                    const float2 h = f2_get(acc);
-                    l += h.x + h.y;
-                }
-                ch_wait_st();
-                tc_fence_before();
-                mbar_arrive(&sm.p_full[r]);
+                const float2 h = f2_get(f2_add(acc0, acc1));
+                l += h.x + h.y;
             }
             // the next item's queries go in before this item's output comes out: all products with this item's
             // are done (its last scores were seen)
@@ -412,6 +447,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<CH_ROWS, D>();
                 uint8_t* dst =
                     a.out + (live ? paged_row_at(a, was.r.first, was.h, was.tile, prow, CH_ROWS, a.os, hb) : 0);
+                const uint32_t stage = sq + (2 + C::KS + C::VS) * C::TILE + warp * C::STAGE;
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
@@ -422,31 +458,36 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     }
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = n > 0 ? __uint_as_float(o[j]) : 0.0f;
-                    if (n > 0 && sm.odd != 0) {
-                        // values set aside: the non-finite ones that this row sees
-                        for (int u = u0; u < u1; ++u) {
-                            const int kb = paged_unit_key<CH_KEYS>(was.t, u);
-                            for (int key = kb; key < kb + CH_KEYS && key <= pos; ++key) {
-                                if (key < wlo && key >= a.n_sink) continue;
-                                const int page = a.table[was.b * a.table_stride + (key >> a.c.ps_shift)];
-                                if ((unsigned)page >= (unsigned)a.c.n_pages) continue;
-                                const uint8_t* pg = a.c.v + (long)page * a.c.page_stride;
+                    if (n > 0 && sm.odd != 0) ch_add_odd(a, was, u0, u1, pos, wlo, 32 * c, v);
+                    if (!done) {
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) {
-                                    const float y = paged_elem(a.c, pg, was.h, key & (a.c.ps - 1), 32 * c + j);
-                                    if (!(fabsf(y) < INFINITY)) v[j] += y;
-                                }
-                            }
-                        }
+                        for (int j = 0; j < 32; ++j) ps[(long)(32 * c + j) * CH_ROWS + prow] = v[j];
+                        continue;
                     }
-                    if (done) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = l != 0.0f ? v[j] * inv : 0.0f;
+                    for (int j = 0; j < 32; ++j) v[j] = l != 0.0f ? v[j] * inv : 0.0f;
+                    if (a.io != GTN_F16) {
                         paged_store<32>(dst, a.io, 32 * c, v, live);
-                    } else if (live) {
-                        float4* q4 = reinterpret_cast<float4*>(ps + (long)prow * D + 32 * c);
+                        continue;
+                    }
+                    // through shared memory, so that four adjacent lanes write a row's 64 bytes
+                    __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) q4[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    for (int j = 0; j < 4; ++j)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                         stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
+                                     "r"(pack_f16(v[8 * j], v[8 * j + 1])), "r"(pack_f16(v[8 * j + 2], v[8 * j + 3])),
+                                     "r"(pack_f16(v[8 * j + 4], v[8 * j + 5])), "r"(pack_f16(v[8 * j + 6], v[8 * j + 7]))
+                                     : "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int lr = 8 * i + (lane >> 2), rw = r * 128 + (warp & 3) * 32 + lr;
+                        const uint4 y = lds16(stage + lr * 64 + (((lane & 3) ^ ((lr >> 1) & 3)) << 4));
+                        if (was.tile * CH_ROWS + rw < was.r.n * a.group)
+                            *reinterpret_cast<uint4*>(
+                                a.out + paged_row_at(a, was.r.first, was.h, was.tile, rw, CH_ROWS, a.os, hb) + 64 * c +
+                                16 * (lane & 3)) = y;
                     }
                 }
                 if (!done && live) {
@@ -461,63 +502,68 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
     } else {
         if (warp == 8) {
             // ---- MMA issue
-            if (lane == 0) {
-                int ks = 0, vs = 0;
-                uint32_t k_ph = 0, v_ph = 0, q_ph = 0, p_ph[2] = {0, 0};
-                bool ok = true;
-                auto qk = [&](int r) {
+            const uint32_t leader = ch_elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t q0 = __shfl_sync(0xffffffffu, sq, 0);
+            const uint32_t k0 = q0 + 2 * C::TILE, v0 = k0 + C::KS * C::TILE;
+            int ks = 0, vs = 0;
+            uint32_t k_ph = 0, v_ph = 0, q_ph = 0, p_ph = 0;
+            bool ok = true;
+            auto qk = [&](int r) {
+                const uint64_t qd = ch_desc(q0 + r * C::TILE, 16), kd = ch_desc(k0 + ks * C::TILE, 16);
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t off = (i >> 2) * HALF + (i & 3) * 32;
-                        tc_mma(tmem + r * 128, ch_desc(sq + r * C::TILE + off, 16), ch_desc(sk + ks * C::TILE + off, 16),
-                               C::IDESC_S, i > 0);
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint32_t off = ((i >> 2) * HALF + (i & 3) * 32) >> 4;
+                    ch_mma_ss(tm + r * 128, qd + off, kd + off, C::IDESC_S, i > 0, leader);
+                }
+                ch_commit(&sm.s_full[r], leader);
+            };
+            while (left > 0 && ok) {
+                const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = u1 - u0;
+                const int nr0 = tile_units(0, u0, u1), nr1 = tile_units(1, u0, u1);
+                ok = wait(&sm.k_full[ks], k_ph);
+                for (int r = 0; r < 2 && ok; ++r) {
+                    if ((r ? nr1 : nr0) == 0) continue;
+                    ok = wait(&sm.q_full[r], (q_ph >> r) & 1u);
+                    q_ph ^= 1u << r;
+                    tc_fence_after();
+                    if (ok) qk(r);
+                }
+                for (int u = 0; u < n && ok; ++u) {
+                    ch_commit(&sm.k_empty[ks], leader);  // the scores of unit u are issued
+                    if (++ks == C::KS) {
+                        ks = 0;
+                        k_ph ^= 1u;
                     }
-                    tc_commit(&sm.s_full[r]);
-                };
-                while (left > 0 && ok) {
-                    const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = u1 - u0;
-                    const int nr[2] = {tile_units(0, u0, u1), tile_units(1, u0, u1)};
-                    ok = wait1(&sm.k_full[ks], k_ph);
+                    if (u + 1 < n) ok = wait(&sm.k_full[ks], k_ph);
+                    if (ok) ok = wait(&sm.v_full[vs], v_ph);
                     for (int r = 0; r < 2 && ok; ++r) {
-                        if (nr[r] == 0) continue;
-                        ok = wait1(&sm.q_full[r], (q_ph >> r) & 1u);
-                        q_ph ^= 1u << r;
-                        tc_fence_after();
-                        if (ok) qk(r);
-                    }
-                    for (int u = 0; u < n && ok; ++u) {
-                        tc_commit(&sm.k_empty[ks]);  // the scores of unit u are issued
-                        if (++ks == C::KS) {
-                            ks = 0;
-                            k_ph ^= 1u;
-                        }
-                        if (u + 1 < n) ok = wait1(&sm.k_full[ks], k_ph);
-                        if (ok) ok = wait1(&sm.v_full[vs], v_ph);
-                        for (int r = 0; r < 2 && ok; ++r) {
-                            if (u >= nr[r]) continue;
-                            if (!(ok = wait1(&sm.p_full[r], p_ph[r]))) break;
-                            p_ph[r] ^= 1u;
+                        const int nr = r ? nr1 : nr0;
+                        if (u >= nr) continue;
+                        const uint64_t vd = ch_desc(v0 + vs * C::TILE, HALF);
+                        for (int h = 0; h < 2 && ok; ++h) {
+                            if (!(ok = wait(&sm.p_full[r][h], (p_ph >> r) & 1u))) break;
                             tc_fence_after();
 #pragma unroll
-                            for (int i = 0; i < CH_KEYS / 16; ++i)
-                                ch_mma_ts(tmem + C::COL_O + r * D, tmem + r * 128 + i * 8,
-                                          ch_desc(sv + vs * C::TILE + i * 2048, HALF), C::IDESC_O, u > 0 || i > 0);
-                            if (u + 1 < nr[r]) qk(r);
-                            else tc_commit(&sm.o_full[r]);
+                            for (int i = 0; i < CH_KEYS / 32; ++i)
+                                ch_mma_ts(tm + C::COL_O + r * D, tm + r * 128 + (4 * h + i) * 8,
+                                          vd + ((4 * h + i) * 2048 >> 4), C::IDESC_O, u > 0 || h > 0 || i > 0, leader);
                         }
                         if (!ok) break;
-                        tc_commit(&sm.v_empty[vs]);
-                        if (++vs == C::VS) {
-                            vs = 0;
-                            v_ph ^= 1u;
-                        }
+                        p_ph ^= 1u << r;
+                        if (u + 1 < nr) qk(r);
+                        else ch_commit(&sm.o_full[r], leader);
                     }
-                    next_item(n);
+                    if (!ok) break;
+                    ch_commit(&sm.v_empty[vs], leader);
+                    if (++vs == C::VS) {
+                        vs = 0;
+                        v_ph ^= 1u;
+                    }
                 }
-                tc_commit(&sm.drain);  // nothing of this CTA is in flight behind this
-                tc_wait(&sm.drain, 0, a.err);
+                next_item(n);
             }
-            __syncwarp();
+            ch_commit(&sm.drain, leader);  // nothing of this CTA is in flight behind this
+            tc_wait(&sm.drain, 0, a.err);
         } else if (!Q8 && warp == 9) {
             // ---- fetch of fp16 pages: lane i issues the boxes of piece i (`box` rows) of a unit
             int ks = 0, vs = 0, k_issued = 0, v_issued = 0;
@@ -617,88 +663,109 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 next_item(u1 - u0);
             }
         } else {
-            // ---- Q8 pages to fp16 tiles: 96 threads, 16 elements of a row at a time
+            // ---- Q8 pages to fp16 tiles: a warp takes groups of RPG rows (of one page), lane = 16 elements; the
+            // next tile's bytes are on their way while one is converted
             int ks = 0, vs = 0;
             uint32_t k_ph = 1, v_ph = 1;
             bool ok = true;
-            const int ct = tid - 288;
-            constexpr int CPR = D / 16, CHUNKS = 128 * CPR;  // 16-element chunks of a row, of a tile
-            constexpr int PER = (CHUNKS + 95) / 96;
-            while (left > 0 && ok) {
-                const int u0 = x.u, u1 = min(x.t.units, u0 + left);
-                const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
-                for (int u = u0; u < u1 && ok; ++u) {
-                    const int kb = paged_unit_key<CH_KEYS>(x.t, u);
-                    const bool whole = seen_whole(kb);
-#pragma unroll 1
-                    for (int kv = 0; kv < 2; ++kv) {
-                        const uint8_t* pool = kv ? a.c.v : a.c.k;
-                        uint4 raw[PER];
-                        uint16_t dl[PER];
-#pragma unroll
-                        for (int i = 0; i < PER; ++i) {
-                            const int ch = ct + 96 * i, row = ch / CPR, key = kb + row;
-                            raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                            dl[i] = 0;
-                            if (ch < CHUNKS && key <= x.t.phi && (key >= lo || key < a.n_sink)) {
-                                const int page = a.table[x.b * a.table_stride + (key >> a.c.ps_shift)];
-                                if ((unsigned)page < (unsigned)a.c.n_pages) {
-                                    const uint8_t* pg = pool + (long)page * a.c.page_stride;
-                                    const int pr = key & (a.c.ps - 1), e = ch % CPR * 16;
-                                    raw[i] = *reinterpret_cast<const uint4*>(pg + paged_row(a.c, x.h, pr) + e);
-                                    dl[i] = reinterpret_cast<const uint16_t*>(pg + paged_delta(a.c, x.h, pr))[e / GTN_QBLK];
-                                } else {
-                                    atomicOr(a.err, GTN_DEVERR_PAGE);
-                                }
-                            }
-                        }
-                        if (!(ok = kv ? wait(&sm.v_empty[vs], v_ph) : wait(&sm.k_empty[ks], k_ph))) break;
-                        const uint32_t tile = kv ? sv + vs * C::TILE : sk + ks * C::TILE;
-#pragma unroll
-                        for (int i = 0; i < PER; ++i) {
-                            const int ch = ct + 96 * i, row = ch / CPR, c16 = ch % CPR;
-                            if (ch >= CHUNKS) continue;
-                            const __half2 d2 = __half2half2(__ushort_as_half(dl[i]));
-                            const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                            uint32_t w[8];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint2 b = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
-                                const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&b.x), d2);
-                                const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&b.y), d2);
-                                w[2 * j] = *reinterpret_cast<const uint32_t*>(&h0);
-                                w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
-                            }
-                            if (kv && !whole) {
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    if ((w[j] & 0x7c00u) == 0x7c00u) { w[j] &= 0xffff0000u; sm.odd = 1; }
-                                    if ((w[j] & 0x7c000000u) == 0x7c000000u) { w[j] &= 0x0000ffffu; sm.odd = 1; }
-                                }
-                            }
-                            const uint32_t at = tile + (c16 >> 2) * HALF + row * 128;
-#pragma unroll
-                            for (int j = 0; j < 2; ++j)
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                                 at + ((((2 * c16 + j) & 7) ^ (row & 7)) << 4)),
-                                             "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
-                                             : "memory");
-                        }
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(kv ? &sm.v_full[vs] : &sm.k_full[ks]);
-                    }
-                    if (!ok) break;
-                    if (++ks == C::KS) {
-                        ks = 0;
-                        k_ph ^= 1u;
-                    }
-                    if (++vs == C::VS) {
-                        vs = 0;
-                        v_ph ^= 1u;
+            constexpr int CPR = D / 16, RPG = 32 / CPR, GROUPS = 128 / RPG, PER = (GROUPS + 2) / 3;
+            const int lrow = lane / CPR, c16 = lane % CPR, w3 = warp - 9;
+            uint4 kraw[PER], vraw[PER];
+            uint16_t kdl[PER], vdl[PER];
+            int page = 0;  // lane i < 8: the page of the unit's 16-key piece i, -1 for none
+            auto find_pages = [&](int kb) {
+                const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0, k0 = kb + 16 * lane;
+                page = -1;
+                if (lane < 8 && k0 <= x.t.phi && (k0 + 15 >= lo || k0 < a.n_sink)) {
+                    page = a.table[x.b * a.table_stride + (k0 >> a.c.ps_shift)];
+                    if ((unsigned)page >= (unsigned)a.c.n_pages) {
+                        page = -1;
+                        atomicOr(a.err, GTN_DEVERR_PAGE);
                     }
                 }
-                next_item(u1 - u0);
+            };
+            auto load = [&](const uint8_t* pool, int kb, uint4 (&raw)[PER], uint16_t (&dl)[PER]) {
+                const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
+                const bool all = kb + CH_KEYS - 1 <= x.t.phi && (kb >= lo || kb + CH_KEYS <= a.n_sink);
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int grp = w3 + 3 * i, k0 = kb + grp * RPG, key = k0 + lrow;
+                    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                    dl[i] = 0;
+                    if (GROUPS % 3 != 0 && grp >= GROUPS) continue;
+                    const int pgi = __shfl_sync(0xffffffffu, page, grp * RPG / 16);
+                    if (pgi >= 0 && (all || (key <= x.t.phi && (key >= lo || key < a.n_sink)))) {
+                        const uint8_t* pg = pool + (long)pgi * a.c.page_stride;
+                        const int cell = x.h * a.c.ps + (key & (a.c.ps - 1));  // row among the page's
+                        raw[i] = *reinterpret_cast<const uint4*>(pg + cell * D + c16 * 16);
+                        dl[i] = *reinterpret_cast<const uint16_t*>(pg + a.c.kv_heads * a.c.ps * D + (cell * (D / 32) + (c16 >> 1)) * 2);
+                    }
+                }
+            };
+            auto convert = [&](uint32_t tile, bool scan, const uint4 (&raw)[PER], const uint16_t (&dl)[PER]) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int grp = w3 + 3 * i, row = grp * RPG + lrow;
+                    if (GROUPS % 3 != 0 && grp >= GROUPS) continue;
+                    const __half2 d2 = __half2half2(__ushort_as_half(dl[i]));
+                    const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint2 b = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
+                        const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&b.x), d2);
+                        const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&b.y), d2);
+                        w[2 * j] = *reinterpret_cast<const uint32_t*>(&h0);
+                        w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                    }
+                    if (scan) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            if ((w[j] & 0x7c00u) == 0x7c00u) { w[j] &= 0xffff0000u; sm.odd = 1; }
+                            if ((w[j] & 0x7c000000u) == 0x7c000000u) { w[j] &= 0x0000ffffu; sm.odd = 1; }
+                        }
+                    }
+                    const uint32_t at = tile + (c16 >> 2) * HALF + row * 128;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                         at + ((((2 * c16 + j) & 7) ^ (row & 7)) << 4)),
+                                     "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                                     : "memory");
+                }
+                fence_async_smem();
+                __syncwarp();
+            };
+            if (left > 0) {
+                find_pages(paged_unit_key<CH_KEYS>(x.t, x.u));
+                load(a.c.k, paged_unit_key<CH_KEYS>(x.t, x.u), kraw, kdl);
+            }
+            while (left > 0 && ok) {
+                const int kb = paged_unit_key<CH_KEYS>(x.t, x.u);
+                const bool scan = !seen_whole(kb);
+                load(a.c.v, kb, vraw, vdl);
+                if (!(ok = wait(&sm.k_empty[ks], k_ph))) break;
+                convert(sk + ks * C::TILE, false, kraw, kdl);
+                if (lane == 0) mbar_arrive(&sm.k_full[ks]);
+                // the next unit, of this item or the next
+                --left;
+                if (left > 0) {
+                    if (++x.u == x.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
+                    find_pages(paged_unit_key<CH_KEYS>(x.t, x.u));
+                }
+                if (!(ok = wait(&sm.v_empty[vs], v_ph))) break;
+                // (the page numbers asked for above are here by now)
+                if (left > 0) load(a.c.k, paged_unit_key<CH_KEYS>(x.t, x.u), kraw, kdl);
+                convert(sv + vs * C::TILE, scan, vraw, vdl);
+                if (lane == 0) mbar_arrive(&sm.v_full[vs]);
+                if (++ks == C::KS) {
+                    ks = 0;
+                    k_ph ^= 1u;
+                }
+                if (++vs == C::VS) {
+                    vs = 0;
+                    v_ph ^= 1u;
+                }
             }
         }
     }

@@ -91,12 +91,33 @@ __device__ __forceinline__ int paged_tiles(const PagedAttnArgs& a, const PagedPi
     const int m = r.n * a.group;
     return r.n > 0 && (m <= p.cut) == p.below ? (m + ROWS - 1) / ROWS : 0;
 }
+// The units of each lane's request (nt row tiles; one kv head), by a whole warp: a request of more than two
+// tiles is summed by all lanes.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ long long paged_req_units(const PagedAttnArgs& a, const PagedPick& p, const PagedReq& r) {
-    const int nt = paged_tiles<ROWS>(a, p, r);
+__device__ __forceinline__ long long paged_req_units(const PagedAttnArgs& a, const PagedReq& r, int nt) {
+    const int lane = threadIdx.x & 31;
     long long s = 0;
-    for (int t = 0; t < nt; ++t) s += paged_tile<ROWS, KEYS>(a, r, t).units;
+    if (nt <= 2)
+        for (int t = 0; t < nt; ++t) s += paged_tile<ROWS, KEYS>(a, r, t).units;
+    for (unsigned big = __ballot_sync(0xffffffffu, nt > 2); big; big &= big - 1) {
+        const int src = __ffs(big) - 1, n = __shfl_sync(0xffffffffu, nt, src);
+        PagedReq q;
+        q.first = 0;
+        q.n = __shfl_sync(0xffffffffu, r.n, src);
+        q.base = __shfl_sync(0xffffffffu, r.base, src);
+        long long one = 0;
+        for (int t = lane; t < n; t += 32) one += paged_tile<ROWS, KEYS>(a, q, t).units;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+        if (lane == src) s = one;
+    }
     return s;
+}
+
+// a / b for a >= 0, b > 0; in 32 bits where they do.
+__device__ __forceinline__ long long paged_div(long long a, long long b) {
+    if (((a | b) >> 31) == 0) return (long long)((unsigned)a / (unsigned)b);
+    return a / b;
 }
 
 // A position on the line of units: item (b, h, tile), unit u of it, the item's first position.
@@ -120,9 +141,21 @@ __device__ __forceinline__ long long paged_sched(const PagedAttnArgs& a, const P
                                                  bool flag, PagedSchedSmem<W>& sm) {
     constexpr int NW = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (a.n_req + THREADS - 1) / THREADS, b0 = min(a.n_req, tid * per), b1 = min(a.n_req, b0 + per);
+    // thread tid holds requests [b0, b0 + per); every warp runs all `per` steps
+    const int per = (a.n_req + THREADS - 1) / THREADS, b0 = tid * per;
+    auto request = [&](int i, PagedReq& r, bool fl) {
+        r.first = r.n = r.base = 0;
+        if (b0 + i >= a.n_req) return 0;
+        r = paged_req(a, b0 + i, fl);
+        return paged_tiles<ROWS>(a, p, r);
+    };
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += paged_req_units<ROWS, KEYS>(a, p, paged_req(a, b, flag)) * a.c.kv_heads;
+    for (int i = 0; i < per; ++i) {
+        PagedReq r;
+        const int nt = request(i, r, flag);
+        mine += paged_req_units<ROWS, KEYS>(a, r, nt);
+    }
+    mine *= a.c.kv_heads;
     long long s = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -139,35 +172,59 @@ __device__ __forceinline__ long long paged_sched(const PagedAttnArgs& a, const P
         total += sm.warp[w];
     }
     before += s - mine;
-    const long long share = (total + workers - 1) / workers;
+    const long long share = paged_div(total + workers - 1, workers);
     for (int i = 0; i < W; ++i) {
         const long long at = share * (first + i);
-        if (at >= total || at < before || at >= before + mine) continue;
-        long long left = at - before, start = before;
-        for (int b = b0; b < b1; ++b) {
-            const PagedReq q = paged_req(a, b, false);
-            const long long one = paged_req_units<ROWS, KEYS>(a, p, q), all = one * a.c.kv_heads;
+        const unsigned own = __ballot_sync(0xffffffffu, at < total && at >= before && at < before + mine);
+        if (!own) continue;
+        // the warp of the thread whose requests hold the position finds the request, head and tile together
+        const int src = __ffs(own) - 1;
+        long long start = __shfl_sync(0xffffffffu, before, src), left = at - start;
+        bool found = false;
+        for (int j = 0; j < per && !found; ++j) {
+            PagedReq r;
+            const int nt = request(j, r, false);
+            const long long mine_one = paged_req_units<ROWS, KEYS>(a, r, nt);
+            const long long one = __shfl_sync(0xffffffffu, mine_one, src), all = one * a.c.kv_heads;
             if (left >= all) {
                 left -= all;
                 start += all;
                 continue;
             }
+            found = true;
             PagedPos x;
-            x.b = b;
-            x.r = q;
-            x.h = (int)(left / one);
+            x.b = __shfl_sync(0xffffffffu, b0 + j, src);
+            x.r.first = __shfl_sync(0xffffffffu, r.first, src);
+            x.r.n = __shfl_sync(0xffffffffu, r.n, src);
+            x.r.base = __shfl_sync(0xffffffffu, r.base, src);
+            const int tiles = __shfl_sync(0xffffffffu, nt, src);
+            x.h = (int)paged_div(left, one);
             left -= x.h * one;
             start += x.h * one;
-            for (x.tile = 0;; ++x.tile) {
-                x.t = paged_tile<ROWS, KEYS>(a, q, x.tile);
-                if (left < x.t.units) break;
-                left -= x.t.units;
-                start += x.t.units;
+            for (int t0 = 0;; t0 += 32) {  // 32 tiles at a time: the first whose end lies behind the position
+                const int t = t0 + lane;
+                const long long mu = t < tiles ? paged_tile<ROWS, KEYS>(a, x.r, t).units : 0;
+                long long e = mu;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long y = __shfl_up_sync(0xffffffffu, e, o);
+                    if (lane >= o) e += y;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, e > left);
+                if (hit || t0 + 32 >= tiles) {
+                    const int l = hit ? __ffs(hit) - 1 : 31;
+                    const long long st = __shfl_sync(0xffffffffu, e - mu, l);
+                    x.tile = t0 + l;
+                    x.u = (int)(left - st);
+                    x.start = start + st;
+                    break;
+                }
+                const long long e31 = __shfl_sync(0xffffffffu, e, 31);
+                left -= e31;
+                start += e31;
             }
-            x.u = (int)left;
-            x.start = start;
-            sm.pos[i] = x;
-            break;
+            x.t = paged_tile<ROWS, KEYS>(a, x.r, x.tile);
+            if (lane == 0) sm.pos[i] = x;
         }
     }
     __syncthreads();
@@ -196,7 +253,8 @@ __device__ __forceinline__ void paged_next(const PagedAttnArgs& a, const PagedPi
 }
 
 // ---- scratch slots ------------------------------------------------------------------------------
-// One slot: ROWS * D sums, ROWS running maxima, ROWS sums of weights.
+// One slot: ROWS * D sums (row by row for warps as workers, column by column for CTAs, whose threads own a row
+// each), ROWS running maxima, ROWS sums of weights.
 template <int ROWS, int D>
 __host__ __device__ constexpr long paged_slot() {
     return (long)ROWS * (D + 2);
@@ -292,6 +350,38 @@ __global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, int workers
         paged_store<4>(a.out + paged_row_at(a, x.first, x.h, x.tile, row, ROWS, a.os, row_bytes(a.io, D)), a.io, c0, y,
                        lane < LANES);
     }
+}
+
+// The same for workers that are CTAs: CTA (worker, 128-row tile, 32 columns), a thread per row.
+template <int ROWS, int D>
+__global__ void __launch_bounds__(128) k_paged_join_cols(PagedAttnArgs a) {
+    pdl_wait();
+    const int w = blockIdx.x, row = blockIdx.y * 128 + threadIdx.x, c0 = blockIdx.z * 32;
+    const PagedJoin x = a.join[w];
+    if (x.last < 0 || blockIdx.y * 128 >= x.nrow) return;
+    const long S = paged_slot<ROWS, D>();
+    const float* part = a.part + 2L * w * S;
+    const int n = x.last - w + 1;
+    auto slot = [&](int i) { return part + (i == 0 ? S : 2L * i * S); };
+    float m = -INFINITY;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, slot(i)[ROWS * D + row]);
+    const float mm = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, y[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = 0.0f;
+    for (int i = 0; i < n; ++i) {
+        const float* ps = slot(i);
+        const float f = exp2f(ps[ROWS * D + row] - mm);
+        l = fmaf(ps[ROWS * (D + 1) + row], f, l);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = fmaf(ps[(c0 + j) * ROWS + row], f, y[j]);
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) y[j] = l != 0.0f ? y[j] * inv : 0.0f;
+    const bool live = row < x.nrow;
+    paged_store<32>(a.out + (live ? paged_row_at(a, x.first, x.h, x.tile, row, ROWS, a.os, row_bytes(a.io, D)) : 0), a.io,
+                    c0, y, live);
 }
 
 }  // namespace gtn
