@@ -39,8 +39,14 @@ struct ChunkCfg {
     static constexpr int SMEM = 1024 + (2 + KS + VS) * TILE + 8 * STAGE;
     static constexpr int POLY = D == 64 ? 3 : 4;  // every POLY-th pair of exponentials on the multiply-add pipe
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
-    // kind::f16, A = B = fp16, D = fp32; scores: both K-major, N = 128; output: B (V) MN-major, N = D
-    static constexpr uint32_t IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    // Keys per score product. 64: the next unit's scores of a half start as soon as the half's weights are
+    // used, so the softmax does not wait for them. But at N = 64 the operands (Q again for every half) come out
+    // of shared memory slower than the product runs, which costs where the products are the bound: at D = 128
+    // one product over both halves (30,000-key chunk: 1144 us against 1284 us with halves; at D = 64 halves win,
+    // window chunks 164 us against 181 us).
+    static constexpr int SN = D == 64 ? 64 : 128;
+    // kind::f16, A = B = fp16, D = fp32; scores: both K-major, N = SN; output: B (V) MN-major, N = D
+    static constexpr uint32_t IDESC_S = (1u << 4) | (((uint32_t)SN >> 3) << 17) | ((128u >> 4) << 24);
     static constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
 };
 
@@ -171,7 +177,7 @@ __device__ __forceinline__ float2 f2_exp2(uint64_t x) {
 
 struct ChunkSmem {
     uint64_t k_full[3], k_empty[3], v_load[3], v_full[3], v_empty[3];
-    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drain;  // p_full: per tile, 64 keys each
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain;  // s, p: per tile and 64-key half
     uint32_t tmem;
     volatile int abort;
     volatile int odd;  // a non-finite value was set aside (stays set)
@@ -224,9 +230,11 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         }
         for (int r = 0; r < 2; ++r) {
             mbar_init(&sm.q_full[r], 128);
-            mbar_init(&sm.s_full[r], 1);
-            mbar_init(&sm.p_full[r][0], 128);
-            mbar_init(&sm.p_full[r][1], 128);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&sm.s_full[r][b], 1);
+                mbar_init(&sm.p_full[r][b], 128);
+            }
+            mbar_init(&sm.pv_done[r], 1);
             mbar_init(&sm.o_full[r], 1);
         }
         mbar_init(&sm.drain, 1);
@@ -246,17 +254,16 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
     int left = x.b < 0 ? 0 : (int)min(total - share * me, share);
     if (tid == 0) a.join[me].last = -1;
 
-    // units of row tile r in [u0, u1) that any of its rows sees to the causal limit: the first n_r
-    auto tile_units = [&](int r, int u0, int u1) {
+    // 64-key halves of units [u0, u1) that some row of row tile r sees to the causal limit: the first so many
+    auto tile_halves = [&](int r, int u0, int u1) {
         const int m1 = min(x.r.n * a.group, x.tile * CH_ROWS + (r + 1) * 128) - 1;  // the tile's last row
         if (m1 < x.tile * CH_ROWS + r * 128) return 0;
         const int phi = x.r.base + m1 / a.group;
-        int n = 0;
         if (phi < 0) return 0;
-        // keys ascend with u: sink units u < ns hold keys u * 128, the others (w0 + u - ns) * 128
-        n = min(x.t.ns, phi / CH_KEYS + 1);
-        if (n == x.t.ns) n += max(0, phi / CH_KEYS - x.t.w0 + 1);
-        return max(0, min(u1, n) - u0);
+        // keys ascend: sink halves q < 2 ns hold keys 64 q, the others 64 (2 w0 + q - 2 ns)
+        int n = min(2 * x.t.ns, phi / 64 + 1);
+        if (n == 2 * x.t.ns) n += max(0, phi / 64 - 2 * x.t.w0 + 1);
+        return max(0, min(2 * u1, n) - 2 * u0);
     };
     // by a whole warp; false once a wait of the CTA has run out
     auto wait = [&](uint64_t* bar, uint32_t ph) {
@@ -270,12 +277,12 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         }
         return true;
     };
-    // a unit that every row of the item (of the positions plo .. phi) sees whole
-    auto whole_for = [&](int kb, int plo, int phi) {
+    // keys [kb, kb + nk) that every row of the positions plo .. phi sees
+    auto whole_for = [&](int kb, int nk, int plo, int phi) {
         const int lo = a.window > 0 ? max(0, phi - a.window + 1) : 0;
-        return kb + CH_KEYS - 1 <= plo && (kb >= lo || kb + CH_KEYS <= a.n_sink);
+        return kb + nk - 1 <= plo && (kb >= lo || kb + nk <= a.n_sink);
     };
-    auto seen_whole = [&](int kb) { return whole_for(kb, x.t.plo, x.t.phi); };
+    auto seen_whole = [&](int kb) { return whole_for(kb, CH_KEYS, x.t.plo, x.t.phi); };
     auto next_item = [&](int done) {
         left -= done;
         if (left > 0) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
@@ -288,38 +295,41 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         const uint32_t ts = lanes + r * 128, to = lanes + C::COL_O + r * D;
         const uint32_t qs = sq + r * C::TILE;
         const long hb = row_bytes(a.io, D);
-        uint32_t s_ph = 0, o_ph = 0;
+        uint32_t s_ph = 0, o_ph = 0, pvn = 0;  // phases (s_full: a bit per half); halves handed to P V so far
         bool ok = true;
         // The row's query into the swizzled tile. Not for a tile without units: its softmax waits for nothing
         // and could pass q_full twice before the MMA warp looks.
         auto load_q = [&]() {
-            if (tile_units(r, x.u, min(x.t.units, x.u + left)) == 0) return;
+            if (tile_halves(r, x.u, min(x.t.units, x.u + left)) == 0) return;
             // D / 8 adjacent lanes per row
             constexpr int CPR = D / 8;
             const int c = lane % CPR;
-            uint4 v[CPR];
+#pragma unroll 1
+            for (int i = 0; i < CPR; i += 4) {
+                uint4 v[4];
 #pragma unroll
-            for (int i = 0; i < CPR; ++i) {
-                const int rw = r * 128 + (warp & 3) * 32 + i * (32 / CPR) + lane / CPR;
-                const bool in = x.tile * CH_ROWS + rw < x.r.n * a.group;
-                const uint8_t* qh = a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, rw, CH_ROWS, a.qs, hb) : 0);
-                v[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (in) v[i] = paged_q8x(qh, a.io, 8 * c);
-            }
+                for (int k = 0; k < 4; ++k) {
+                    const int rw = r * 128 + (warp & 3) * 32 + (i + k) * (32 / CPR) + lane / CPR;
+                    const bool in = x.tile * CH_ROWS + rw < x.r.n * a.group;
+                    const uint8_t* qh = a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, rw, CH_ROWS, a.qs, hb) : 0);
+                    v[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (in) v[k] = paged_q8x(qh, a.io, 8 * c);
+                }
 #pragma unroll
-            for (int i = 0; i < CPR; ++i) {
-                const int rw = (warp & 3) * 32 + i * (32 / CPR) + lane / CPR;
-                const uint32_t dst = qs + (c >> 3) * HALF + rw * 128 + (((c & 7) ^ (rw & 7)) << 4);
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z),
-                             "r"(v[i].w)
-                             : "memory");
+                for (int k = 0; k < 4; ++k) {
+                    const int rw = (warp & 3) * 32 + (i + k) * (32 / CPR) + lane / CPR;
+                    const uint32_t dst = qs + (c >> 3) * HALF + rw * 128 + (((c & 7) ^ (rw & 7)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[k].x), "r"(v[k].y),
+                                 "r"(v[k].z), "r"(v[k].w)
+                                 : "memory");
+                }
             }
             fence_async_smem();
             mbar_arrive(&sm.q_full[r]);
         };
         if (left > 0) load_q();
         while (left > 0 && ok) {
-            const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = tile_units(r, u0, u1);
+            const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = tile_halves(r, u0, u1);
             const int m_row = x.tile * CH_ROWS + r * 128 + row;
             const bool live = m_row < x.r.n * a.group;
             const int pos = live ? x.r.base + m_row / a.group : -1;
@@ -329,12 +339,17 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             const int tlo = x.r.base + t0 / a.group, thi = x.r.base + min(x.r.n - 1, (t0 + 127) / a.group);
             // the maximum in use (base 2; a row behind the item's last needs none), the sum of weights
             float mu = live ? -INFINITY : 0.0f, l = 0.0f;
-            for (int u = 0; u < n; ++u) {
-                if (!(ok = wait(&sm.s_full[r], s_ph))) break;
-                s_ph ^= 1u;
+            for (int q = 0; q < n; ++q) {
+                const int b = q & 1;
+                if (!(ok = wait(&sm.s_full[r][b], (s_ph >> b) & 1u))) break;
+                s_ph ^= 1u << b;
                 tc_fence_after();
-                const int kb = paged_unit_key<CH_KEYS>(x.t, u0 + u);
-                const bool whole = whole_for(kb, tlo, thi);
+                const int kb = paged_unit_key<CH_KEYS>(x.t, u0 + (q >> 1)) + 64 * b;
+                const uint32_t tb = ts + 64 * b;
+                uint32_t v[2][32];
+                ch_ld32(tb, v[0]);
+                ch_ld32(tb + 32, v[1]);
+                const bool whole = whole_for(kb, 64, tlo, thi);
                 // the keys of chunk i (32) that this row sees, as bits
                 auto seen_bits = [&](int i) -> uint32_t {
                     const int k0 = kb + 32 * i;
@@ -348,85 +363,69 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     for (int j = 0; j < 32; ++j)
                         if (!((bits >> j) & 1u)) v[j] = 0xff800000u;
                 };
-                auto grown = [&](float mx) {  // moves the maximum in use; the rows' sums so far follow
-                    float f = 1.0f;
-                    if (mx > mu + CH_GROW || (mu == -INFINITY && mx > mu)) {
-                        f = ex2(mu - mx);  // 0 when nothing was seen yet
-                        mu = mx;
-                        l *= f;
-                    }
-                    if (u == 0 || !__any_sync(0xffffffffu, f != 1.0f)) return;
-                    // P V of the unit before is done (its commit came before this unit's scores')
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        ch_ld32(to + 32 * c, o);
-                        ch_wait_ld(o);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        ch_st32(to + 32 * c, o);
-                    }
-                };
-                // first the maximum, then the weights, 64 keys at a time
+                ch_wait_ld(v[0]);
+                ch_wait_ld(v[1]);
+                if (!whole) {
+                    const uint32_t b0 = seen_bits(0), b1 = seen_bits(1);
+                    if (__any_sync(0xffffffffu, b0 != ~0u)) hide(v[0], b0);
+                    if (__any_sync(0xffffffffu, b1 != ~0u)) hide(v[1], b1);
+                }
                 float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll 1
-                for (int i = 0; i < 4; i += 2) {
-                    uint32_t v[2][32];
-                    ch_ld32(ts + 32 * i, v[0]);
-                    ch_ld32(ts + 32 * i + 32, v[1]);
-                    ch_wait_ld(v[0]);
-                    ch_wait_ld(v[1]);
-                    if (!whole) {
-                        const uint32_t b0 = seen_bits(i), b1 = seen_bits(i + 1);
-                        if (__any_sync(0xffffffffu, b0 != ~0u)) hide(v[0], b0);
-                        if (__any_sync(0xffffffffu, b1 != ~0u)) hide(v[1], b1);
-                    }
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        mx0 = max3_nan(mx0, __uint_as_float(v[0][j]), __uint_as_float(v[0][j + 1]));
-                        mx1 = max3_nan(mx1, __uint_as_float(v[1][j]), __uint_as_float(v[1][j + 1]));
-                    }
+                for (int j = 0; j < 32; j += 2) {
+                    mx0 = max3_nan(mx0, __uint_as_float(v[0][j]), __uint_as_float(v[0][j + 1]));
+                    mx1 = max3_nan(mx1, __uint_as_float(v[1][j]), __uint_as_float(v[1][j + 1]));
                 }
                 const float mx = max3_nan(mx0, mx1, mx1) * a.scale_log2;
                 if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);  // NaN or +infinity: the row has no softmax
-                grown(mx);
+                // the maximum in use moves when the new one lies too far above it; the sums so far follow
+                const bool grow = mx > mu + CH_GROW || (mu == -INFINITY && mx > mu);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? ex2(mu - mx) : 1.0f;  // 0 when nothing was seen yet
+                    if (grow) mu = mx;
+                    l *= f;
+                    if (q > 0) {
+                        // O as of the half before (P V of the one before that is done: these scores came behind it, so
+                        // the barrier is at most one phase back)
+                        if (!(ok = wait(&sm.pv_done[r], (pvn - 1) & 1u))) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[32];
+                            ch_ld32(to + 32 * c, o);
+                            ch_wait_ld(o);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            ch_st32(to + 32 * c, o);
+                        }
+                    }
+                }
                 const float sub = CH_BIAS - (mu == -INFINITY ? 0.0f : mu);
                 const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), sub2 = f2_pack(sub, sub);
                 uint64_t acc0 = 0, acc1 = 0;
-#pragma unroll 1
-                for (int i = 0; i < 4; i += 2) {
-                    uint32_t v[2][32], w[32];
-                    ch_ld32(ts + 32 * i, v[0]);
-                    ch_ld32(ts + 32 * i + 32, v[1]);
-                    ch_wait_ld(v[0]);
-                    ch_wait_ld(v[1]);
-                    if (!whole) {
-                        const uint32_t b0 = seen_bits(i), b1 = seen_bits(i + 1);
-                        if (__any_sync(0xffffffffu, b0 != ~0u)) hide(v[0], b0);
-                        if (__any_sync(0xffffffffu, b1 != ~0u)) hide(v[1], b1);
-                    }
+                uint32_t w[32];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const uint64_t t =
-                                f2_fma(f2_pack(__uint_as_float(v[h][2 * j]), __uint_as_float(v[h][2 * j + 1])), sc2, sub2);
-                            float2 e;
-                            if (j % C::POLY == C::POLY - 1) {
-                                e = f2_exp2(t);
-                            } else {
-                                e = f2_get(t);
-                                e = make_float2(ex2(e.x), ex2(e.y));
-                            }
-                            if (j & 1) acc1 = f2_add(acc1, f2_pack(e.x, e.y));
-                            else acc0 = f2_add(acc0, f2_pack(e.x, e.y));
-                            w[16 * h + j] = pack_f16(e.x, e.y);
+                    for (int j = 0; j < 16; ++j) {
+                        const uint64_t t =
+                            f2_fma(f2_pack(__uint_as_float(v[h][2 * j]), __uint_as_float(v[h][2 * j + 1])), sc2, sub2);
+                        float2 e;
+                        if (j % C::POLY == C::POLY - 1) {
+                            e = f2_exp2(t);
+                        } else {
+                            e = f2_get(t);
+                            e = make_float2(ex2(e.x), ex2(e.y));
                         }
-                    ch_st32(ts + 16 * i, w);  // over scores that are read
-                    ch_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&sm.p_full[r][i >> 1]);
-                }
+                        if (j & 1) acc1 = f2_add(acc1, f2_pack(e.x, e.y));
+                        else acc0 = f2_add(acc0, f2_pack(e.x, e.y));
+                        w[16 * h + j] = pack_f16(e.x, e.y);
+                    }
+                ch_st32(tb, w);  // over scores that are read
+                ch_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sm.p_full[r][b]);
+                ++pvn;
                 const float2 h = f2_get(f2_add(acc0, acc1));
                 l += h.x + h.y;
             }
@@ -448,6 +447,14 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 uint8_t* dst =
                     a.out + (live ? paged_row_at(a, was.r.first, was.h, was.tile, prow, CH_ROWS, a.os, hb) : 0);
                 const uint32_t stage = sq + (2 + C::KS + C::VS) * C::TILE + warp * C::STAGE;
+                uint8_t* orow[4];  // the rows whose 16 bytes this lane writes
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int rw = r * 128 + (warp & 3) * 32 + 8 * i + (lane >> 2);
+                    orow[i] = was.tile * CH_ROWS + rw < was.r.n * a.group
+                                  ? a.out + paged_row_at(a, was.r.first, was.h, was.tile, rw, CH_ROWS, a.os, hb) + 16 * (lane & 3)
+                                  : nullptr;
+                }
 #pragma unroll 1
                 for (int c = 0; c < D / 32; ++c) {
                     uint32_t o[32];
@@ -482,12 +489,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int lr = 8 * i + (lane >> 2), rw = r * 128 + (warp & 3) * 32 + lr;
+                        const int lr = 8 * i + (lane >> 2);
                         const uint4 y = lds16(stage + lr * 64 + (((lane & 3) ^ ((lr >> 1) & 3)) << 4));
-                        if (was.tile * CH_ROWS + rw < was.r.n * a.group)
-                            *reinterpret_cast<uint4*>(
-                                a.out + paged_row_at(a, was.r.first, was.h, was.tile, rw, CH_ROWS, a.os, hb) + 64 * c +
-                                16 * (lane & 3)) = y;
+                        if (orow[i]) *reinterpret_cast<uint4*>(orow[i] + 64 * c) = y;
                     }
                 }
                 if (!done && live) {
@@ -508,25 +512,30 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             int ks = 0, vs = 0;
             uint32_t k_ph = 0, v_ph = 0, q_ph = 0, p_ph = 0;
             bool ok = true;
-            auto qk = [&](int r) {
-                const uint64_t qd = ch_desc(q0 + r * C::TILE, 16), kd = ch_desc(k0 + ks * C::TILE, 16);
+            // scores of half b of the unit in stage ks, or (b = 0) of both halves; `two`: the second is wanted
+            auto qk = [&](int r, int b, bool two) {
+                const uint64_t qd = ch_desc(q0 + r * C::TILE, 16), kd = ch_desc(k0 + ks * C::TILE + b * 8192, 16);
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
                     const uint32_t off = ((i >> 2) * HALF + (i & 3) * 32) >> 4;
-                    ch_mma_ss(tm + r * 128, qd + off, kd + off, C::IDESC_S, i > 0, leader);
+                    ch_mma_ss(tm + r * 128 + b * 64, qd + off, kd + off, C::IDESC_S, i > 0, leader);
                 }
-                ch_commit(&sm.s_full[r], leader);
+                ch_commit(&sm.s_full[r][b], leader);
+                if (C::SN == 128 && two) ch_commit(&sm.s_full[r][1], leader);
             };
             while (left > 0 && ok) {
                 const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = u1 - u0;
-                const int nr0 = tile_units(0, u0, u1), nr1 = tile_units(1, u0, u1);
+                const int n0 = tile_halves(0, u0, u1), n1 = tile_halves(1, u0, u1);
                 ok = wait(&sm.k_full[ks], k_ph);
-                for (int r = 0; r < 2 && ok; ++r) {
-                    if ((r ? nr1 : nr0) == 0) continue;
-                    ok = wait(&sm.q_full[r], (q_ph >> r) & 1u);
-                    q_ph ^= 1u << r;
-                    tc_fence_after();
-                    if (ok) qk(r);
+                for (int i = 0; i < (C::SN == 64 ? 4 : 2) && ok; ++i) {
+                    const int b = i >> 1, r = i & 1, nr = r ? n1 : n0;
+                    if (b >= nr) continue;
+                    if (b == 0) {
+                        ok = wait(&sm.q_full[r], (q_ph >> r) & 1u);
+                        q_ph ^= 1u << r;
+                        tc_fence_after();
+                    }
+                    if (ok) qk(r, b, nr > 1);
                 }
                 for (int u = 0; u < n && ok; ++u) {
                     ch_commit(&sm.k_empty[ks], leader);  // the scores of unit u are issued
@@ -536,22 +545,20 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     }
                     if (u + 1 < n) ok = wait(&sm.k_full[ks], k_ph);
                     if (ok) ok = wait(&sm.v_full[vs], v_ph);
-                    for (int r = 0; r < 2 && ok; ++r) {
-                        const int nr = r ? nr1 : nr0;
-                        if (u >= nr) continue;
-                        const uint64_t vd = ch_desc(v0 + vs * C::TILE, HALF);
-                        for (int h = 0; h < 2 && ok; ++h) {
-                            if (!(ok = wait(&sm.p_full[r][h], (p_ph >> r) & 1u))) break;
-                            tc_fence_after();
+                    for (int i = 0; i < 4 && ok; ++i) {
+                        const int b = i >> 1, r = i & 1, nr = r ? n1 : n0, q = 2 * u + b;
+                        if (q >= nr) continue;
+                        if (!(ok = wait(&sm.p_full[r][b], (p_ph >> i) & 1u))) break;
+                        p_ph ^= 1u << i;
+                        tc_fence_after();
+                        const uint64_t vd = ch_desc(v0 + vs * C::TILE + b * 8192, HALF);
 #pragma unroll
-                            for (int i = 0; i < CH_KEYS / 32; ++i)
-                                ch_mma_ts(tm + C::COL_O + r * D, tm + r * 128 + (4 * h + i) * 8,
-                                          vd + ((4 * h + i) * 2048 >> 4), C::IDESC_O, u > 0 || h > 0 || i > 0, leader);
-                        }
-                        if (!ok) break;
-                        p_ph ^= 1u << r;
-                        if (u + 1 < nr) qk(r);
-                        else ch_commit(&sm.o_full[r], leader);
+                        for (int j = 0; j < 4; ++j)
+                            ch_mma_ts(tm + C::COL_O + r * D, tm + r * 128 + b * 64 + j * 8, vd + (j * 2048 >> 4), C::IDESC_O,
+                                      q > 0 || j > 0, leader);
+                        ch_commit(&sm.pv_done[r], leader);
+                        if (C::SN == 64 ? q + 2 < nr : b == 1 && q + 1 < nr) qk(r, C::SN == 64 ? b : 0, q + 2 < nr);
+                        if (q + 1 == nr) ch_commit(&sm.o_full[r], leader);
                     }
                     if (!ok) break;
                     ch_commit(&sm.v_empty[vs], leader);
