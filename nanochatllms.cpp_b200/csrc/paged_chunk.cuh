@@ -670,18 +670,21 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 next_item(u1 - u0);
             }
         } else {
-            // ---- Q8 pages to fp16 tiles: a warp takes groups of RPG rows (of one page), lane = 16 elements; the
-            // next tile's bytes are on their way while one is converted
+            // ---- Q8 pages to fp16 tiles: a warp takes groups of RPG rows (of one page), lane = 16 elements, in
+            // batches of three; the next batch's bytes are on their way while one is converted
             int ks = 0, vs = 0;
             uint32_t k_ph = 1, v_ph = 1;
             bool ok = true;
-            constexpr int CPR = D / 16, RPG = 32 / CPR, GROUPS = 128 / RPG, PER = (GROUPS + 2) / 3;
+            constexpr int CPR = D / 16, RPG = 32 / CPR, GROUPS = 128 / RPG, NB = (GROUPS + 8) / 9;  // batches per tile
             const int lrow = lane / CPR, c16 = lane % CPR, w3 = warp - 9;
-            uint4 kraw[PER], vraw[PER];
-            uint16_t kdl[PER], vdl[PER];
+            struct Batch {
+                uint4 raw[3];
+                uint16_t dl[3];
+            };
             int page = 0;  // lane i < 8: the page of the unit's 16-key piece i, -1 for none
-            auto find_pages = [&](int kb) {
-                const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0, k0 = kb + 16 * lane;
+            auto find_pages = [&]() {
+                const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
+                const int k0 = paged_unit_key<CH_KEYS>(x.t, x.u) + 16 * lane;
                 page = -1;
                 if (lane < 8 && k0 <= x.t.phi && (k0 + 15 >= lo || k0 < a.n_sink)) {
                     page = a.table[x.b * a.table_stride + (k0 >> a.c.ps_shift)];
@@ -691,37 +694,38 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     }
                 }
             };
-            auto load = [&](const uint8_t* pool, int kb, uint4 (&raw)[PER], uint16_t (&dl)[PER]) {
+            auto load = [&](const uint8_t* pool, int batch, Batch& t) {
+                const int kb = paged_unit_key<CH_KEYS>(x.t, x.u);
                 const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
                 const bool all = kb + CH_KEYS - 1 <= x.t.phi && (kb >= lo || kb + CH_KEYS <= a.n_sink);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int grp = w3 + 3 * i, k0 = kb + grp * RPG, key = k0 + lrow;
-                    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                    dl[i] = 0;
-                    if (GROUPS % 3 != 0 && grp >= GROUPS) continue;
-                    const int pgi = __shfl_sync(0xffffffffu, page, grp * RPG / 16);
-                    if (pgi >= 0 && (all || (key <= x.t.phi && (key >= lo || key < a.n_sink)))) {
+                for (int i = 0; i < 3; ++i) {
+                    const int grp = w3 + 3 * (3 * batch + i), key = kb + grp * RPG + lrow;
+                    t.raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                    t.dl[i] = 0;
+                    const int pgi = __shfl_sync(0xffffffffu, page, (grp * RPG / 16) & 7);
+                    if (grp < GROUPS && pgi >= 0 && (all || (key <= x.t.phi && (key >= lo || key < a.n_sink)))) {
                         const uint8_t* pg = pool + (long)pgi * a.c.page_stride;
                         const int cell = x.h * a.c.ps + (key & (a.c.ps - 1));  // row among the page's
-                        raw[i] = *reinterpret_cast<const uint4*>(pg + cell * D + c16 * 16);
-                        dl[i] = *reinterpret_cast<const uint16_t*>(pg + a.c.kv_heads * a.c.ps * D + (cell * (D / 32) + (c16 >> 1)) * 2);
+                        t.raw[i] = *reinterpret_cast<const uint4*>(pg + cell * D + c16 * 16);
+                        t.dl[i] = *reinterpret_cast<const uint16_t*>(pg + a.c.kv_heads * a.c.ps * D +
+                                                                     (cell * (D / 32) + (c16 >> 1)) * 2);
                     }
                 }
             };
-            auto convert = [&](uint32_t tile, bool scan, const uint4 (&raw)[PER], const uint16_t (&dl)[PER]) {
+            auto convert = [&](uint32_t tile, int batch, bool scan, const Batch& t) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int grp = w3 + 3 * i, row = grp * RPG + lrow;
-                    if (GROUPS % 3 != 0 && grp >= GROUPS) continue;
-                    const __half2 d2 = __half2half2(__ushort_as_half(dl[i]));
-                    const uint32_t in[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                for (int i = 0; i < 3; ++i) {
+                    const int grp = w3 + 3 * (3 * batch + i), row = grp * RPG + lrow;
+                    if (grp >= GROUPS) continue;
+                    const __half2 d2 = __half2half2(__ushort_as_half(t.dl[i]));
+                    const uint32_t in[4] = {t.raw[i].x, t.raw[i].y, t.raw[i].z, t.raw[i].w};
                     uint32_t w[8];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint2 b = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
-                        const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&b.x), d2);
-                        const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&b.y), d2);
+                        const uint2 y = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
+                        const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&y.x), d2);
+                        const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&y.y), d2);
                         w[2 * j] = *reinterpret_cast<const uint32_t*>(&h0);
                         w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
                     }
@@ -740,31 +744,34 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                                      "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
                                      : "memory");
                 }
-                fence_async_smem();
-                __syncwarp();
             };
+            Batch cur, nxt;
             if (left > 0) {
-                find_pages(paged_unit_key<CH_KEYS>(x.t, x.u));
-                load(a.c.k, paged_unit_key<CH_KEYS>(x.t, x.u), kraw, kdl);
+                find_pages();
+                load(a.c.k, 0, cur);
             }
             while (left > 0 && ok) {
-                const int kb = paged_unit_key<CH_KEYS>(x.t, x.u);
-                const bool scan = !seen_whole(kb);
-                load(a.c.v, kb, vraw, vdl);
-                if (!(ok = wait(&sm.k_empty[ks], k_ph))) break;
-                convert(sk + ks * C::TILE, false, kraw, kdl);
-                if (lane == 0) mbar_arrive(&sm.k_full[ks]);
-                // the next unit, of this item or the next
-                --left;
-                if (left > 0) {
-                    if (++x.u == x.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
-                    find_pages(paged_unit_key<CH_KEYS>(x.t, x.u));
+                const bool scan = !seen_whole(paged_unit_key<CH_KEYS>(x.t, x.u));
+#pragma unroll 1
+                for (int j = 0; j < 2 * NB && ok; ++j) {
+                    const int kv = j >= NB, jb = kv ? j - NB : j;
+                    if (j + 1 < 2 * NB) {
+                        load(j + 1 >= NB ? a.c.v : a.c.k, j + 1 >= NB ? j + 1 - NB : j + 1, nxt);
+                    } else if (--left > 0) {  // the next unit, of this item or the next
+                        if (++x.u == x.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
+                        find_pages();
+                        load(a.c.k, 0, nxt);
+                    }
+                    if (jb == 0) ok = kv ? wait(&sm.v_empty[vs], v_ph) : wait(&sm.k_empty[ks], k_ph);
+                    if (!ok) break;
+                    convert(kv ? sv + vs * C::TILE : sk + ks * C::TILE, jb, kv && scan, cur);
+                    if (jb == NB - 1) {
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(kv ? &sm.v_full[vs] : &sm.k_full[ks]);
+                    }
+                    cur = nxt;
                 }
-                if (!(ok = wait(&sm.v_empty[vs], v_ph))) break;
-                // (the page numbers asked for above are here by now)
-                if (left > 0) load(a.c.k, paged_unit_key<CH_KEYS>(x.t, x.u), kraw, kdl);
-                convert(sv + vs * C::TILE, scan, vraw, vdl);
-                if (lane == 0) mbar_arrive(&sm.v_full[vs]);
                 if (++ks == C::KS) {
                     ks = 0;
                     k_ph ^= 1u;
