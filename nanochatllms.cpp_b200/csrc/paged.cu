@@ -197,10 +197,152 @@ struct RopeFreq {
 
 constexpr int APP_THREADS = 256;
 
-// One CTA per row, one warp per head; lane l holds elements l, l + 32, ... of its head, so that a 32-element
-// block is one element per lane (the activation quantizer's layout).
-template <int D>
+// The angle in 64 bits, reduced to [-pi, pi] before the fp32 sine (an fp32 angle is off by pos * 2^-24 radians).
+__device__ __forceinline__ float2 rope_cs(int pos, double freq) {
+    const double x = (double)pos * freq;
+    const double r = fma(-rint(x * 0.15915494309189535), 6.283185307179586, x);
+    float sn, cn;
+    sincosf((float)r, &sn, &cn);
+    return make_float2(cn, sn);
+}
+
+// Eight elements of a row in dtype DT, from a 16-byte aligned place (Q8: element e0 of the row's blocks).
+template <int DT>
+__device__ __forceinline__ void app_load8(const uint8_t* head, int e0, float (&x)[8], uint2* raw, uint16_t* dl) {
+    if (DT == GTN_F16) {
+        const uint4 v = *reinterpret_cast<const uint4*>(head + 2 * e0);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = h2f((uint16_t)w[i]);
+            x[2 * i + 1] = h2f((uint16_t)(w[i] >> 16));
+        }
+    } else if (DT == GTN_F32) {
+        const float4 a = *reinterpret_cast<const float4*>(head + 4 * e0), b = *reinterpret_cast<const float4*>(head + 4 * e0 + 16);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint8_t* blk = head + e0 / GTN_QBLK * GTN_Q8_BYTES;
+        *dl = ld_u16(blk);
+        const uint8_t* p = blk + 2 + e0 % GTN_QBLK;  // even addresses
+        *raw = make_uint2(ld_u16(p) | ((uint32_t)ld_u16(p + 2) << 16), ld_u16(p + 4) | ((uint32_t)ld_u16(p + 6) << 16));
+        const float d = h2f(*dl);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = (float)(int8_t)(raw->x >> (8 * i)) * d;
+            x[4 + i] = (float)(int8_t)(raw->y >> (8 * i)) * d;
+        }
+    }
+}
+
+// One CTA per row; a thread takes two groups of eight elements of a head: those that rotate into each other (i
+// and i + half / 8, for i < half / 8), or two neighbours of the rest. D / 16 adjacent lanes hold a head, so the
+// absmax of a 32-element block is a few shuffles. Bound by its loads and stores: 16 bytes each (fp16).
+// For rows that are 16-byte aligned and a rotated width of whole groups; k_paged_append_any takes the others.
+template <int D, int SDT>
 static __global__ void __launch_bounds__(APP_THREADS) k_paged_append(AppendArgs a, const __grid_constant__ RopeFreq fr) {
+    constexpr int TPH = D / 16, NB = D / GTN_QBLK;  // threads and blocks of a head
+    __shared__ float2 cs[64];
+    pdl_wait();
+    pdl_trigger();
+    const int t = blockIdx.x, tid = threadIdx.x;
+    const int pos = a.pos[t], slot = a.slots[t];
+    if (pos < 0) return;
+    if (tid < a.half) cs[tid] = rope_cs(pos, fr.f[tid]);
+    const int kvh = a.c.kv_heads, page = slot >> a.c.ps_shift, r = slot & (a.c.ps - 1), hg = a.half >> 3;
+    const bool store = slot >= 0 && page < a.c.n_pages;
+    if (slot >= 0 && !store && tid == 0 && a.err) atomicOr(a.err, GTN_DEVERR_PAGE);
+    const long hb = row_bytes(SDT, D);
+    const int heads = a.heads + (store ? 2 * kvh : 0);
+    const int i = tid % TPH, g0 = i < hg ? i : 2 * hg + 2 * (i - hg), g1 = i < hg ? i + hg : g0 + 1;  // the groups
+    bool ready = false;
+    for (int hh = tid / TPH; hh - tid / TPH < heads; hh += APP_THREADS / TPH) {  // (the whole CTA takes every turn)
+        const bool live = hh < heads;
+        const int part = hh < a.heads ? 0 : hh < a.heads + kvh ? 1 : 2, h = hh - (part == 0 ? 0 : part == 1 ? a.heads : a.heads + kvh);
+        const uint8_t* src = (part == 0 ? a.q + (long)t * a.qs : part == 1 ? a.k + (long)t * a.ks : a.v + (long)t * a.vs) + h * hb;
+        float x[2][8];
+        uint2 raw[2] = {};
+        uint16_t dl[2] = {};
+        if (live) {
+            app_load8<SDT>(src, 8 * g0, x[0], &raw[0], &dl[0]);
+            app_load8<SDT>(src, 8 * g1, x[1], &raw[1], &dl[1]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[0][e] = x[1][e] = 0.0f;
+        }
+        if (!ready) __syncthreads();  // the angles, behind the first loads
+        ready = true;
+        if (part != 2 && i < hg) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 w = cs[8 * i + e];
+                const float p = x[0][e], q = x[1][e];
+                x[0][e] = fmaf(p, w.x, -(q * w.y));
+                x[1][e] = fmaf(p, w.y, q * w.x);
+            }
+        }
+        const int odt = part == 0 ? a.odt : a.c.dt;
+        uint8_t* pg = (part == 1 ? a.c.k : a.c.v) + (long)page * a.c.page_stride;
+        uint8_t* dst = part == 0 ? a.out + (long)t * a.os + h * row_bytes(a.odt, D) : pg + paged_row(a.c, h, r);
+        if (odt == GTN_F16) {
+            if (!live) continue;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = (uint32_t)f2h(x[k][2 * e]) | ((uint32_t)f2h(x[k][2 * e + 1]) << 16);
+                *reinterpret_cast<uint4*>(dst + 16 * (k ? g1 : g0)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            continue;
+        }
+        // the activation quantizer (warp_quant_block): absmax of each block over the head's lanes
+        float mx[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx[k] = fmaxf(mx[k], fabsf(x[k][e]));
+        float m0 = 0.0f, m1 = 0.0f;  // of this lane's two groups' blocks
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float m = fmaxf(g0 >> 2 == b ? mx[0] : 0.0f, g1 >> 2 == b ? mx[1] : 0.0f);
+#pragma unroll
+            for (int o = 1; o < TPH; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (g0 >> 2 == b) m0 = m;
+            if (g1 >> 2 == b) m1 = m;
+        }
+        if (!live) continue;
+        const bool pass = SDT == GTN_Q8 && part == 2;  // V blocks pass unchanged
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int g = k ? g1 : g0;
+            const float delta = (k ? m1 : m0) / 127.0f, inv = delta != 0.0f ? 1.0f / delta : 0.0f;
+            uint32_t w[2] = {0u, 0u};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(uint8_t)(int8_t)roundf(x[k][e] * inv) << (8 * (e & 3));
+            uint16_t dh = f2h(delta);
+            if (pass) {
+                w[0] = raw[k].x;
+                w[1] = raw[k].y;
+                dh = dl[k];
+            }
+            if (part == 0) {
+                uint8_t* blk = dst + (g >> 2) * GTN_Q8_BYTES;
+                uint16_t* y = reinterpret_cast<uint16_t*>(blk + 2 + 8 * (g & 3));
+                if ((g & 3) == 0) *reinterpret_cast<uint16_t*>(blk) = dh;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            } else {
+                *reinterpret_cast<uint2*>(dst + 8 * g) = make_uint2(w[0], w[1]);
+                if ((g & 3) == 0) reinterpret_cast<uint16_t*>(pg + paged_delta(a.c, h, r))[g >> 2] = dh;
+            }
+        }
+    }
+}
+
+// Any alignment of the rows and any rotated width. One CTA per row, one warp per head; lane l holds elements l,
+// l + 32, ... of its head, so that a 32-element block is one element per lane (the activation quantizer's layout).
+template <int D>
+static __global__ void __launch_bounds__(APP_THREADS) k_paged_append_any(AppendArgs a, const __grid_constant__ RopeFreq fr) {
     constexpr int NB = D / GTN_QBLK;
     __shared__ float2 cs[64];
     __shared__ float buf[APP_THREADS / 32][D];
@@ -208,15 +350,7 @@ static __global__ void __launch_bounds__(APP_THREADS) k_paged_append(AppendArgs 
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int pos = a.pos[t], slot = a.slots[t];
     if (pos < 0) return;
-    if (tid < a.half) {
-        // the angle in 64 bits, reduced to [-pi, pi] before the fp32 sine: an fp32 angle is off by
-        // pos * 2^-24 radians
-        const double x = (double)pos * fr.f[tid];
-        const double r = fma(-rint(x * 0.15915494309189535), 6.283185307179586, x);
-        float sn, cn;
-        sincosf((float)r, &sn, &cn);
-        cs[tid] = make_float2(cn, sn);
-    }
+    if (tid < a.half) cs[tid] = rope_cs(pos, fr.f[tid]);
     __syncthreads();
     const int kvh = a.c.kv_heads, page = slot >> a.c.ps_shift, r = slot & (a.c.ps - 1);
     const bool store = slot >= 0 && page < a.c.n_pages;
@@ -395,8 +529,16 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
     a.err = device_error_word();
     RopeFreq fr;
     for (int j = 0; j < 64; ++j) fr.f[j] = j < a.half ? std::pow((double)rope_base, -2.0 * j / (2 * a.half)) : 0.0;
-    const cudaError_t e = d == 64 ? launch_pdl(k_paged_append<64>, dim3(rows), dim3(APP_THREADS), 0, S(stream), a, fr)
-                                  : launch_pdl(k_paged_append<128>, dim3(rows), dim3(APP_THREADS), 0, S(stream), a, fr);
+    bool aligned = a.half % 8 == 0;
+    for (const gtn_tensor* t : rt)
+        aligned = aligned && (t->dtype == GTN_Q8 || ((uintptr_t)t->data % 16 == 0 && bstride(t, 0) % 16 == 0));
+#define GTN_APP(DV, SDT) launch_pdl(k_paged_append<DV, SDT>, dim3(rows), dim3(APP_THREADS), 0, S(stream), a, fr)
+#define GTN_APP_D(DV)                                                                              \
+    (!aligned ? launch_pdl(k_paged_append_any<DV>, dim3(rows), dim3(APP_THREADS), 0, S(stream), a, fr) \
+     : a.sdt == GTN_F16 ? GTN_APP(DV, GTN_F16) : a.sdt == GTN_F32 ? GTN_APP(DV, GTN_F32) : GTN_APP(DV, GTN_Q8))
+    const cudaError_t e = d == 64 ? GTN_APP_D(64) : GTN_APP_D(128);
+#undef GTN_APP_D
+#undef GTN_APP
     return cuda_status(e, who);
 }
 

@@ -120,23 +120,31 @@ def nbytes(dt: int, shape: Sequence[int]) -> int:
 
 
 def _ptr(buf) -> int:
-    if hasattr(buf, "data_ptr"):
+    try:
         return buf.data_ptr()
-    return int(buf)
+    except AttributeError:
+        return int(buf)
+
+
+_raw_stream = None  # torch's current stream of the current device as an integer, once torch has one
 
 
 def _stream(stream):
+    global _raw_stream
     if stream is not None:
-        if hasattr(stream, "cuda_stream"):
-            return C.c_void_p(stream.cuda_stream)
-        return C.c_void_p(int(stream))
-    try:
-        import torch
-        if torch.cuda.is_available():
-            return C.c_void_p(torch.cuda.current_stream().cuda_stream)
-    except Exception:
-        pass
-    return C.c_void_p(0)
+        return C.c_void_p(stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream))
+    if _raw_stream is None:
+        try:
+            import torch
+            if not torch.cuda.is_available():
+                return C.c_void_p(0)
+            torch.cuda.init()
+            get, dev = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+            get(dev())
+            _raw_stream = lambda: get(dev())  # noqa: E731
+        except Exception:
+            return C.c_void_p(0)
+    return C.c_void_p(_raw_stream())
 
 
 @dataclass
@@ -147,6 +155,10 @@ class GT:
     dtype: int
     shape: tuple
     strides: tuple | None = None
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_ref", None)  # a kept descriptor does not outlive a field
 
     def desc(self) -> gtn_tensor:
         t = gtn_tensor()
@@ -165,7 +177,15 @@ class GT:
 
 
 def _d(t):
-    return None if t is None else C.byref(t.desc())
+    """The descriptor by reference: kept with a GT, and made anew when the buffer's address has changed."""
+    if t is None:
+        return None
+    r = t._ref
+    if r is None or r[1] != _ptr(t.buf):
+        c = t.desc()
+        r = (C.byref(c), c.data)
+        object.__setattr__(t, "_ref", r)
+    return r[0]
 
 
 # ---- gten::ops (src/gten/ops.h) -------------------------------------------------------------
@@ -231,6 +251,7 @@ class PagedCache:
         self.k, self.v = k, v  # keeps the buffers alive
         self.d_head, self.kv_heads = d_head, kv_heads
         self._desc = gtn_paged_cache(_ptr(k), _ptr(v), dtype, n_pages, page_size, kv_heads, d_head, page_stride)
+        self._by_ref = C.byref(self._desc)
 
     @staticmethod
     def page_bytes(dtype: int, page_size: int, kv_heads: int, d_head: int) -> int:
@@ -254,7 +275,7 @@ def paged_plan(ctx_lens: GT, new_lens: GT, free_pages: GT, n_free: GT, page_size
 def paged_append(q: GT, k: GT, v: GT, pos: GT, slots: GT, cache: PagedCache, q_out: GT, rope_pct: float = 1.0,
                  rope_base: float = 10000.0, stream=None):
     """Rotary at each row's own position, K and V rows into their pages, rotated queries to q_out."""
-    _check(lib().gtn_paged_append(_d(q), _d(k), _d(v), _d(pos), _d(slots), _d(cache), _d(q_out), rope_pct, rope_base,
+    _check(lib().gtn_paged_append(_d(q), _d(k), _d(v), _d(pos), _d(slots), cache._by_ref, _d(q_out), rope_pct, rope_base,
                                   _stream(stream)), "paged_append")
 
 
@@ -268,16 +289,16 @@ def paged_attn(q: GT, cache: PagedCache, block_table: GT, q_start: GT, kv_lens: 
     """Attention of the new tokens over the pages (causal; window > 0: the last ``window`` keys and the
     first ``n_sink``). ``workspace``: a device buffer (uint8 tensor) of paged_attn_workspace bytes; without
     one, a tensor is taken from torch's allocator for this call, on the call's stream."""
-    d = cache.d_head
     if workspace is None:
         import torch
-        st = stream
-        if st is not None and not hasattr(st, "cuda_stream"):
-            st = torch.cuda.ExternalStream(int(st))
-        n = paged_attn_workspace(max(1, q.shape[-1] // d), d)
-        with torch.cuda.stream(st):
+        n = paged_attn_workspace(max(1, q.shape[-1] // cache.d_head), cache.d_head)
+        if stream is None:
             workspace = torch.empty(n, dtype=torch.uint8, device="cuda")
-    _check(lib().gtn_paged_attn(_d(q), _d(cache), _d(block_table), _d(q_start), _d(kv_lens), _d(out), scale, window,
+        else:
+            st = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream))
+            with torch.cuda.stream(st):
+                workspace = torch.empty(n, dtype=torch.uint8, device="cuda")
+    _check(lib().gtn_paged_attn(_d(q), cache._by_ref, _d(block_table), _d(q_start), _d(kv_lens), _d(out), scale, window,
                                 n_sink, max_new, _ptr(workspace), workspace.numel(), _stream(stream)), "paged_attn")
 
 
