@@ -240,38 +240,40 @@ __device__ __forceinline__ void app_load8(const uint8_t* head, int e0, float (&x
 // absmax of a 32-element block is a few shuffles. Bound by its loads and stores: 16 bytes each (fp16).
 // For rows that are 16-byte aligned and a rotated width of whole groups; k_paged_append_any takes the others.
 template <int D, int SDT>
-static __global__ void __launch_bounds__(APP_THREADS) k_paged_append(AppendArgs a, const __grid_constant__ RopeFreq fr) {
+static __global__ void __launch_bounds__(APP_THREADS, 5) k_paged_append(AppendArgs a, const __grid_constant__ RopeFreq fr) {
     constexpr int TPH = D / 16, NB = D / GTN_QBLK;  // threads and blocks of a head
     __shared__ float2 cs[64];
     pdl_wait();
     pdl_trigger();
     const int t = blockIdx.x, tid = threadIdx.x;
+    const int kvh = a.c.kv_heads, hg = a.half >> 3, heads = a.heads + 2 * kvh;
+    const long hb = row_bytes(SDT, D);
+    const int i = tid % TPH, g0 = i < hg ? i : 2 * hg + 2 * (i - hg), g1 = i < hg ? i + hg : g0 + 1;  // the groups
+    float x[2][8];
+    uint2 raw[2];
+    uint16_t dl[2];
+    auto load = [&](int hh) {
+        if (hh < heads) {
+            const uint8_t* src = hh < a.heads         ? a.q + (long)t * a.qs + hh * hb
+                                 : hh < a.heads + kvh ? a.k + (long)t * a.ks + (hh - a.heads) * hb
+                                                      : a.v + (long)t * a.vs + (hh - a.heads - kvh) * hb;
+            app_load8<SDT>(src, 8 * g0, x[0], &raw[0], &dl[0]);
+            app_load8<SDT>(src, 8 * g1, x[1], &raw[1], &dl[1]);
+        }
+    };
+    load(tid / TPH);  // on its way while the position and the angles are found
     const int pos = a.pos[t], slot = a.slots[t];
     if (pos < 0) return;
     if (tid < a.half) cs[tid] = rope_cs(pos, fr.f[tid]);
-    const int kvh = a.c.kv_heads, page = slot >> a.c.ps_shift, r = slot & (a.c.ps - 1), hg = a.half >> 3;
+    const int page = slot >> a.c.ps_shift, r = slot & (a.c.ps - 1);
     const bool store = slot >= 0 && page < a.c.n_pages;
     if (slot >= 0 && !store && tid == 0 && a.err) atomicOr(a.err, GTN_DEVERR_PAGE);
-    const long hb = row_bytes(SDT, D);
-    const int heads = a.heads + (store ? 2 * kvh : 0);
-    const int i = tid % TPH, g0 = i < hg ? i : 2 * hg + 2 * (i - hg), g1 = i < hg ? i + hg : g0 + 1;  // the groups
-    bool ready = false;
-    for (int hh = tid / TPH; hh - tid / TPH < heads; hh += APP_THREADS / TPH) {  // (the whole CTA takes every turn)
-        const bool live = hh < heads;
+    __syncthreads();
+    for (int turn = 0; turn < heads; turn += APP_THREADS / TPH) {  // (the whole CTA takes every turn)
+        const int hh = turn + tid / TPH;
+        if (turn > 0) load(hh);
         const int part = hh < a.heads ? 0 : hh < a.heads + kvh ? 1 : 2, h = hh - (part == 0 ? 0 : part == 1 ? a.heads : a.heads + kvh);
-        const uint8_t* src = (part == 0 ? a.q + (long)t * a.qs : part == 1 ? a.k + (long)t * a.ks : a.v + (long)t * a.vs) + h * hb;
-        float x[2][8];
-        uint2 raw[2] = {};
-        uint16_t dl[2] = {};
-        if (live) {
-            app_load8<SDT>(src, 8 * g0, x[0], &raw[0], &dl[0]);
-            app_load8<SDT>(src, 8 * g1, x[1], &raw[1], &dl[1]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[0][e] = x[1][e] = 0.0f;
-        }
-        if (!ready) __syncthreads();  // the angles, behind the first loads
-        ready = true;
+        const bool live = hh < heads && (part == 0 || store);
         if (part != 2 && i < hg) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
