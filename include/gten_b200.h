@@ -129,7 +129,7 @@ int gtn_token_embed(const gtn_tensor* weight, const gtn_tensor* tokens, gtn_tens
  * gtn_check (the rows that it concerns are unspecified). Numerics: fp32 (not the reference's order). */
 
 /* Descriptor of a paged cache. k and v are two pools of n_pages pages each, page_stride bytes apart
- * (0: page after page), 16-byte aligned, page_stride a multiple of 16. Inside a page:
+ * (0: page after page), 16-byte aligned, page_stride a multiple of 16 below 2^31. Inside a page:
  *   GTN_F16  fp16 [kv_heads][page_size][d_head];
  *   GTN_Q8   int8 [kv_heads][page_size][d_head], then the fp16 deltas [kv_heads][page_size][d_head / 32]
  *            (the values of Q8 blocks, values and deltas apart so that rows are 16-byte aligned).

@@ -15,7 +15,7 @@ int paged_cache_args(const gtn_paged_cache* c, const char* who, PagedCache* out)
                 c->d_head);
     GTN_REQUIRE(c->n_pages > 0 && (long)c->n_pages * c->page_size < (1L << 31), "%s: n_pages %d", who, c->n_pages);
     const long stride = c->page_stride ? c->page_stride : need;
-    GTN_REQUIRE(stride >= need && stride % 16 == 0 && stride < (1L << 40), "%s: page_stride %ld (pages of %ld bytes)",
+    GTN_REQUIRE(stride >= need && stride % 16 == 0 && stride < (1L << 31), "%s: page_stride %ld (pages of %ld bytes)",
                 who, (long)c->page_stride, need);
     GTN_REQUIRE((((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0, "%s: pools must be 16-byte aligned", who);
     out->k = (uint8_t*)c->k;

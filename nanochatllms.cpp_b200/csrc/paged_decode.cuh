@@ -56,6 +56,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // 16 bytes from global to shared memory, or 16 zero bytes (src is then not read).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const uint8_t* src, bool take) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -123,13 +126,15 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
 
     // ---- copies: the warp's position `y` on the line runs STAGES - 1 steps ahead of the computed one
     PagedPos y = x;
-    int ahead = left, slot_in = 0, page = 0;
+    int ahead = left, slot_in = 0, page = 0, ykb = 0, ylo = 0;  // ykb: first key of the step at y
+    const long vk = a.c.v - a.c.k;                              // from a byte of the K pool to V's
+    const int hrow = a.c.ps * RB;                               // bytes of a head in a page
     // lane i < NH: the page of the step's 16-key piece i; -1: no key of it is seen
     auto find_page = [&]() {
+        ykb = paged_unit_key<KEYS>(y.t, y.u);
         if (lane < NH) {
-            const int k0 = paged_unit_key<KEYS>(y.t, y.u) + 16 * lane;
-            const int lo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
-            const bool need = k0 <= y.t.phi && (k0 + 15 >= lo || k0 < a.n_sink);
+            const int k0 = ykb + 16 * lane;
+            const bool need = k0 <= y.t.phi && (k0 + 15 >= ylo || k0 < a.n_sink);
             page = need ? a.table[y.b * a.table_stride + (k0 >> a.c.ps_shift)] : -1;
             if (need && (unsigned)page >= (unsigned)a.c.n_pages) {
                 page = -1;
@@ -137,43 +142,66 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
             }
         }
     };
+    ylo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
     find_page();
+    // where this lane's 16 bytes of copy i go in a stage: rows lie 128 (64) bytes apart with their chunks exchanged
+    constexpr int CPR = RB / 16, RPI = 32 / CPR;  // chunks per row, rows per copy instruction
+    const int cr = lane / CPR, cc = lane % CPR;
+    const uint32_t d0 = RB == 256 ? (cc >> 3) * (KEYS * 128) + cr * 128 + (((cc & 7) ^ cr) << 4)
+                      : RB == 128 ? cr * 128 + ((cc ^ cr) << 4)
+                                  : cr * 64 + ((cc ^ ((cr >> 1) & 3)) << 4);
+    auto dst_of = [&](int i) {  // copy i: rows i * RPI + cr
+        if (RB == 256) return (d0 ^ ((uint32_t)(i & 3) << 5)) + i * 256;
+        if (RB == 128) return (d0 ^ ((uint32_t)(i & 1) << 6)) + i * 512;
+        return d0 + i * 512;
+    };
     auto fetch = [&]() {
         if (ahead > 0) {
-            const int kb = paged_unit_key<KEYS>(y.t, y.u);
-            const int lo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
             const uint32_t st = ring + slot_in * C::STAGE;
-            const bool whole = kb + KEYS - 1 <= y.t.phi && (kb >= lo || kb + KEYS <= a.n_sink);
-            constexpr int CPR = RB / 16, RPI = 32 / CPR;  // chunks per row, rows per copy instruction
-            const int r = lane / CPR, ch = lane % CPR;
+            // every key of the step is seen by some row and every page is there
+            const bool whole = ykb + KEYS - 1 <= y.t.phi && (ykb >= ylo || ykb + KEYS <= a.n_sink) &&
+                               !__any_sync(0xffffffffu, lane < NH && page < 0);
+            const uint8_t* head = a.c.k + (long)y.h * hrow + lane * 16;
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
                 const int pg = __shfl_sync(0xffffffffu, page, h);
-                const int row0 = (kb + 16 * h) & (a.c.ps - 1);
-                const long off = (long)(pg < 0 ? 0 : pg) * a.c.page_stride + paged_row(a.c, y.h, row0) + lane * 16;
+                const int row0 = (ykb + 16 * h) & (a.c.ps - 1);
+                const uint8_t* src = head + (unsigned long)(unsigned)max(pg, 0) * (unsigned)a.c.page_stride + row0 * RB;
+                const uint8_t* vsrc = src + vk;
+                if (whole) {
 #pragma unroll
-                for (int i = 0; i < 16 / RPI; ++i) {
-                    const int row = 16 * h + i * RPI + r, key = kb + row;
-                    const bool take = pg >= 0 && (whole || (key <= y.t.phi && (key >= lo || key < a.n_sink)));
-                    uint32_t dst;
-                    if (RB == 256) dst = (ch >> 3) * (KEYS * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
-                    else if (RB == 128) dst = row * 128 + ((ch ^ (row & 7)) << 4);
-                    else dst = row * 64 + ((ch ^ ((row >> 1) & 3)) << 4);
-                    cp_async16(st + dst, a.c.k + off + i * 512, take);
-                    cp_async16(st + KEYS * RB + dst, a.c.v + off + i * 512, take);
+                    for (int i = 0; i < 16 / RPI; ++i) {
+                        const uint32_t d = st + dst_of(h * (16 / RPI) + i);
+                        cp_async16(d, src + i * 512);
+                        cp_async16(d + KEYS * RB, vsrc + i * 512);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 16 / RPI; ++i) {
+                        const int key = ykb + 16 * h + i * RPI + cr;
+                        const bool take = pg >= 0 && key <= y.t.phi && (key >= ylo || key < a.n_sink);
+                        const uint32_t d = st + dst_of(h * (16 / RPI) + i);
+                        cp_async16(d, src + i * 512, take);
+                        cp_async16(d + KEYS * RB, vsrc + i * 512, take);
+                    }
                 }
             }
             if (Q) {  // the deltas: lanes 0-15 K's, 16-31 V's
                 constexpr int LPP = 2 * NC;  // lanes per 16-key piece (16 keys of NC fp16 deltas)
                 static_assert(!Q || LPP * NH == 16, "half a warp each");
                 const int h = (lane & 15) / LPP, pg = __shfl_sync(0xffffffffu, page, h);
-                const uint8_t* src = (lane < 16 ? a.c.k : a.c.v) + (long)(pg < 0 ? 0 : pg) * a.c.page_stride +
-                                     paged_delta(a.c, y.h, (kb + 16 * h) & (a.c.ps - 1)) + lane % LPP * 16;
+                const uint8_t* src = (lane < 16 ? a.c.k : a.c.v) +
+                                     (unsigned long)(unsigned)max(pg, 0) * (unsigned)a.c.page_stride +
+                                     (long)a.c.kv_heads * hrow +
+                                     (y.h * a.c.ps + ((ykb + 16 * h) & (a.c.ps - 1))) * (NC * 2) + lane % LPP * 16;
                 cp_async16(st + 2 * KEYS * RB + lane * 16, src, pg >= 0);
             }
             slot_in = slot_in + 1 == C::STAGES ? 0 : slot_in + 1;
             if (--ahead > 0) {
-                if (++y.u == y.t.units) paged_next<ROWS, KEYS>(a, p, y);
+                if (++y.u == y.t.units) {
+                    paged_next<ROWS, KEYS>(a, p, y);
+                    ylo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
+                }
                 find_page();
             }
         }
