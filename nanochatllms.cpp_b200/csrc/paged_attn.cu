@@ -28,7 +28,7 @@ static cudaError_t launch_decode(PagedAttnArgs a, const PagedPick& p, int most_r
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_paged_decode<DT, D, ROWS>, dim3(ctas), dim3(32 * PD_WARPS), C::SMEM, st, a, p);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_join<ROWS, D>, dim3((workers + 3) / 4, most_rows), dim3(128), 0, st, a, workers);
+    return launch_pdl(k_paged_join<ROWS, D>, dim3((workers + 3) / 4, std::min(most_rows, ROWS)), dim3(128), 0, st, a, workers);
 }
 
 template <int ROWS>
@@ -152,7 +152,10 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     cudaError_t e = cudaSuccess;
     if (most <= 16) {
         p.cut = 0x7fffffff;
-        e = most <= 8 ? decode<8>(a, p, (int)most, S(stream)) : decode<16>(a, p, (int)most, S(stream));
+        if (most == 1 && a.c.dt == GTN_Q8)
+            e = d == 64 ? launch_decode<GTN_Q8, 64, 1>(a, p, 1, S(stream)) : launch_decode<GTN_Q8, 128, 1>(a, p, 1, S(stream));
+        else
+            e = most <= 8 ? decode<8>(a, p, (int)most, S(stream)) : decode<16>(a, p, (int)most, S(stream));
     } else {
         PagedAttnArgs c = a;
         c.part = (float*)((uint8_t*)workspace + decode_ws_bytes(d));

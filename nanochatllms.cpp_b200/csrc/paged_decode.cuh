@@ -15,6 +15,13 @@
 // read of K and V meets all banks once.
 // Q8 caches keep their 8-bit values exact in fp16; the deltas are applied in fp32, to the scores per
 // 32-element block of K and to the weights per 32-column block of V before these round to fp16.
+//
+// One query row per kv head over a Q8 cache (no grouping, single tokens) is bound by instructions on that way: 7
+// of 8 rows of every fragment are empty. There (ROWS = 1) a lane owns whole keys: scores are 8-bit dot products
+// (dp4a) of the key with the query, itself split into two bytes per element (q = scale (256 hi + lo), 2^-16 of
+// the block's largest; Q8 queries are their own byte, exactly), softmax runs on one or two scores per lane, and
+// only P V goes through the matrix instructions, the weights turned into its fragment in shared memory.
+// (MiniCPM's batch of 64, Q8: 1,341 -> 900 instructions per 64 keys.)
 #pragma once
 #include "paged_sched.cuh"
 
@@ -38,6 +45,12 @@ struct DecodeCfg {
     static constexpr int SMEM = PD_WARPS * STAGES * STAGE;
     // perm(0) in the lowest digit
     static constexpr uint32_t PERM = !Q ? 0x73625140u : D == 64 ? 0x67235410u : 0x57136420u;
+    static constexpr uint32_t inverse() {
+        uint32_t v = 0;
+        for (int i = 0; i < 8; ++i) v |= (uint32_t)i << (4 * ((PERM >> (4 * i)) & 7));
+        return v;
+    }
+    static constexpr uint32_t INVERSE = inverse();
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -105,7 +118,8 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
     constexpr bool Q = C::Q;
     constexpr int KEYS = C::KEYS, RB = C::RB, NC = D / 32, NT = KEYS / 8, NH = KEYS / 16;
     constexpr int NO = D / 8;        // 8-column tiles of the output
-    constexpr bool R16 = ROWS == 16;
+    constexpr bool R16 = ROWS == 16, ONE = ROWS == 1;
+    static_assert(!ONE || Q, "single rows of fp16 caches run as eight");
     constexpr int NR = R16 ? 2 : 1;  // rows per lane: g, and g + 8
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ PagedSchedSmem<PD_WARPS> sm;
@@ -233,28 +247,65 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
     while (left > 0) {
         const int u0 = x.u, u1 = min(x.t.units, u0 + left);
         const int nrow = min(ROWS, x.r.n * a.group - x.tile * ROWS);  // query rows of this item
-        // query fragments: k step i covers elements 4 (i % 2) .. + 3 of every lane's eight of chunk i / 2
-        uint32_t qa[2 * NC][4];
+        uint32_t qa[ONE ? 1 : 2 * NC][4];                       // query fragments
+        uint32_t qhi[ONE ? D / 4 : 1], qlo[ONE ? D / 4 : 1];    // or the query's bytes
+        float qsc[ONE ? NC : 1];                                // and what they are worth, per 32 elements
+        bool has_lo = false;
         int pos[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int row = g + 8 * r;
-            const bool in = row < nrow;
-            pos[r] = in ? x.r.base + (x.tile * ROWS + row) / a.group : -1;
-            const uint8_t* qh = a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, row, ROWS, a.qs, hb) : 0);
+        if constexpr (ONE) {
+            pos[0] = x.r.base + x.tile / a.group;
+            const uint8_t* qh = a.q + paged_row_at(a, x.r.first, x.h, x.tile, 0, ROWS, a.qs, hb);
+            has_lo = a.io == GTN_F16;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (in) v = paged_q8x(qh, a.io, 32 * c + 8 * t);
-                qa[2 * c][r] = v.x;
-                qa[2 * c][2 + r] = v.y;
-                qa[2 * c + 1][r] = v.z;
-                qa[2 * c + 1][2 + r] = v.w;
-            }
-        }
-        if (!R16) {
+                uint32_t hi, lo = 0;
+                if (a.io == GTN_F16) {
+                    const float v = h2f(reinterpret_cast<const uint16_t*>(qh)[32 * c + lane]);
+                    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(v))));
+                    const int q16 = top > 0.0f ? __float2int_rn(v * (32512.0f / top)) : 0;
+                    hi = (uint32_t)((q16 + 128) >> 8);
+                    lo = (uint32_t)(q16 - (int)(hi << 8));
+                    qsc[c] = top * (1.0f / 32512.0f);  // (infinite or NaN with any element of the block)
+                } else {
+                    const uint8_t* blk = qh + c * GTN_Q8_BYTES;
+                    hi = blk[2 + lane];
+                    qsc[c] = h2f(ld_u16(blk));
+                }
+                // four lanes' bytes to a word, and the words to every lane
+                hi &= 0xffu;
+                lo &= 0xffu;
+                hi |= __shfl_down_sync(0xffffffffu, hi, 1) << 8;
+                lo |= __shfl_down_sync(0xffffffffu, lo, 1) << 8;
+                hi |= __shfl_down_sync(0xffffffffu, hi, 2) << 16;
+                lo |= __shfl_down_sync(0xffffffffu, lo, 2) << 16;
 #pragma unroll
-            for (int i = 0; i < 2 * NC; ++i) qa[i][1] = qa[i][3] = 0u;
+                for (int i = 0; i < 8; ++i) {
+                    qhi[8 * c + i] = __shfl_sync(0xffffffffu, hi, 4 * i);
+                    qlo[8 * c + i] = __shfl_sync(0xffffffffu, lo, 4 * i);
+                }
+            }
+        } else {
+            // query fragments: k step i covers elements 4 (i % 2) .. + 3 of every lane's eight of chunk i / 2
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                const int row = g + 8 * r;
+                const bool in = row < nrow;
+                pos[r] = in ? x.r.base + (x.tile * ROWS + row) / a.group : -1;
+                const uint8_t* qh = a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, row, ROWS, a.qs, hb) : 0);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (in) v = paged_q8x(qh, a.io, 32 * c + 8 * t);
+                    qa[2 * c][r] = v.x;
+                    qa[2 * c][2 + r] = v.y;
+                    qa[2 * c + 1][r] = v.z;
+                    qa[2 * c + 1][2 + r] = v.w;
+                }
+            }
+            if (!R16) {
+#pragma unroll
+                for (int i = 0; i < 2 * NC; ++i) qa[i][1] = qa[i][3] = 0u;
+            }
         }
         float o[NO][4], m[NR], l[NR];
 #pragma unroll
@@ -278,116 +329,190 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
             const int kb = paged_unit_key<KEYS>(x.t, u);
             const bool full = kb + KEYS - 1 <= full_hi && (kb >= full_lo || kb + KEYS <= a.n_sink);
 
-            // ---- scores
-            float sc[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[n][i] = 0.0f;
-                const uint32_t row = sk + n * 8 * (Q ? RB : 128);
-                if (!Q) {
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        const uint4 f = lds16(row + chunk(koff, c));
-                        mma_16816(sc[n], qa[2 * c], f.x, f.y);
-                        mma_16816(sc[n], qa[2 * c + 1], f.z, f.w);
-                    }
-                } else {
-                    // deltas of keys p0 and p1: NC halves each
-                    uint2 w0, w1;
-                    if (D == 64) {
-                        w0.x = lds4(sd + (8 * n + p0) * 4);
-                        w1.x = lds4(sd + (8 * n + p1) * 4);
-                    } else {
-                        w0 = lds8(sd + (8 * n + p0) * 8);
-                        w1 = lds8(sd + (8 * n + p1) * 8);
-                    }
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        float blk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        const uint2 f = lds8(row + chunk(koff, c));
-                        const uint2 lo = tc_bytes_to_f16x4(f.x ^ 0x80808080u, 0x64806480u);
-                        const uint2 hi = tc_bytes_to_f16x4(f.y ^ 0x80808080u, 0x64806480u);
-                        mma_16816(blk, qa[2 * c], lo.x, lo.y);
-                        mma_16816(blk, qa[2 * c + 1], hi.x, hi.y);
-                        const float d0 = h2f((uint16_t)((c < 2 ? w0.x : w0.y) >> (16 * (c & 1))));
-                        const float d1 = h2f((uint16_t)((c < 2 ? w1.x : w1.y) >> (16 * (c & 1))));
-#pragma unroll
-                        for (int r = 0; r < NR; ++r) {
-                            sc[n][2 * r] = fmaf(blk[2 * r], d0, sc[n][2 * r]);
-                            sc[n][2 * r + 1] = fmaf(blk[2 * r + 1], d1, sc[n][2 * r + 1]);
-                        }
-                    }
-                }
-            }
-            bool mixed = false;  // some row sees a key of this step that another does not
-            if (!full) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int key = kb + 8 * n + (e ? p1 : p0);
-#pragma unroll
-                        for (int r = 0; r < NR; ++r) {
-                            const bool see = key <= pos[r] && (a.window == 0 || key > pos[r] - a.window || key < a.n_sink);
-                            if (!see) sc[n][2 * r + e] = -INFINITY;
-                        }
-                    }
-                mixed = x.t.plo != x.t.phi;
-            }
-
-            // ---- softmax: running maximum and sum per row, in base 2
             uint32_t pa[NH][Q ? NC : 1][4];  // weight fragments of 16 keys (Q8: times the deltas of V's block c)
+            bool mixed = false;              // some row sees a key of this step that another does not
+            if constexpr (ONE) {
+                constexpr int KPL = KEYS / 32;  // keys per lane
+                float sc[KPL];
+                float mx = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                float mx = sc[0][2 * r];
+                for (int k = 0; k < KPL; ++k) {
+                    const int kr = lane + 32 * k, key = kb + kr;
+                    const uint2 dw = D == 64 ? make_uint2(lds4(sd + kr * 4), 0u) : lds8(sd + kr * 8);
+                    float v = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m[r], mx * a.scale_log2), ms = mn == -INFINITY ? 0.0f : mn;
-                if (__any_sync(0xffffffffu, mn > m[r])) {
-                    const float f = ex2(m[r] - ms);
-                    l[r] *= f;
+                    for (int c = 0; c < NC; ++c) {
+                        int hi = 0, lo = 0;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int ch = 2 * c + j;
+                            const uint4 f = lds16(sk + kr * RB + ((ch ^ (D == 64 ? (kr >> 1) & 3 : kr & 7)) << 4));
+                            const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                hi = dp4a((int)w[i], (int)qhi[4 * ch + i], hi);
+                                if (has_lo) lo = dp4a((int)w[i], (int)qlo[4 * ch + i], lo);
+                            }
+                        }
+                        const float d = h2f((uint16_t)((c < 2 ? dw.x : dw.y) >> (16 * (c & 1))));
+                        v = fmaf((float)(has_lo ? (hi << 8) + lo : hi) * qsc[c], d, v);
+                    }
+                    const bool see = full || (key <= pos[0] && (a.window == 0 || key > pos[0] - a.window || key < a.n_sink));
+                    sc[k] = see ? v * a.scale_log2 : -INFINITY;
+                    mx = fmaxf(mx, sc[k]);
+                }
+                // the maximum as an order-preserving integer
+                const uint32_t ub = __float_as_uint(mx);
+                const uint32_t mk = __reduce_max_sync(0xffffffffu, (ub & 0x80000000u) ? ~ub : (ub | 0x80000000u));
+                mx = __uint_as_float((mk & 0x80000000u) ? (mk ^ 0x80000000u) : ~mk);
+                const float mn = fmaxf(m[0], mx), ms = mn == -INFINITY ? 0.0f : mn;
+                if (mn > m[0]) {
+                    const float f = ex2(m[0] - ms);
+                    l[0] *= f;
 #pragma unroll
                     for (int j = 0; j < NO; ++j) {
-                        o[j][2 * r] *= f;
-                        o[j][2 * r + 1] *= f;
+                        o[j][0] *= f;
+                        o[j][1] *= f;
                     }
-                    m[r] = mn;
+                    m[0] = mn;
                 }
-                float sum = 0.0f;
+                __syncwarp();  // K is read: its place takes the weights, as the fragments want them
+#pragma unroll
+                for (int k = 0; k < KPL; ++k) {
+                    const int kr = lane + 32 * k;
+                    const float e = ex2(sc[k] + (PD_BIAS - ms));
+                    l[0] += e;
+                    const uint2 dw = D == 64 ? make_uint2(lds4(sd + C::DELTA + kr * 4), 0u) : lds8(sd + C::DELTA + kr * 8);
+                    const int te = (int)(C::INVERSE >> (4 * (kr & 7))) & 7;  // 2 t + e of this key among its 8
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        // a hidden key's delta may hold anything: its weight is zero whatever it is
+                        const float y = sc[k] == -INFINITY ? 0.0f : e * h2f((uint16_t)((c < 2 ? dw.x : dw.y) >> (16 * (c & 1))));
+                        const uint32_t at = sk + ((((c * 4 + (te >> 1)) * NH + (kr >> 4)) * 2 + ((kr >> 3) & 1)) * 2 + (te & 1)) * 2;
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(f2h(y)) : "memory");
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int i = 0; i < NH / 2; ++i) {
+                        const uint4 v = lds16(sk + (c * 4 + t) * NH * 8 + 16 * i);
+                        pa[2 * i][c][0] = g == 0 ? v.x : 0u;
+                        pa[2 * i][c][2] = g == 0 ? v.y : 0u;
+                        pa[2 * i + 1][c][0] = g == 0 ? v.z : 0u;
+                        pa[2 * i + 1][c][2] = g == 0 ? v.w : 0u;
+                    }
+            } else {
+                // ---- scores
+                float sc[NT][4];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float e0 = ex2(fmaf(sc[n][2 * r], a.scale_log2, PD_BIAS - ms));
-                    const float e1 = ex2(fmaf(sc[n][2 * r + 1], a.scale_log2, PD_BIAS - ms));
-                    sum += e0 + e1;
-                    const int s = n >> 1, at = r + 2 * (n & 1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[n][i] = 0.0f;
+                    const uint32_t row = sk + n * 8 * (Q ? RB : 128);
                     if (!Q) {
-                        pa[s][0][at] = pack_f16(e0, e1);
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) {
+                            const uint4 f = lds16(row + chunk(koff, c));
+                            mma_16816(sc[n], qa[2 * c], f.x, f.y);
+                            mma_16816(sc[n], qa[2 * c + 1], f.z, f.w);
+                        }
                     } else {
+                        // deltas of keys p0 and p1: NC halves each
                         uint2 w0, w1;
                         if (D == 64) {
-                            w0.x = lds4(sd + C::DELTA + (8 * n + p0) * 4);
-                            w1.x = lds4(sd + C::DELTA + (8 * n + p1) * 4);
+                            w0.x = lds4(sd + (8 * n + p0) * 4);
+                            w1.x = lds4(sd + (8 * n + p1) * 4);
                         } else {
-                            w0 = lds8(sd + C::DELTA + (8 * n + p0) * 8);
-                            w1 = lds8(sd + C::DELTA + (8 * n + p1) * 8);
+                            w0 = lds8(sd + (8 * n + p0) * 8);
+                            w1 = lds8(sd + (8 * n + p1) * 8);
                         }
 #pragma unroll
                         for (int c = 0; c < NC; ++c) {
-                            float y0 = e0 * h2f((uint16_t)((c < 2 ? w0.x : w0.y) >> (16 * (c & 1))));
-                            float y1 = e1 * h2f((uint16_t)((c < 2 ? w1.x : w1.y) >> (16 * (c & 1))));
-                            // a hidden key's delta may hold anything: its weight is zero whatever it is
-                            if (!full) {
-                                y0 = sc[n][2 * r] == -INFINITY ? 0.0f : y0;
-                                y1 = sc[n][2 * r + 1] == -INFINITY ? 0.0f : y1;
+                            float blk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            const uint2 f = lds8(row + chunk(koff, c));
+                            const uint2 lo = tc_bytes_to_f16x4(f.x ^ 0x80808080u, 0x64806480u);
+                            const uint2 hi = tc_bytes_to_f16x4(f.y ^ 0x80808080u, 0x64806480u);
+                            mma_16816(blk, qa[2 * c], lo.x, lo.y);
+                            mma_16816(blk, qa[2 * c + 1], hi.x, hi.y);
+                            const float d0 = h2f((uint16_t)((c < 2 ? w0.x : w0.y) >> (16 * (c & 1))));
+                            const float d1 = h2f((uint16_t)((c < 2 ? w1.x : w1.y) >> (16 * (c & 1))));
+#pragma unroll
+                            for (int r = 0; r < NR; ++r) {
+                                sc[n][2 * r] = fmaf(blk[2 * r], d0, sc[n][2 * r]);
+                                sc[n][2 * r + 1] = fmaf(blk[2 * r + 1], d1, sc[n][2 * r + 1]);
                             }
-                            pa[s][c][at] = pack_f16(y0, y1);
                         }
                     }
                 }
-                l[r] += sum;
+                if (!full) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int key = kb + 8 * n + (e ? p1 : p0);
+#pragma unroll
+                            for (int r = 0; r < NR; ++r) {
+                                const bool see = key <= pos[r] && (a.window == 0 || key > pos[r] - a.window || key < a.n_sink);
+                                if (!see) sc[n][2 * r + e] = -INFINITY;
+                            }
+                        }
+                    mixed = x.t.plo != x.t.phi;
+                }
+
+                // ---- softmax: running maximum and sum per row, in base 2
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float mx = sc[0][2 * r];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float mn = fmaxf(m[r], mx * a.scale_log2), ms = mn == -INFINITY ? 0.0f : mn;
+                    if (__any_sync(0xffffffffu, mn > m[r])) {
+                        const float f = ex2(m[r] - ms);
+                        l[r] *= f;
+#pragma unroll
+                        for (int j = 0; j < NO; ++j) {
+                            o[j][2 * r] *= f;
+                            o[j][2 * r + 1] *= f;
+                        }
+                        m[r] = mn;
+                    }
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float e0 = ex2(fmaf(sc[n][2 * r], a.scale_log2, PD_BIAS - ms));
+                        const float e1 = ex2(fmaf(sc[n][2 * r + 1], a.scale_log2, PD_BIAS - ms));
+                        sum += e0 + e1;
+                        const int s = n >> 1, at = r + 2 * (n & 1);
+                        if (!Q) {
+                            pa[s][0][at] = pack_f16(e0, e1);
+                        } else {
+                            uint2 w0, w1;
+                            if (D == 64) {
+                                w0.x = lds4(sd + C::DELTA + (8 * n + p0) * 4);
+                                w1.x = lds4(sd + C::DELTA + (8 * n + p1) * 4);
+                            } else {
+                                w0 = lds8(sd + C::DELTA + (8 * n + p0) * 8);
+                                w1 = lds8(sd + C::DELTA + (8 * n + p1) * 8);
+                            }
+#pragma unroll
+                            for (int c = 0; c < NC; ++c) {
+                                float y0 = e0 * h2f((uint16_t)((c < 2 ? w0.x : w0.y) >> (16 * (c & 1))));
+                                float y1 = e1 * h2f((uint16_t)((c < 2 ? w1.x : w1.y) >> (16 * (c & 1))));
+                                // a hidden key's delta may hold anything: its weight is zero whatever it is
+                                if (!full) {
+                                    y0 = sc[n][2 * r] == -INFINITY ? 0.0f : y0;
+                                    y1 = sc[n][2 * r + 1] == -INFINITY ? 0.0f : y1;
+                                }
+                                pa[s][c][at] = pack_f16(y0, y1);
+                            }
+                        }
+                    }
+                    l[r] += sum;
+                }
             }
             if (!R16) {
 #pragma unroll
@@ -475,8 +600,8 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             float ll = l[r];
-            ll += __shfl_xor_sync(0xffffffffu, ll, 1);
-            ll += __shfl_xor_sync(0xffffffffu, ll, 2);
+#pragma unroll
+            for (int i = 1; i < (ONE ? 32 : 4); i <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, i);
             const int row = g + 8 * r;
             const bool live = row < nrow, done = u0 == 0 && u1 == x.t.units;
             float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<ROWS, D>();

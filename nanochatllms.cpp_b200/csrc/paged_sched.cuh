@@ -257,7 +257,7 @@ __device__ __forceinline__ void paged_next(const PagedAttnArgs& a, const PagedPi
 // each), ROWS running maxima, ROWS sums of weights.
 template <int ROWS, int D>
 __host__ __device__ constexpr long paged_slot() {
-    return (long)ROWS * (D + 2);
+    return ((long)ROWS * (D + 2) + 3) / 4 * 4;  // (whole 16 bytes)
 }
 
 // Writes columns [c0, c0 + N) of one head's row in dtype io, 32 / N adjacent lanes per 32-element block;
