@@ -23,6 +23,7 @@ static cudaError_t launch_decode(PagedAttnArgs a, const PagedPick& p, int most_r
     using C = DecodeCfg<DT, D, ROWS>;
     static_assert(C::OCC <= DECODE_CTAS, "workspace");
     const int ctas = sm_count() * C::OCC, workers = ctas * PD_WARPS;
+    a.workers_mul = (unsigned)((1ull << 32) / (unsigned)workers + 1);
     a.join = reinterpret_cast<PagedJoin*>(a.part + (long)workers * 2 * paged_slot<ROWS, D>());
     cudaError_t e = ensure_smem(k_paged_decode<DT, D, ROWS>, C::SMEM);
     if (e != cudaSuccess) return e;
@@ -54,6 +55,7 @@ template <int DT, int D>
 static cudaError_t launch_chunk(PagedAttnArgs a, const PagedPick& p, cudaStream_t st) {
     using C = ChunkCfg<D>;
     const int ctas = sm_count();
+    a.workers_mul = (unsigned)((1ull << 32) / (unsigned)ctas + 1);
     a.join = reinterpret_cast<PagedJoin*>(a.part + (long)ctas * 2 * paged_slot<CH_ROWS, D>());
     cudaError_t e = ensure_smem(k_paged_chunk<DT, D>, C::SMEM);
     if (e != cudaSuccess) return e;
@@ -104,7 +106,13 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     GTN_REQUIRE(q->shape[1] % d == 0, "%s: q of %d columns, d_head %d", who, q->shape[1], d);
     const int heads = q->shape[1] / d;
     GTN_REQUIRE(heads % a.c.kv_heads == 0, "%s: heads %d not a multiple of kv heads %d", who, heads, a.c.kv_heads);
-    GTN_REQUIRE((long)q->shape[0] * heads < (1L << 31), "%s: %d rows of %d heads", who, q->shape[0], heads);
+    // what the kernels count in 32 bits: rows by the group (paged_group), units on the line
+    const long group = heads / a.c.kv_heads, rows = q->shape[0], cap = (long)block_table->shape[1] * a.c.ps;
+    GTN_REQUIRE(rows * group * group < (1L << 32) && rows * heads < (1L << 31), "%s: %ld rows of %d heads", who, rows, heads);
+    const long few = max_new > 0 && max_new * group <= 16 ? rows * group : 0;  // tiles of the decode kernel beyond one a request
+    GTN_REQUIRE(((few + n) * (cap / 16 + 2)) * a.c.kv_heads < (1L << 31) &&
+                    ((rows * group / CH_ROWS + n) * (cap / CH_KEYS + 2)) * a.c.kv_heads < (1L << 31),
+                "%s: %ld rows of %d requests over tables of %ld keys are too many for one call", who, rows, n, cap);
     const gtn_tensor* rt[] = {q, out};
     for (const gtn_tensor* t : rt) {
         GTN_REQUIRE(t->strides[1] == 1 && t->strides[0] >= t->shape[1], "%s: row strides", who);
@@ -135,8 +143,9 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     a.n_req = n;
     a.rows = q->shape[0];
     a.heads = heads;
-    a.group = heads / a.c.kv_heads;
-    a.cap = (long)block_table->shape[1] * a.c.ps;
+    a.group = (int)group;
+    a.group_mul = group > 1 ? (unsigned)(((1ull << 32) + group - 1) / group) : 0;
+    a.cap = cap;
     a.window = window;
     a.n_sink = n_sink;
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)d)) * 1.4426950408889634f;

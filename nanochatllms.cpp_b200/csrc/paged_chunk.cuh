@@ -181,7 +181,7 @@ struct ChunkSmem {
     uint32_t tmem;
     volatile int abort;
     volatile int odd;  // a non-finite value was set aside (stays set)
-    PagedSchedSmem<1> sched;
+    unsigned pre[CH_THREADS], wsum[CH_THREADS / 32];
 };
 
 // Adds the values that were set aside (non-finite) to a row's columns c0 .. c0 + 31, as far as it sees them.
@@ -244,21 +244,25 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
     }
     pdl_wait();
     pdl_trigger();
-    const int me = blockIdx.x, workers = gridDim.x;
+    const int me = blockIdx.x;
+    if (tid == 0) a.join[me].last = -1;
     tc_fence_before();
-    const long long total = paged_sched<CH_ROWS, CH_KEYS, CH_THREADS>(a, p, workers, me, me == 0, sm.sched);
+    paged_sched<CH_ROWS, CH_KEYS, CH_THREADS, true>(a, p, me == 0, sm.pre, sm.wsum);
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    const long long share = (total + workers - 1) / workers;
-    PagedPos x = sm.sched.pos[0];
-    int left = x.b < 0 ? 0 : (int)min(total - share * me, share);
-    if (tid == 0) a.join[me].last = -1;
+    const unsigned total = sm.pre[CH_THREADS - 1], share = paged_share(total, a.workers_mul);
+    PagedPos x{};
+    int left = 0;
+    if (share * (unsigned)me < total) {
+        x = paged_locate<CH_ROWS, CH_KEYS, CH_THREADS, true>(a, p, share * (unsigned)me, sm.pre);
+        left = (int)min(total - share * (unsigned)me, share);
+    }
 
     // 64-key halves of units [u0, u1) that some row of row tile r sees to the causal limit: the first so many
     auto tile_halves = [&](int r, int u0, int u1) {
         const int m1 = min(x.r.n * a.group, x.tile * CH_ROWS + (r + 1) * 128) - 1;  // the tile's last row
         if (m1 < x.tile * CH_ROWS + r * 128) return 0;
-        const int phi = x.r.base + m1 / a.group;
+        const int phi = x.r.base + paged_group(a, m1);
         if (phi < 0) return 0;
         // keys ascend: sink halves q < 2 ns hold keys 64 q, the others 64 (2 w0 + q - 2 ns)
         int n = min(2 * x.t.ns, phi / 64 + 1);
@@ -332,11 +336,11 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             const int u0 = x.u, u1 = min(x.t.units, u0 + left), n = tile_halves(r, u0, u1);
             const int m_row = x.tile * CH_ROWS + r * 128 + row;
             const bool live = m_row < x.r.n * a.group;
-            const int pos = live ? x.r.base + m_row / a.group : -1;
+            const int pos = live ? x.r.base + paged_group(a, m_row) : -1;
             const int wlo = a.window > 0 ? pos - a.window + 1 : 0;
             // positions of this tile's first and last row
             const int t0 = x.tile * CH_ROWS + r * 128;
-            const int tlo = x.r.base + t0 / a.group, thi = x.r.base + min(x.r.n - 1, (t0 + 127) / a.group);
+            const int tlo = x.r.base + paged_group(a, t0), thi = x.r.base + min(x.r.n - 1, paged_group(a, t0 + 127));
             // the maximum in use (base 2; a row behind the item's last needs none), the sum of weights
             float mu = live ? -INFINITY : 0.0f, l = 0.0f;
             for (int q = 0; q < n; ++q) {
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     ps[CH_ROWS * (D + 1) + prow] = l;
                 }
                 if (tid == 0 && u0 == 0 && u1 < was.t.units)
-                    a.join[me] = PagedJoin{(int)((was.start + was.t.units - 1) / share), was.r.first, was.h, was.tile,
+                    a.join[me] = PagedJoin{(int)((was.start + (unsigned)was.t.units - 1) / share), was.r.first, was.h, was.tile,
                                            min(CH_ROWS, was.r.n * a.group - was.tile * CH_ROWS)};
             }
         }

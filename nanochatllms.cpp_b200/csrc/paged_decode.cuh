@@ -64,11 +64,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const uint8_t* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -122,17 +117,16 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
     static_assert(!ONE || Q, "single rows of fp16 caches run as eight");
     constexpr int NR = R16 ? 2 : 1;  // rows per lane: g, and g + 8
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ PagedSchedSmem<PD_WARPS> sm;
+    __shared__ unsigned s_pre[32 * PD_WARPS], s_wsum[PD_WARPS];
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int workers = gridDim.x * PD_WARPS, me = blockIdx.x * PD_WARPS + warp;
-    const long long total =
-        paged_sched<ROWS, KEYS, 32 * PD_WARPS>(a, p, workers, blockIdx.x * PD_WARPS, blockIdx.x == 0, sm);
-    const long long share = (total + workers - 1) / workers;
-    PagedPos x = sm.pos[warp];
+    const unsigned me = blockIdx.x * PD_WARPS + warp;
     if (lane == 0) a.join[me].last = -1;
-    if (x.b < 0) return;
+    paged_sched<ROWS, KEYS, 32 * PD_WARPS, false>(a, p, blockIdx.x == 0, s_pre, s_wsum);
+    const unsigned total = s_pre[32 * PD_WARPS - 1], share = paged_share(total, a.workers_mul);
+    if (share * me >= total) return;
+    PagedPos x = paged_locate<ROWS, KEYS, 32 * PD_WARPS, false>(a, p, share * me, s_pre);
     int left = (int)min(total - share * me, share);
     const long hb = row_bytes(a.io, D);
     const uint32_t ring = smem_u32(smem) + warp * (C::STAGES * C::STAGE);
@@ -253,7 +247,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
         bool has_lo = false;
         int pos[NR];
         if constexpr (ONE) {
-            pos[0] = x.r.base + x.tile / a.group;
+            pos[0] = x.r.base + paged_group(a, x.tile);
             const uint8_t* qh = a.q + paged_row_at(a, x.r.first, x.h, x.tile, 0, ROWS, a.qs, hb);
             has_lo = a.io == GTN_F16;
 #pragma unroll
@@ -290,7 +284,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
             for (int r = 0; r < NR; ++r) {
                 const int row = g + 8 * r;
                 const bool in = row < nrow;
-                pos[r] = in ? x.r.base + (x.tile * ROWS + row) / a.group : -1;
+                pos[r] = in ? x.r.base + paged_group(a, x.tile * ROWS + row) : -1;
                 const uint8_t* qh = a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, row, ROWS, a.qs, hb) : 0);
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
@@ -604,7 +598,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
             for (int i = 1; i < (ONE ? 32 : 4); i <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, i);
             const int row = g + 8 * r;
             const bool live = row < nrow, done = u0 == 0 && u1 == x.t.units;
-            float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<ROWS, D>();
+            float* ps = a.part + (2L * (int)me + (u0 == 0)) * paged_slot<ROWS, D>();
             uint8_t* dst = a.out + (live ? paged_row_at(a, x.r.first, x.h, x.tile, row, ROWS, a.os, hb) : 0);
             const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
 #pragma unroll
@@ -629,7 +623,7 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
             }
         }
         if (u0 == 0 && u1 < x.t.units && lane == 0)
-            a.join[me] = PagedJoin{(int)((x.start + x.t.units - 1) / share), x.r.first, x.h, x.tile, nrow};
+            a.join[me] = PagedJoin{(int)((x.start + (unsigned)x.t.units - 1) / share), x.r.first, x.h, x.tile, nrow};
         left -= u1 - u0;
         if (left > 0) paged_next<ROWS, KEYS>(a, p, x);
     }

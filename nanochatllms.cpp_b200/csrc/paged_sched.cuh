@@ -14,6 +14,12 @@
 
 namespace gtn {
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // What a worker says of the item that begins in its range and goes on behind it.
 struct PagedJoin {
     int last;                   // the last worker of the item; -1: there is no such item
@@ -29,7 +35,9 @@ struct PagedAttnArgs {
     const int32_t *table, *q_start, *kv_lens;
     long table_stride;
     int n_req, rows, heads, group, window, n_sink;
+    unsigned group_mul;  // floor(x / group) = umulhi(x, group_mul) for x < 2^32 / group (0: group is 1)
     long cap;          // keys that a row of the table can hold
+    unsigned workers_mul;  // floor(2^32 / workers) + 1
     float scale_log2;  // scale * log2(e): the softmax runs in base 2
     float* part;       // scratch slots: [worker][2] of ROWS * (D + 2) floats
     PagedJoin* join;   // [worker]
@@ -61,18 +69,25 @@ struct PagedTile {
     int plo, phi;  // positions of the tile's first and last token
     int ns, w0, units;
 };
+// A kernel spends some 20 cycles per instruction that it runs for the first time (the instruction cache is cold
+// at its start), so what follows is short code rather than little work: 32-bit numbers (the host refuses calls of
+// 2^31 units or more), a multiplication for the division by the group, loops that are not unrolled.
+__device__ __forceinline__ int paged_group(const PagedAttnArgs& a, int m) {
+    return a.group_mul ? (int)__umulhi((unsigned)m, a.group_mul) : m;
+}
 template <int ROWS, int KEYS>
 __device__ __forceinline__ PagedTile paged_tile(const PagedAttnArgs& a, const PagedReq& r, int tile) {
     PagedTile t;
-    t.plo = r.base + tile * ROWS / a.group;
-    t.phi = r.base + min(r.n - 1, (tile * ROWS + ROWS - 1) / a.group);
+    t.plo = r.base + paged_group(a, tile * ROWS);
+    t.phi = r.base + min(r.n - 1, paged_group(a, tile * ROWS + ROWS - 1));
     t.ns = t.w0 = 0;
     t.units = 1;  // a tile that sees nothing still writes its zeros
     if (t.phi >= 0) {
-        const int lo = a.window > 0 ? max(0, t.plo - a.window + 1) : 0;
-        t.w0 = lo / KEYS;
-        t.ns = min((min(a.n_sink, t.phi + 1) + KEYS - 1) / KEYS, t.w0);
-        t.units = t.ns + t.phi / KEYS - t.w0 + 1;
+        if (a.window > 0) {
+            t.w0 = (unsigned)max(0, t.plo - a.window + 1) / KEYS;
+            t.ns = min((int)(((unsigned)min(a.n_sink, t.phi + 1) + KEYS - 1) / KEYS), t.w0);
+        }
+        t.units = t.ns + (int)((unsigned)t.phi / KEYS) - t.w0 + 1;
     }
     return t;
 }
@@ -89,35 +104,7 @@ struct PagedPick {
 template <int ROWS>
 __device__ __forceinline__ int paged_tiles(const PagedAttnArgs& a, const PagedPick& p, const PagedReq& r) {
     const int m = r.n * a.group;
-    return r.n > 0 && (m <= p.cut) == p.below ? (m + ROWS - 1) / ROWS : 0;
-}
-// The units of each lane's request (nt row tiles; one kv head), by a whole warp: a request of more than two
-// tiles is summed by all lanes.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ long long paged_req_units(const PagedAttnArgs& a, const PagedReq& r, int nt) {
-    const int lane = threadIdx.x & 31;
-    long long s = 0;
-    if (nt <= 2)
-        for (int t = 0; t < nt; ++t) s += paged_tile<ROWS, KEYS>(a, r, t).units;
-    for (unsigned big = __ballot_sync(0xffffffffu, nt > 2); big; big &= big - 1) {
-        const int src = __ffs(big) - 1, n = __shfl_sync(0xffffffffu, nt, src);
-        PagedReq q;
-        q.first = 0;
-        q.n = __shfl_sync(0xffffffffu, r.n, src);
-        q.base = __shfl_sync(0xffffffffu, r.base, src);
-        long long one = 0;
-        for (int t = lane; t < n; t += 32) one += paged_tile<ROWS, KEYS>(a, q, t).units;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
-        if (lane == src) s = one;
-    }
-    return s;
-}
-
-// a / b for a >= 0, b > 0; in 32 bits where they do.
-__device__ __forceinline__ long long paged_div(long long a, long long b) {
-    if (((a | b) >> 31) == 0) return (long long)((unsigned)a / (unsigned)b);
-    return a / b;
+    return r.n > 0 && (m <= p.cut) == p.below ? (int)((unsigned)(m + ROWS - 1) / ROWS) : 0;
 }
 
 // A position on the line of units: item (b, h, tile), unit u of it, the item's first position.
@@ -125,110 +112,118 @@ struct PagedPos {
     int b, h, tile, u;
     PagedReq r;
     PagedTile t;
-    long long start;
-};
-template <int W>
-struct PagedSchedSmem {
-    long long warp[33];
-    PagedPos pos[W];
+    unsigned start;
 };
 
-// Total units (returned), and in sm.pos[i] the item at position (first + i) * share of workers first ..
-// first + W - 1 of `workers` (its b is -1 at or past the end). Called by all THREADS threads of the CTA; ends
-// with a barrier.
-template <int ROWS, int KEYS, int THREADS, int W>
-__device__ __forceinline__ long long paged_sched(const PagedAttnArgs& a, const PagedPick& p, int workers, int first,
-                                                 bool flag, PagedSchedSmem<W>& sm) {
-    constexpr int NW = THREADS / 32;
+// Units of the tiles [0, nt) of a request (one kv head), by a whole warp.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ unsigned paged_warp_units(const PagedAttnArgs& a, const PagedReq& r, int nt) {
+    unsigned s = 0;
+#pragma unroll 1
+    for (int t = threadIdx.x & 31; t < nt; t += 32) s += paged_tile<ROWS, KEYS>(a, r, t).units;
+    return __reduce_add_sync(0xffffffffu, s);
+}
+
+// pre[i]: units of the requests of threads 0 .. i of THREADS, thread i holding `per` requests from i * per on.
+// By the whole CTA; ends with a barrier. BIG: requests of many tiles are common (each is summed by a warp).
+template <int ROWS, int KEYS, int THREADS, bool BIG>
+__device__ __forceinline__ void paged_sched(const PagedAttnArgs& a, const PagedPick& p, bool flag, unsigned* pre,
+                                            unsigned* wsum) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // thread tid holds requests [b0, b0 + per); every warp runs all `per` steps
-    const int per = (a.n_req + THREADS - 1) / THREADS, b0 = tid * per;
-    auto request = [&](int i, PagedReq& r, bool fl) {
-        r.first = r.n = r.base = 0;
-        if (b0 + i >= a.n_req) return 0;
-        r = paged_req(a, b0 + i, fl);
-        return paged_tiles<ROWS>(a, p, r);
-    };
-    long long mine = 0;
+    const int per = (a.n_req + THREADS - 1) / THREADS;
+    unsigned mine = 0;
+#pragma unroll 1
     for (int i = 0; i < per; ++i) {
+        const int b = tid * per + i;
         PagedReq r;
-        const int nt = request(i, r, flag);
-        mine += paged_req_units<ROWS, KEYS>(a, r, nt);
-    }
-    mine *= a.c.kv_heads;
-    long long s = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
-    }
-    if (lane == 31) sm.warp[warp] = s;
-    if (tid < W) sm.pos[tid].b = -1;
-    __syncthreads();
-    long long before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        before += w < warp ? sm.warp[w] : 0;
-        total += sm.warp[w];
-    }
-    before += s - mine;
-    const long long share = paged_div(total + workers - 1, workers);
-    for (int i = 0; i < W; ++i) {
-        const long long at = share * (first + i);
-        const unsigned own = __ballot_sync(0xffffffffu, at < total && at >= before && at < before + mine);
-        if (!own) continue;
-        // the warp of the thread whose requests hold the position finds the request, head and tile together
-        const int src = __ffs(own) - 1;
-        long long start = __shfl_sync(0xffffffffu, before, src), left = at - start;
-        bool found = false;
-        for (int j = 0; j < per && !found; ++j) {
-            PagedReq r;
-            const int nt = request(j, r, false);
-            const long long mine_one = paged_req_units<ROWS, KEYS>(a, r, nt);
-            const long long one = __shfl_sync(0xffffffffu, mine_one, src), all = one * a.c.kv_heads;
-            if (left >= all) {
-                left -= all;
-                start += all;
-                continue;
+        r.first = r.n = r.base = 0;
+        if (b < a.n_req) r = paged_req(a, b, flag);
+        const int nt = paged_tiles<ROWS>(a, p, r);
+        if (BIG) {
+            for (unsigned any = __ballot_sync(0xffffffffu, nt > 0); any; any &= any - 1) {
+                const int src = __ffs(any) - 1;
+                PagedReq q;
+                q.first = 0;
+                q.n = __shfl_sync(0xffffffffu, r.n, src);
+                q.base = __shfl_sync(0xffffffffu, r.base, src);
+                const unsigned one = paged_warp_units<ROWS, KEYS>(a, q, __shfl_sync(0xffffffffu, nt, src));
+                if (lane == src) mine += one;
             }
-            found = true;
-            PagedPos x;
-            x.b = __shfl_sync(0xffffffffu, b0 + j, src);
-            x.r.first = __shfl_sync(0xffffffffu, r.first, src);
-            x.r.n = __shfl_sync(0xffffffffu, r.n, src);
-            x.r.base = __shfl_sync(0xffffffffu, r.base, src);
-            const int tiles = __shfl_sync(0xffffffffu, nt, src);
-            x.h = (int)paged_div(left, one);
-            left -= x.h * one;
-            start += x.h * one;
-            for (int t0 = 0;; t0 += 32) {  // 32 tiles at a time: the first whose end lies behind the position
-                const int t = t0 + lane;
-                const long long mu = t < tiles ? paged_tile<ROWS, KEYS>(a, x.r, t).units : 0;
-                long long e = mu;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long y = __shfl_up_sync(0xffffffffu, e, o);
-                    if (lane >= o) e += y;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, e > left);
-                if (hit || t0 + 32 >= tiles) {
-                    const int l = hit ? __ffs(hit) - 1 : 31;
-                    const long long st = __shfl_sync(0xffffffffu, e - mu, l);
-                    x.tile = t0 + l;
-                    x.u = (int)(left - st);
-                    x.start = start + st;
-                    break;
-                }
-                const long long e31 = __shfl_sync(0xffffffffu, e, 31);
-                left -= e31;
-                start += e31;
-            }
-            x.t = paged_tile<ROWS, KEYS>(a, x.r, x.tile);
-            if (lane == 0) sm.pos[i] = x;
+        } else {
+#pragma unroll 1
+            for (int t = 0; t < nt; ++t) mine += paged_tile<ROWS, KEYS>(a, r, t).units;
         }
     }
+    mine *= a.c.kv_heads;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, mine, o);
+        if (lane >= o) mine += y;
+    }
+    if (lane == 31) wsum[warp] = mine;
     __syncthreads();
-    return total;
+    for (int w = 0; w < warp; ++w) mine += wsum[w];
+    pre[tid] = mine;
+    __syncthreads();
+}
+// Units per worker, a bit more than total / workers at most (the same for every worker).
+__device__ __forceinline__ unsigned paged_share(unsigned total, unsigned workers_mul) {
+    return total ? __umulhi(total - 1, workers_mul) + 1 : 1;
+}
+
+// The item at position `at` < total of the line, by a whole warp.
+template <int ROWS, int KEYS, int THREADS, bool BIG>
+__device__ __forceinline__ PagedPos paged_locate(const PagedAttnArgs& a, const PagedPick& p, unsigned at,
+                                                 const unsigned* pre) {
+    const int lane = threadIdx.x & 31, per = (a.n_req + THREADS - 1) / THREADS;
+    int before = 0;  // threads whose requests end at or before the position
+#pragma unroll 1
+    for (int j = lane; j < THREADS; j += 32) before += pre[j] <= at;
+    before = __reduce_add_sync(0xffffffffu, before);
+    PagedPos x;
+    x.b = before * per;
+    x.start = before ? pre[before - 1] : 0;
+    unsigned one;
+    int nt;
+#pragma unroll 1
+    for (;; ++x.b) {
+        x.r = paged_req(a, x.b, false);
+        nt = paged_tiles<ROWS>(a, p, x.r);
+        one = paged_warp_units<ROWS, KEYS>(a, x.r, nt);
+        if (at - x.start < one * a.c.kv_heads || x.b + 1 >= a.n_req) break;
+        x.start += one * a.c.kv_heads;
+    }
+    x.h = (int)((at - x.start) / one);
+    x.start += x.h * one;
+#pragma unroll 1
+    for (int t0 = 0;; t0 += 32) {  // 32 tiles at a time: the first whose end lies behind the position
+        const unsigned mu = t0 + lane < nt ? paged_tile<ROWS, KEYS>(a, x.r, t0 + lane).units : 0;
+        unsigned e = mu;
+        if (BIG) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(0xffffffffu, e, o);
+                if (lane >= o) e += y;
+            }
+        } else if (nt > 1) {
+#pragma unroll 1
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned y = __shfl_up_sync(0xffffffffu, e, o);
+                if (lane >= o) e += y;
+            }
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, e > at - x.start);
+        const int l = hit ? __ffs(hit) - 1 : 31;
+        if (hit || t0 + 32 >= nt) {
+            x.start += __shfl_sync(0xffffffffu, e - mu, l);
+            x.tile = t0 + l;
+            break;
+        }
+        x.start += __shfl_sync(0xffffffffu, e, 31);
+    }
+    x.u = (int)(at - x.start);
+    x.t = paged_tile<ROWS, KEYS>(a, x.r, x.tile);
+    return x;
 }
 
 // The next item on the line (b >= n_req behind the last one).
@@ -236,20 +231,18 @@ template <int ROWS, int KEYS>
 __device__ __forceinline__ void paged_next(const PagedAttnArgs& a, const PagedPick& p, PagedPos& x) {
     x.start += x.t.units;
     x.u = 0;
-    if (++x.tile < paged_tiles<ROWS>(a, p, x.r)) {
-        x.t = paged_tile<ROWS, KEYS>(a, x.r, x.tile);
-        return;
-    }
-    x.tile = 0;
-    if (++x.h == a.c.kv_heads) {
-        x.h = 0;
-        while (++x.b < a.n_req) {
-            x.r = paged_req(a, x.b, false);
-            if (paged_tiles<ROWS>(a, p, x.r) > 0) break;
+    if (++x.tile >= paged_tiles<ROWS>(a, p, x.r)) {
+        x.tile = 0;
+        if (++x.h == a.c.kv_heads) {
+            x.h = 0;
+            while (++x.b < a.n_req) {
+                x.r = paged_req(a, x.b, false);
+                if (paged_tiles<ROWS>(a, p, x.r) > 0) break;
+            }
+            if (x.b >= a.n_req) return;
         }
-        if (x.b >= a.n_req) return;
     }
-    x.t = paged_tile<ROWS, KEYS>(a, x.r, 0);
+    x.t = paged_tile<ROWS, KEYS>(a, x.r, x.tile);
 }
 
 // ---- scratch slots ------------------------------------------------------------------------------
@@ -303,7 +296,7 @@ __device__ __forceinline__ void paged_store(uint8_t* head, int io, int c0, const
 // Offset of an item's row in q or out: token, head.
 __device__ __forceinline__ long paged_row_at(const PagedAttnArgs& a, int first, int h, int tile, int row, int rows_per_tile,
                                              long stride, long head_bytes) {
-    const int m = tile * rows_per_tile + row, tok = m / a.group;
+    const int m = tile * rows_per_tile + row, tok = paged_group(a, m);
     return (long)(first + tok) * stride + (long)(h * a.group + m - tok * a.group) * head_bytes;
 }
 
@@ -331,7 +324,7 @@ __global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, int workers
 #pragma unroll 4
         for (int i = lane / LANES; i < n; i += WAYS) {
             const float* ps = slot(i);
-            const float f = exp2f(ps[ROWS * D + row] - mm);
+            const float f = ex2(ps[ROWS * D + row] - mm);
             const float4 v = *reinterpret_cast<const float4*>(ps + row * D + c0);
             l = fmaf(ps[ROWS * (D + 1) + row], f, l);
             y[0] = fmaf(v.x, f, y[0]);
@@ -371,7 +364,7 @@ __global__ void __launch_bounds__(128) k_paged_join_cols(PagedAttnArgs a) {
     for (int j = 0; j < 32; ++j) y[j] = 0.0f;
     for (int i = 0; i < n; ++i) {
         const float* ps = slot(i);
-        const float f = exp2f(ps[ROWS * D + row] - mm);
+        const float f = ex2(ps[ROWS * D + row] - mm);
         l = fmaf(ps[ROWS * (D + 1) + row], f, l);
 #pragma unroll
         for (int j = 0; j < 32; ++j) y[j] = fmaf(ps[(c0 + j) * ROWS + row], f, y[j]);
