@@ -320,23 +320,32 @@ __global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, int workers
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float mm = m == -INFINITY ? 0.0f : m;
         float l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int c0 = lane % LANES * 4;
-#pragma unroll 4
-        for (int i = lane / LANES; i < n; i += WAYS) {
-            const float* ps = slot(i);
-            const float f = ex2(ps[ROWS * D + row] - mm);
-            const float4 v = *reinterpret_cast<const float4*>(ps + row * D + c0);
-            l = fmaf(ps[ROWS * (D + 1) + row], f, l);
-            y[0] = fmaf(v.x, f, y[0]);
-            y[1] = fmaf(v.y, f, y[1]);
-            y[2] = fmaf(v.z, f, y[2]);
-            y[3] = fmaf(v.w, f, y[3]);
+        const int c0 = lane % LANES * 4, way = lane / LANES;
+        for (int i0 = 0; i0 < n; i0 += 32) {  // lane i: the weight of part i0 + i
+            float f = 0.0f;
+            if (i0 + lane < n) {
+                const float* ps = slot(i0 + lane) + ROWS * D + row;
+                f = ex2(ps[0] - mm);
+                l = fmaf(ps[ROWS], f, l);
+            }
+            const int k = min(32, n - i0);
+#pragma unroll 8
+            for (int i = 0; i < k; i += WAYS) {
+                const float w = __shfl_sync(0xffffffffu, f, (i + way) & 31);
+                if (WAYS == 1 || i + way < k) {
+                    const float4 v = *reinterpret_cast<const float4*>(slot(i0 + i + way) + row * D + c0);
+                    y[0] = fmaf(v.x, w, y[0]);
+                    y[1] = fmaf(v.y, w, y[1]);
+                    y[2] = fmaf(v.z, w, y[2]);
+                    y[3] = fmaf(v.w, w, y[3]);
+                }
+            }
         }
-        if (WAYS == 2) {
-            l += __shfl_xor_sync(0xffffffffu, l, 16);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (WAYS == 2)
 #pragma unroll
             for (int j = 0; j < 4; ++j) y[j] += __shfl_xor_sync(0xffffffffu, y[j], 16);
-        }
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = l != 0.0f ? y[j] * inv : 0.0f;
