@@ -18,8 +18,18 @@ static int64_t chunk_ws_bytes(int d) {
     return (int64_t)sm_count() * 2 * CH_ROWS * (d + 2) * (int64_t)sizeof(float) + join_bytes(sm_count());
 }
 
+// The three launches of a call. `chunk_ctas` of the join: 0 without a chunk kernel.
+template <int D, int ROWS>
+static cudaError_t launch_join(const PagedAttnArgs& dec, const PagedAttnArgs& chunk, int chunk_ctas, int workers, int rows,
+                               cudaStream_t st) {
+    const int n = chunk_ctas * (CH_ROWS / 128) * (D / 32);
+    return launch_pdl(k_paged_join<ROWS, CH_ROWS, D>, dim3(n + (workers + 3) / 4 * rows), dim3(128), 0, st, dec, chunk, n,
+                      workers, rows);
+}
+
 template <int DT, int D, int ROWS>
-static cudaError_t launch_decode(PagedAttnArgs a, const PagedPick& p, int most_rows, cudaStream_t st) {
+static cudaError_t launch_decode(PagedAttnArgs a, const PagedPick& p, int most_rows, const PagedAttnArgs& chunk,
+                                 int chunk_ctas, cudaStream_t st) {
     using C = DecodeCfg<DT, D, ROWS>;
     static_assert(C::OCC <= DECODE_CTAS, "workspace");
     const int ctas = sm_count() * C::OCC, workers = ctas * PD_WARPS;
@@ -29,14 +39,15 @@ static cudaError_t launch_decode(PagedAttnArgs a, const PagedPick& p, int most_r
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_paged_decode<DT, D, ROWS>, dim3(ctas), dim3(32 * PD_WARPS), C::SMEM, st, a, p);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_join<ROWS, D>, dim3((workers + 3) / 4, std::min(most_rows, ROWS)), dim3(128), 0, st, a, workers);
+    return launch_join<D, ROWS>(a, chunk, chunk_ctas, workers, std::min(most_rows, ROWS), st);
 }
 
 template <int ROWS>
-static cudaError_t decode(const PagedAttnArgs& a, const PagedPick& p, int most, cudaStream_t st) {
+static cudaError_t decode(const PagedAttnArgs& a, const PagedPick& p, int most, const PagedAttnArgs& chunk, int cc,
+                          cudaStream_t st) {
     if (a.c.d == 64)
-        return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 64, ROWS>(a, p, most, st) : launch_decode<GTN_Q8, 64, ROWS>(a, p, most, st);
-    return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 128, ROWS>(a, p, most, st) : launch_decode<GTN_Q8, 128, ROWS>(a, p, most, st);
+        return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 64, ROWS>(a, p, most, chunk, cc, st) : launch_decode<GTN_Q8, 64, ROWS>(a, p, most, chunk, cc, st);
+    return a.c.dt == GTN_F16 ? launch_decode<GTN_F16, 128, ROWS>(a, p, most, chunk, cc, st) : launch_decode<GTN_Q8, 128, ROWS>(a, p, most, chunk, cc, st);
 }
 
 // A pool of fp16 pages as [page][kv head and row][d] for boxes of `box` rows x 64 columns.
@@ -52,7 +63,7 @@ static bool page_map(const PagedCache& c, uint8_t* pool, int box, CUtensorMap* m
 }
 
 template <int DT, int D>
-static cudaError_t launch_chunk(PagedAttnArgs a, const PagedPick& p, cudaStream_t st) {
+static cudaError_t launch_chunk(PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
     using C = ChunkCfg<D>;
     const int ctas = sm_count();
     a.workers_mul = (unsigned)((1ull << 32) / (unsigned)ctas + 1);
@@ -62,12 +73,10 @@ static cudaError_t launch_chunk(PagedAttnArgs a, const PagedPick& p, cudaStream_
     CUtensorMap km{}, vm{};
     const int box = std::min(a.c.ps, CH_KEYS);
     if (DT == GTN_F16 && (!page_map(a.c, a.c.k, box, &km) || !page_map(a.c, a.c.v, box, &vm))) return cudaErrorInvalidValue;
-    e = launch_pdl(k_paged_chunk<DT, D>, dim3(ctas), dim3(CH_THREADS), C::SMEM, st, a, p, km, vm, box);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_join_cols<CH_ROWS, D>, dim3(ctas, CH_ROWS / 128, D / 32), dim3(128), 0, st, a);
+    return launch_pdl(k_paged_chunk<DT, D>, dim3(ctas), dim3(CH_THREADS), C::SMEM, st, a, p, km, vm, box);
 }
 
-static cudaError_t chunk(const PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
+static cudaError_t chunk(PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
     if (a.c.d == 64) return a.c.dt == GTN_F16 ? launch_chunk<GTN_F16, 64>(a, p, st) : launch_chunk<GTN_Q8, 64>(a, p, st);
     return a.c.dt == GTN_F16 ? launch_chunk<GTN_F16, 128>(a, p, st) : launch_chunk<GTN_Q8, 128>(a, p, st);
 }
@@ -156,15 +165,17 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     // is it for a single request, where the other's empty launch would cost more than its choice gives.
     PagedPick p;
     p.below = true;
+    p.chained = false;
     p.cut = a.group <= 8 ? 8 : a.group <= 16 ? 16 : 0;
     const long most = max_new > 0 ? (long)max_new * a.group : 0x7fffffffL;
     cudaError_t e = cudaSuccess;
     if (most <= 16) {
         p.cut = 0x7fffffff;
         if (most == 1 && a.c.dt == GTN_Q8)
-            e = d == 64 ? launch_decode<GTN_Q8, 64, 1>(a, p, 1, S(stream)) : launch_decode<GTN_Q8, 128, 1>(a, p, 1, S(stream));
+            e = d == 64 ? launch_decode<GTN_Q8, 64, 1>(a, p, 1, a, 0, S(stream))
+                        : launch_decode<GTN_Q8, 128, 1>(a, p, 1, a, 0, S(stream));
         else
-            e = most <= 8 ? decode<8>(a, p, (int)most, S(stream)) : decode<16>(a, p, (int)most, S(stream));
+            e = most <= 8 ? decode<8>(a, p, (int)most, a, 0, S(stream)) : decode<16>(a, p, (int)most, a, 0, S(stream));
     } else {
         PagedAttnArgs c = a;
         c.part = (float*)((uint8_t*)workspace + decode_ws_bytes(d));
@@ -172,7 +183,16 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
         PagedPick rest = p;
         rest.below = false;
         e = chunk(c, rest, S(stream));
-        if (e == cudaSuccess && p.cut > 0) e = p.cut == 8 ? decode<8>(a, p, 8, S(stream)) : decode<16>(a, p, 16, S(stream));
+        p.chained = true;
+        if (e == cudaSuccess) {
+            if (p.cut == 0)
+                e = d == 64 ? launch_join<64, 8>(a, c, sm_count(), 0, 1, S(stream))
+                            : launch_join<128, 8>(a, c, sm_count(), 0, 1, S(stream));
+            else if (p.cut == 8)
+                e = decode<8>(a, p, 8, c, sm_count(), S(stream));
+            else
+                e = decode<16>(a, p, 16, c, sm_count(), S(stream));
+        }
     }
     return cuda_status(e, who);
 }

@@ -100,6 +100,7 @@ __device__ __forceinline__ int paged_unit_key(const PagedTile& t, int u) {
 struct PagedPick {
     int cut;
     bool below;
+    bool chained;  // the decode kernel behind the chunk kernel of the same call (see there)
 };
 template <int ROWS>
 __device__ __forceinline__ int paged_tiles(const PagedAttnArgs& a, const PagedPick& p, const PagedReq& r) {
@@ -300,12 +301,11 @@ __device__ __forceinline__ long paged_row_at(const PagedAttnArgs& a, int first, 
     return (long)(first + tok) * stride + (long)(h * a.group + m - tok * a.group) * head_bytes;
 }
 
-// Joins the items that cross borders: warp (worker w, row y, y + gridDim.y, ...) the one that begins in w's range.
+// Joins the items that cross borders: the one that begins in worker w's range, rows row0, row0 + step, ..., by a
+// warp.
 template <int ROWS, int D>
-__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, int workers) {
-    pdl_wait();
-    const int lane = threadIdx.x & 31, w = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (w >= workers) return;
+__device__ __forceinline__ void paged_join_rows(const PagedAttnArgs& a, int w, int row0, int step) {
+    const int lane = threadIdx.x & 31;
     const PagedJoin x = a.join[w];
     if (x.last < 0) return;
     constexpr int LANES = D / 4, WAYS = D == 64 ? 2 : 1;  // four columns per lane; parts taken side by side
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, int workers
     const float* part = a.part + 2L * w * S;
     const int n = x.last - w + 1;  // part 0: slot 1 of worker w; part i: slot 0 of worker w + i
     auto slot = [&](int i) { return part + (i == 0 ? S : 2L * i * S); };
-    for (int row = blockIdx.y; row < x.nrow; row += gridDim.y) {
+    for (int row = row0; row < x.nrow; row += step) {
         float m = -INFINITY;
         for (int i = lane; i < n; i += 32) m = fmaxf(m, slot(i)[ROWS * D + row]);
 #pragma unroll
@@ -354,13 +354,12 @@ __global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a, int workers
     }
 }
 
-// The same for workers that are CTAs: CTA (worker, 128-row tile, 32 columns), a thread per row.
+// The same for workers that are CTAs: 128 rows of the item and columns c0 .. c0 + 31, by a CTA of a thread per row.
 template <int ROWS, int D>
-__global__ void __launch_bounds__(128) k_paged_join_cols(PagedAttnArgs a) {
-    pdl_wait();
-    const int w = blockIdx.x, row = blockIdx.y * 128 + threadIdx.x, c0 = blockIdx.z * 32;
+__device__ __forceinline__ void paged_join_cols(const PagedAttnArgs& a, int w, int half, int c0) {
+    const int row = half * 128 + threadIdx.x;
     const PagedJoin x = a.join[w];
-    if (x.last < 0 || blockIdx.y * 128 >= x.nrow) return;
+    if (x.last < 0 || half * 128 >= x.nrow) return;
     const long S = paged_slot<ROWS, D>();
     const float* part = a.part + 2L * w * S;
     const int n = x.last - w + 1;
@@ -384,6 +383,22 @@ __global__ void __launch_bounds__(128) k_paged_join_cols(PagedAttnArgs a) {
     const bool live = row < x.nrow;
     paged_store<32>(a.out + (live ? paged_row_at(a, x.first, x.h, x.tile, row, ROWS, a.os, row_bytes(a.io, D)) : 0), a.io,
                     c0, y, live);
+}
+
+// What both kernels of a call have left: the first `chunk_ctas` CTAs join the chunk kernel's items, the others the
+// decode kernel's, four workers (of `workers`) and one row (of row_step) each.
+template <int ROWS, int CROWS, int D>
+__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs dec, PagedAttnArgs chunk, int chunk_ctas, int workers,
+                                                    int row_step) {
+    pdl_wait();
+    constexpr int PER = CROWS / 128 * (D / 32);  // CTAs of a worker's item
+    const int i = blockIdx.x;
+    if (i < chunk_ctas) {
+        paged_join_cols<CROWS, D>(chunk, i / PER, i % (CROWS / 128), i % PER / (CROWS / 128) * 32);
+        return;
+    }
+    const int w = (i - chunk_ctas) / row_step * 4 + (threadIdx.x >> 5);
+    if (w < workers) paged_join_rows<ROWS, D>(dec, w, (i - chunk_ctas) % row_step, row_step);
 }
 
 }  // namespace gtn

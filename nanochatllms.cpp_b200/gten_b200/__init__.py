@@ -284,20 +284,29 @@ def paged_attn_workspace(heads: int, d_head: int) -> int:
     return int(lib().gtn_paged_attn_workspace(heads, d_head))
 
 
+_scratch_bytes: dict = {}
+
+
+def _scratch(heads: int, d_head: int, stream):
+    """paged_attn's workspace from torch's allocator, for one call on the stream."""
+    import torch
+    key = (heads, d_head, torch.cuda.current_device())
+    n = _scratch_bytes.get(key)
+    if n is None:
+        n = _scratch_bytes[key] = paged_attn_workspace(max(1, heads), d_head)
+    if stream is None:
+        return torch.empty(n, dtype=torch.uint8, device="cuda")
+    with torch.cuda.stream(stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream))):
+        return torch.empty(n, dtype=torch.uint8, device="cuda")
+
+
 def paged_attn(q: GT, cache: PagedCache, block_table: GT, q_start: GT, kv_lens: GT, out: GT, scale: float = 0.0,
                window: int = 0, n_sink: int = 0, max_new: int = 0, workspace=None, stream=None):
     """Attention of the new tokens over the pages (causal; window > 0: the last ``window`` keys and the
     first ``n_sink``). ``workspace``: a device buffer (uint8 tensor) of paged_attn_workspace bytes; without
     one, a tensor is taken from torch's allocator for this call, on the call's stream."""
     if workspace is None:
-        import torch
-        n = paged_attn_workspace(max(1, q.shape[-1] // cache.d_head), cache.d_head)
-        if stream is None:
-            workspace = torch.empty(n, dtype=torch.uint8, device="cuda")
-        else:
-            st = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(int(stream))
-            with torch.cuda.stream(st):
-                workspace = torch.empty(n, dtype=torch.uint8, device="cuda")
+        workspace = _scratch(q.shape[-1] // cache.d_head, cache.d_head, stream)
     _check(lib().gtn_paged_attn(_d(q), cache._by_ref, _d(block_table), _d(q_start), _d(kv_lens), _d(out), scale, window,
                                 n_sink, max_new, _ptr(workspace), workspace.numel(), _stream(stream)), "paged_attn")
 
