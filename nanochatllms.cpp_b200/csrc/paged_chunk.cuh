@@ -37,7 +37,6 @@ struct ChunkCfg {
     static constexpr int KS = D == 64 ? 3 : 2, VS = D == 64 ? 3 : 2;
     static constexpr int STAGE = 32 * 64;  // bytes per softmax warp: 32 rows x 32 fp16 outputs on their way out
     static constexpr int SMEM = 1024 + (2 + KS + VS) * TILE + 8 * STAGE;
-    static constexpr int POLY = D == 64 ? 3 : 4;  // every POLY-th pair of exponentials on the multiply-add pipe
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
     // Keys per score product. 64: the next unit's scores of a half start as soon as the half's weights are
     // used, so the softmax does not wait for them. But at N = 64 the operands (Q again for every half) come out
@@ -154,27 +153,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN i
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of a pair on the multiply-add pipe: x = n + f with n the nearest integer (by adding 1.5 * 2^23, which
-// leaves n in the low bits), 2^f by a polynomial of degree 4, 2^n by an integer add to the exponent. The
-// coefficients minimise the largest relative error on [-1/2, 1/2] (Remez exchange): 2.6e-6, a hundredth of
-// the rounding to fp16 that follows. x below -126 gives about 2^-126; NaN is not kept (the caller looks).
-__device__ __forceinline__ float2 f2_exp2(uint64_t x) {
-    float2 v = f2_get(x);
-    x = f2_pack(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
-    const uint64_t magic = f2_pack(12582912.0f, 12582912.0f), back = f2_pack(-12582912.0f, -12582912.0f);
-    const uint64_t t = f2_add(x, magic), n = f2_add(t, back), f = f2_fma(n, f2_pack(-1.0f, -1.0f), x);
-    uint64_t q = f2_fma(f2_pack(0.009570102207362652f, 0.009570102207362652f), f,
-                        f2_pack(0.05591785907745361f, 0.05591785907745361f));
-    q = f2_fma(q, f, f2_pack(0.240247443318367f, 0.240247443318367f));
-    q = f2_fma(q, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
-    q = f2_fma(q, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
-    v = f2_get(q);
-    const float2 e = f2_get(t);
-    v.x = __int_as_float(__float_as_int(v.x) + (__float_as_int(e.x) << 23));
-    v.y = __int_as_float(__float_as_int(v.y) + (__float_as_int(e.y) << 23));
-    return v;
-}
-
 struct ChunkSmem {
     uint64_t k_full[3], k_empty[3], v_load[3], v_full[3], v_empty[3];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain;  // s, p: per tile and 64-key half
@@ -202,9 +180,29 @@ static __device__ __noinline__ void ch_add_odd(const PagedAttnArgs& a, const Pag
     }
 }
 
+// Q8 queries and outputs, out of line: seldom code beside the loops costs instruction cache.
+static __device__ __noinline__ uint4 ch_q8_query(const PagedAttnArgs& a, const PagedPos& x, int row, int e0, int d) {
+    return paged_q8x(a.q + paged_row_at(a, x.r.first, x.h, x.tile, row, CH_ROWS, a.qs, row_bytes(GTN_Q8, d)), GTN_Q8, e0);
+}
+static __device__ __noinline__ void ch_q8_store(const PagedAttnArgs& a, const PagedPos& x, int row, int c0, int d,
+                                                const float (&v)[32]) {
+    uint8_t* blk = a.out + paged_row_at(a, x.r.first, x.h, x.tile, row, CH_ROWS, a.os, row_bytes(GTN_Q8, d)) +
+                   c0 / GTN_QBLK * GTN_Q8_BYTES;
+    float m = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) m = fmaxf(m, fabsf(v[i]));
+    const float delta = m / 127.0f, inv = delta != 0.0f ? 1.0f / delta : 0.0f;
+    *reinterpret_cast<uint16_t*>(blk) = f2h(delta);
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t lo = (uint8_t)(int8_t)roundf(v[2 * i] * inv), hi = (uint8_t)(int8_t)roundf(v[2 * i + 1] * inv);
+        reinterpret_cast<uint16_t*>(blk + 2)[i] = (uint16_t)(lo | (hi << 8));
+    }
+}
+
 template <int DT, int D>
 __global__ void __launch_bounds__(CH_THREADS, 1)
-    k_paged_chunk(PagedAttnArgs a, PagedPick p, const __grid_constant__ CUtensorMap kmap,
+    k_paged_chunk(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedPick p, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, int box) {
     using C = ChunkCfg<D>;
     constexpr bool Q8 = DT == GTN_Q8;
@@ -308,23 +306,36 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             // D / 8 adjacent lanes per row
             constexpr int CPR = D / 8;
             const int c = lane % CPR;
+            const int m0 = x.tile * CH_ROWS + r * 128 + (warp & 3) * 32 + lane / CPR, m1 = x.r.n * a.group;
+            const int l0 = (warp & 3) * 32 + lane / CPR;  // the lane's first row of the tile
+            if (a.io == GTN_F16) {
 #pragma unroll 1
-            for (int i = 0; i < CPR; i += 4) {
-                uint4 v[4];
+                for (int i = 0; i < 32; i += 4 * (32 / CPR)) {
+                    uint4 v[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int rw = r * 128 + (warp & 3) * 32 + (i + k) * (32 / CPR) + lane / CPR;
-                    const bool in = x.tile * CH_ROWS + rw < x.r.n * a.group;
-                    const uint8_t* qh = a.q + (in ? paged_row_at(a, x.r.first, x.h, x.tile, rw, CH_ROWS, a.qs, hb) : 0);
-                    v[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (in) v[k] = paged_q8x(qh, a.io, 8 * c);
+                    for (int k = 0; k < 4; ++k) {
+                        const int m = m0 + i + k * (32 / CPR), tok = paged_group(a, m);
+                        v[k] = make_uint4(0u, 0u, 0u, 0u);
+                        if (m < m1)
+                            v[k] = *reinterpret_cast<const uint4*>(a.q + (long)(x.r.first + tok) * a.qs +
+                                                                   (x.h * a.group + m - tok * a.group) * (D * 2) + 16 * c);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int rw = l0 + i + k * (32 / CPR);
+                        const uint32_t dst = qs + (c >> 3) * HALF + rw * 128 + (((c & 7) ^ (rw & 7)) << 4);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[k].x), "r"(v[k].y),
+                                     "r"(v[k].z), "r"(v[k].w)
+                                     : "memory");
+                    }
                 }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int rw = (warp & 3) * 32 + (i + k) * (32 / CPR) + lane / CPR;
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 32; i += 32 / CPR) {
+                    const int rw = l0 + i;
+                    const uint4 v = m0 + i < m1 ? ch_q8_query(a, x, r * 128 + rw, 8 * c, D) : make_uint4(0u, 0u, 0u, 0u);
                     const uint32_t dst = qs + (c >> 3) * HALF + rw * 128 + (((c & 7) ^ (rw & 7)) << 4);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[k].x), "r"(v[k].y),
-                                 "r"(v[k].z), "r"(v[k].w)
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                                  : "memory");
                 }
             }
@@ -414,13 +425,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     for (int j = 0; j < 16; ++j) {
                         const uint64_t t =
                             f2_fma(f2_pack(__uint_as_float(v[h][2 * j]), __uint_as_float(v[h][2 * j + 1])), sc2, sub2);
-                        float2 e;
-                        if (j % C::POLY == C::POLY - 1) {
-                            e = f2_exp2(t);
-                        } else {
-                            e = f2_get(t);
-                            e = make_float2(ex2(e.x), ex2(e.y));
-                        }
+                        float2 e = f2_get(t);
+                        e = make_float2(ex2(e.x), ex2(e.y));
                         if (j & 1) acc1 = f2_add(acc1, f2_pack(e.x, e.y));
                         else acc0 = f2_add(acc0, f2_pack(e.x, e.y));
                         w[16 * h + j] = pack_f16(e.x, e.y);
@@ -448,8 +454,6 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 const float inv = l != 0.0f ? 1.0f / l : 0.0f;
                 const int prow = r * 128 + row;
                 float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<CH_ROWS, D>();
-                uint8_t* dst =
-                    a.out + (live ? paged_row_at(a, was.r.first, was.h, was.tile, prow, CH_ROWS, a.os, hb) : 0);
                 const uint32_t stage = sq + (2 + C::KS + C::VS) * C::TILE + warp * C::STAGE;
                 uint8_t* orow[4];  // the rows whose 16 bytes this lane writes
 #pragma unroll
@@ -478,7 +482,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = l != 0.0f ? v[j] * inv : 0.0f;
                     if (a.io != GTN_F16) {
-                        paged_store<32>(dst, a.io, 32 * c, v, live);
+                        if (live) ch_q8_store(a, was, prow, 32 * c, D, v);
                         continue;
                     }
                     // through shared memory, so that four adjacent lanes write a row's 64 bytes
