@@ -418,9 +418,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 const float sub = CH_BIAS - (mu == -INFINITY ? 0.0f : mu);
                 const uint64_t sc2 = f2_pack(a.scale_log2, a.scale_log2), sub2 = f2_pack(sub, sub);
                 uint64_t acc0 = 0, acc1 = 0;
-                uint32_t w[32];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const uint64_t t =
@@ -429,9 +429,10 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                         e = make_float2(ex2(e.x), ex2(e.y));
                         if (j & 1) acc1 = f2_add(acc1, f2_pack(e.x, e.y));
                         else acc0 = f2_add(acc0, f2_pack(e.x, e.y));
-                        w[16 * h + j] = pack_f16(e.x, e.y);
+                        w[j] = pack_f16(e.x, e.y);
                     }
-                ch_st32(tb, w);  // over scores that are read
+                    ch_st16(tb + 16 * h, w);  // over scores that are read
+                }
                 ch_wait_st();
                 tc_fence_before();
                 mbar_arrive(&sm.p_full[r][b]);
