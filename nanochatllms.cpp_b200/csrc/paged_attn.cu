@@ -64,7 +64,7 @@ static bool page_map(const PagedCache& c, uint8_t* pool, int box, CUtensorMap* m
 
 template <int DT, int D>
 static cudaError_t launch_chunk(PagedAttnArgs& a, const PagedPick& p, cudaStream_t st) {
-    using C = ChunkCfg<D>;
+    using C = ChunkCfg<DT, D>;
     const int ctas = sm_count();
     a.workers_mul = (unsigned)((1ull << 32) / (unsigned)ctas + 1);
     a.join = reinterpret_cast<PagedJoin*>(a.part + (long)ctas * 2 * paged_slot<CH_ROWS, D>());

@@ -31,12 +31,18 @@ constexpr int CH_KEYS = 128;
 constexpr float CH_BIAS = 7.0f;
 constexpr float CH_GROW = 8.0f;
 
-template <int D>
+template <int DT, int D>
 struct ChunkCfg {
     static constexpr int TILE = 128 * D * 2;  // bytes of a Q, K or V tile
-    static constexpr int KS = D == 64 ? 3 : 2, VS = D == 64 ? 3 : 2;
+    // tiles of K and V in flight; for a Q8 cache also the pages' bytes of RS tiles each (at D = 128 one of K less
+    // makes room for them)
+    static constexpr bool Q8 = DT == GTN_Q8;
+    static constexpr int KS = D == 64 ? 3 : Q8 ? 1 : 2, VS = D == 64 ? 3 : 2;
+    static constexpr int RS = Q8 ? (D == 64 ? 2 : 1) : 0;
+    static constexpr int RAW = 128 * (D + D / 16);  // 128 rows of 8-bit values, then their deltas
     static constexpr int STAGE = 32 * 64;  // bytes per softmax warp: 32 rows x 32 fp16 outputs on their way out
-    static constexpr int SMEM = 1024 + (2 + KS + VS) * TILE + 8 * STAGE;
+    static constexpr int OUT = (2 + KS + VS) * TILE, RAW0 = OUT + 8 * STAGE;  // offsets
+    static constexpr int SMEM = 1024 + RAW0 + 2 * RS * RAW;
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
     // Keys per score product. 64: the next unit's scores of a half start as soon as the half's weights are
     // used, so the softmax does not wait for them. But at N = 64 the operands (Q again for every half) come out
@@ -153,8 +159,17 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN i
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// Untiled bulk copy (16-byte aligned, a multiple of 16 bytes), counted on `bar`.
+__device__ __forceinline__ void ch_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+        "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
 struct ChunkSmem {
     uint64_t k_full[3], k_empty[3], v_load[3], v_full[3], v_empty[3];
+    uint64_t raw_full[2][2], raw_empty[2][2];  // Q8: K and V, per raw tile
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain;  // s, p: per tile and 64-key half
     uint32_t tmem;
     volatile int abort;
@@ -204,7 +219,7 @@ template <int DT, int D>
 __global__ void __launch_bounds__(CH_THREADS, 1)
     k_paged_chunk(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedPick p, const __grid_constant__ CUtensorMap kmap,
                   const __grid_constant__ CUtensorMap vmap, int box) {
-    using C = ChunkCfg<D>;
+    using C = ChunkCfg<DT, D>;
     constexpr bool Q8 = DT == GTN_Q8;
     constexpr int HALVES = D / 64, HALF = 128 * 128;  // 64-column halves of a tile, bytes of one
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -234,6 +249,10 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             }
             mbar_init(&sm.pv_done[r], 1);
             mbar_init(&sm.o_full[r], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&sm.raw_full[i >> 1][i & 1], 1);
+            mbar_init(&sm.raw_empty[i >> 1][i & 1], 3);
         }
         mbar_init(&sm.drain, 1);
         sm.abort = 0;
@@ -455,7 +474,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 const float inv = l != 0.0f ? 1.0f / l : 0.0f;
                 const int prow = r * 128 + row;
                 float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<CH_ROWS, D>();
-                const uint32_t stage = sq + (2 + C::KS + C::VS) * C::TILE + warp * C::STAGE;
+                const uint32_t stage = sq + C::OUT + warp * C::STAGE;
                 uint8_t* orow[4];  // the rows whose 16 bytes this lane writes
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -679,107 +698,106 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 next_item(u1 - u0);
             }
         } else {
-            // ---- Q8 pages to fp16 tiles: a warp takes groups of RPG rows (of one page), lane = 16 elements, in
-            // batches of three; the next batch's bytes are on their way while one is converted
-            int ks = 0, vs = 0;
-            uint32_t k_ph = 1, v_ph = 1;
+            // ---- Q8 pages to fp16 tiles. Warp 9 brings the pages' bytes into shared memory, RS units ahead (bulk
+            // copies of 16 rows and of their deltas, a lane each); all three convert: a warp takes groups of RPG
+            // rows, lane = 16 elements of a row.
+            int ks = 0, vs = 0, rs = 0;
+            uint32_t k_ph = 1, v_ph = 1, r_ph = 0;
             bool ok = true;
-            constexpr int CPR = D / 16, RPG = 32 / CPR, GROUPS = 128 / RPG, NB = (GROUPS + 8) / 9;  // batches per tile
+            constexpr int CPR = D / 16, RPG = 32 / CPR, GROUPS = 128 / RPG, RSD = C::RS > 0 ? C::RS : 1;
             const int lrow = lane / CPR, c16 = lane % CPR, w3 = warp - 9;
-            struct Batch {
-                uint4 raw[3];
-                uint16_t dl[3];
-            };
-            int page = 0;  // lane i < 8: the page of the unit's 16-key piece i, -1 for none
-            auto find_pages = [&]() {
-                const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
-                const int k0 = paged_unit_key<CH_KEYS>(x.t, x.u) + 16 * lane;
+            PagedPos y = x;  // warp 9: the unit whose bytes are asked for next
+            int ahead = left, asked = 0, page = -1;
+            auto fetch = [&]() {  // K and V of the unit at y
+                const int slot = asked % RSD;
+                const int lo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
+                const int k0 = paged_unit_key<CH_KEYS>(y.t, y.u) + 16 * (lane & 7);
+                // lane i of 8: the 16-key piece i; lanes 0-7 copy the values, 8-15 the deltas
                 page = -1;
-                if (lane < 8 && k0 <= x.t.phi && (k0 + 15 >= lo || k0 < a.n_sink)) {
-                    page = a.table[x.b * a.table_stride + (k0 >> a.c.ps_shift)];
+                if (lane < 16 && k0 <= y.t.phi && (k0 + 15 >= lo || k0 < a.n_sink)) {
+                    page = a.table[y.b * a.table_stride + (k0 >> a.c.ps_shift)];
                     if ((unsigned)page >= (unsigned)a.c.n_pages) {
                         page = -1;
                         atomicOr(a.err, GTN_DEVERR_PAGE);
                     }
                 }
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0) & 0xffu) * 16 * (D + D / 16);
+                const int cell = y.h * a.c.ps + (k0 & (a.c.ps - 1));  // row among the page's
+                const bool dl = lane >= 8;
+                const long off = (long)max(page, 0) * a.c.page_stride +
+                                 (dl ? (long)a.c.kv_heads * a.c.ps * D + cell * (D / 16) : (long)cell * D);
+                const uint32_t dst = dl ? 128 * D + (lane & 7) * D : (lane & 7) * 16 * D;
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (asked >= C::RS && !(ok = wait(&sm.raw_empty[kv][slot], (uint32_t)(asked / RSD - 1) & 1u))) return;
+                    if (lane == 0) mbar_arrive_expect_tx(&sm.raw_full[kv][slot], bytes);
+                    __syncwarp();
+                    if (page >= 0)
+                        ch_bulk(sq + C::RAW0 + (kv * RSD + slot) * C::RAW + dst, (kv ? a.c.v : a.c.k) + off, dl ? D : 16 * D,
+                                &sm.raw_full[kv][slot]);
+                }
+                ++asked;
+                if (--ahead > 0 && ++y.u == y.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, y);
             };
-            auto load = [&](const uint8_t* pool, int batch, Batch& t) {
+            if (warp == 9)
+                for (int i = 0; i < C::RS && ahead > 0 && ok; ++i) fetch();
+            while (left > 0 && ok) {
                 const int kb = paged_unit_key<CH_KEYS>(x.t, x.u);
+                const bool scan = !seen_whole(kb);
                 const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
                 const bool all = kb + CH_KEYS - 1 <= x.t.phi && (kb >= lo || kb + CH_KEYS <= a.n_sink);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const int grp = w3 + 3 * (3 * batch + i), key = kb + grp * RPG + lrow;
-                    t.raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                    t.dl[i] = 0;
-                    const int pgi = __shfl_sync(0xffffffffu, page, (grp * RPG / 16) & 7);
-                    if (grp < GROUPS && pgi >= 0 && (all || (key <= x.t.phi && (key >= lo || key < a.n_sink)))) {
-                        const uint8_t* pg = pool + (long)pgi * a.c.page_stride;
-                        const int cell = x.h * a.c.ps + (key & (a.c.ps - 1));  // row among the page's
-                        t.raw[i] = *reinterpret_cast<const uint4*>(pg + cell * D + c16 * 16);
-                        t.dl[i] = *reinterpret_cast<const uint16_t*>(pg + a.c.kv_heads * a.c.ps * D +
-                                                                     (cell * (D / 32) + (c16 >> 1)) * 2);
-                    }
-                }
-            };
-            auto convert = [&](uint32_t tile, int batch, bool scan, const Batch& t) {
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const int grp = w3 + 3 * (3 * batch + i), row = grp * RPG + lrow;
-                    if (grp >= GROUPS) continue;
-                    const __half2 d2 = __half2half2(__ushort_as_half(t.dl[i]));
-                    const uint32_t in[4] = {t.raw[i].x, t.raw[i].y, t.raw[i].z, t.raw[i].w};
-                    uint32_t w[8];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint2 y = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
-                        const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&y.x), d2);
-                        const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&y.y), d2);
-                        w[2 * j] = *reinterpret_cast<const uint32_t*>(&h0);
-                        w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
-                    }
-                    if (scan) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if ((w[j] & 0x7c00u) == 0x7c00u) { w[j] &= 0xffff0000u; sm.odd = 1; }
-                            if ((w[j] & 0x7c000000u) == 0x7c000000u) { w[j] &= 0x0000ffffu; sm.odd = 1; }
-                        }
-                    }
-                    const uint32_t at = tile + (c16 >> 2) * HALF + row * 128;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                         at + ((((2 * c16 + j) & 7) ^ (row & 7)) << 4)),
-                                     "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
-                                     : "memory");
-                }
-            };
-            Batch cur, nxt;
-            if (left > 0) {
-                find_pages();
-                load(a.c.k, 0, cur);
-            }
-            while (left > 0 && ok) {
-                const bool scan = !seen_whole(paged_unit_key<CH_KEYS>(x.t, x.u));
 #pragma unroll 1
-                for (int j = 0; j < 2 * NB && ok; ++j) {
-                    const int kv = j >= NB, jb = kv ? j - NB : j;
-                    if (j + 1 < 2 * NB) {
-                        load(j + 1 >= NB ? a.c.v : a.c.k, j + 1 >= NB ? j + 1 - NB : j + 1, nxt);
-                    } else if (--left > 0) {  // the next unit, of this item or the next
-                        if (++x.u == x.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
-                        find_pages();
-                        load(a.c.k, 0, nxt);
-                    }
-                    if (jb == 0) ok = kv ? wait(&sm.v_empty[vs], v_ph) : wait(&sm.k_empty[ks], k_ph);
+                for (int kv = 0; kv < 2 && ok; ++kv) {
+                    ok = wait(&sm.raw_full[kv][rs], r_ph) && (kv ? wait(&sm.v_empty[vs], v_ph) : wait(&sm.k_empty[ks], k_ph));
                     if (!ok) break;
-                    convert(kv ? sv + vs * C::TILE : sk + ks * C::TILE, jb, kv && scan, cur);
-                    if (jb == NB - 1) {
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(kv ? &sm.v_full[vs] : &sm.k_full[ks]);
+                    const uint32_t raw = sq + C::RAW0 + (kv * RSD + rs) * C::RAW;
+                    const uint32_t tile = kv ? sv + vs * C::TILE : sk + ks * C::TILE;
+#pragma unroll 2
+                    for (int grp = w3; grp < GROUPS; grp += 3) {
+                        const int row = grp * RPG + lrow, key = kb + row;
+                        uint4 f = lds16(raw + row * D + c16 * 16);
+                        uint16_t d1;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(d1) : "r"(raw + 128 * D + (row * (D / 32) + (c16 >> 1)) * 2) : "memory");
+                        if (!all && (key > x.t.phi || (key < lo && key >= a.n_sink))) {  // nobody sees it: zeros
+                            f = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                            d1 = 0;
+                        }
+                        const __half2 d2 = __half2half2(__ushort_as_half(d1));
+                        const uint32_t in[4] = {f.x, f.y, f.z, f.w};
+                        uint32_t w[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint2 q = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
+                            const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&q.x), d2);
+                            const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&q.y), d2);
+                            w[2 * j] = *reinterpret_cast<const uint32_t*>(&h0);
+                            w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                        }
+                        if (kv && scan) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                if ((w[j] & 0x7c00u) == 0x7c00u) { w[j] &= 0xffff0000u; sm.odd = 1; }
+                                if ((w[j] & 0x7c000000u) == 0x7c000000u) { w[j] &= 0x0000ffffu; sm.odd = 1; }
+                            }
+                        }
+                        const uint32_t at = tile + (c16 >> 2) * HALF + row * 128;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                             at + ((((2 * c16 + j) & 7) ^ (row & 7)) << 4)),
+                                         "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                                         : "memory");
                     }
-                    cur = nxt;
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(kv ? &sm.v_full[vs] : &sm.k_full[ks]);
+                        mbar_arrive(&sm.raw_empty[kv][rs]);
+                    }
+                }
+                if (!ok) break;
+                if (++rs == RSD) {
+                    rs = 0;
+                    r_ph ^= 1u;
                 }
                 if (++ks == C::KS) {
                     ks = 0;
@@ -789,7 +807,13 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     vs = 0;
                     v_ph ^= 1u;
                 }
+                if (warp == 9 && ahead > 0) fetch();
+                if (--left > 0 && ++x.u == x.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
             }
+            // a wait has run out somewhere: the copies in flight end before the shared memory goes
+            if (warp == 9 && sm.abort != 0)
+                for (int i = max(0, asked - RSD); i < asked; ++i)
+                    for (int kv = 0; kv < 2; ++kv) tc_wait(&sm.raw_full[kv][i % RSD], (uint32_t)(i / RSD) & 1u, a.err);
         }
     }
     tc_fence_before();
