@@ -40,7 +40,7 @@ struct ChunkCfg {
     static constexpr int KS = D == 64 ? 3 : Q8 ? 1 : 2, VS = D == 64 ? 3 : 2;
     static constexpr int RS = Q8 ? (D == 64 ? 2 : 1) : 0;
     static constexpr int RAW = 128 * (D + D / 16);  // 128 rows of 8-bit values, then their deltas
-    static constexpr int STAGE = 32 * 64;  // bytes per softmax warp: 32 rows x 32 fp16 outputs on their way out
+    static constexpr int STAGE = 32 * 32;  // bytes per softmax warp: 32 rows x 16 fp16 outputs on their way out
     static constexpr int OUT = (2 + KS + VS) * TILE, RAW0 = OUT + 8 * STAGE;  // offsets
     static constexpr int SMEM = 1024 + RAW0 + 2 * RS * RAW;
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
@@ -177,9 +177,9 @@ struct ChunkSmem {
     unsigned pre[CH_THREADS], wsum[CH_THREADS / 32];
 };
 
-// Adds the values that were set aside (non-finite) to a row's columns c0 .. c0 + 31, as far as it sees them.
+// Adds the values that were set aside (non-finite) to a row's columns c0 .. c0 + 15, as far as it sees them.
 static __device__ __noinline__ void ch_add_odd(const PagedAttnArgs& a, const PagedPos& x, int u0, int u1, int pos, int wlo,
-                                               int c0, float (&v)[32]) {
+                                               int c0, float (&v)[16]) {
     for (int u = u0; u < u1; ++u) {
         const int kb = paged_unit_key<CH_KEYS>(x.t, u);
         for (int key = kb; key < kb + CH_KEYS && key <= pos; ++key) {
@@ -187,7 +187,7 @@ static __device__ __noinline__ void ch_add_odd(const PagedAttnArgs& a, const Pag
             const int page = a.table[x.b * a.table_stride + (key >> a.c.ps_shift)];
             if ((unsigned)page >= (unsigned)a.c.n_pages) continue;
             const uint8_t* pg = a.c.v + (long)page * a.c.page_stride;
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < 16; ++j) {
                 const float y = paged_elem(a.c, pg, x.h, key & (a.c.ps - 1), c0 + j);
                 if (!(fabsf(y) < INFINITY)) v[j] += y;
             }
@@ -199,19 +199,41 @@ static __device__ __noinline__ void ch_add_odd(const PagedAttnArgs& a, const Pag
 static __device__ __noinline__ uint4 ch_q8_query(const PagedAttnArgs& a, const PagedPos& x, int row, int e0, int d) {
     return paged_q8x(a.q + paged_row_at(a, x.r.first, x.h, x.tile, row, CH_ROWS, a.qs, row_bytes(GTN_Q8, d)), GTN_Q8, e0);
 }
-static __device__ __noinline__ void ch_q8_store(const PagedAttnArgs& a, const PagedPos& x, int row, int c0, int d,
-                                                const float (&v)[32]) {
-    uint8_t* blk = a.out + paged_row_at(a, x.r.first, x.h, x.tile, row, CH_ROWS, a.os, row_bytes(GTN_Q8, d)) +
-                   c0 / GTN_QBLK * GTN_Q8_BYTES;
-    float m = 0.0f;
+template <int D>
+static __device__ __noinline__ void ch_q8_rows(const PagedAttnArgs& a, const PagedPos& x, int row, bool live, bool any,
+                                               bool odd, uint32_t to, float inv, int u0, int u1, int pos, int wlo) {
+    uint8_t* blk = a.out + (live ? paged_row_at(a, x.r.first, x.h, x.tile, row, CH_ROWS, a.os, row_bytes(GTN_Q8, D)) : 0);
 #pragma unroll 1
-    for (int i = 0; i < 32; ++i) m = fmaxf(m, fabsf(v[i]));
-    const float delta = m / 127.0f, inv = delta != 0.0f ? 1.0f / delta : 0.0f;
-    *reinterpret_cast<uint16_t*>(blk) = f2h(delta);
-#pragma unroll 1
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t lo = (uint8_t)(int8_t)roundf(v[2 * i] * inv), hi = (uint8_t)(int8_t)roundf(v[2 * i + 1] * inv);
-        reinterpret_cast<uint16_t*>(blk + 2)[i] = (uint16_t)(lo | (hi << 8));
+    for (int c = 0; c < D; c += 32, blk += GTN_Q8_BYTES) {
+        float v[32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t o[16];
+            float y[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = 0u;
+            if (any) {
+                tc_ld16(to + c + 16 * h, o);
+                tc_wait_ld(o);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[j] = __uint_as_float(o[j]);
+            if (odd) ch_add_odd(a, x, u0, u1, pos, wlo, c + 16 * h, y);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[16 * h + j] = y[j] * inv;
+        }
+        // the activation quantizer (warp_quant_block)
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) m = fmaxf(m, fabsf(v[i]));
+        const float delta = m / 127.0f, iv = delta != 0.0f ? 1.0f / delta : 0.0f;
+        if (!live) continue;
+        *reinterpret_cast<uint16_t*>(blk) = f2h(delta);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t lo = (uint8_t)(int8_t)roundf(v[2 * i] * iv), hi = (uint8_t)(int8_t)roundf(v[2 * i + 1] * iv);
+            reinterpret_cast<uint16_t*>(blk + 2)[i] = (uint16_t)(lo | (hi << 8));
+        }
     }
 }
 
@@ -475,51 +497,54 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 const int prow = r * 128 + row;
                 float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<CH_ROWS, D>();
                 const uint32_t stage = sq + C::OUT + warp * C::STAGE;
-                uint8_t* orow[4];  // the rows whose 16 bytes this lane writes
+                const bool odd = n > 0 && sm.odd != 0;
+                if (done && a.io != GTN_F16) {
+                    ch_q8_rows<D>(a, was, prow, live, n > 0, odd, to, inv, u0, u1, pos, wlo);
+                } else {
+                    uint8_t* orow[2];  // the rows whose 16 bytes this lane writes
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int rw = r * 128 + (warp & 3) * 32 + 8 * i + (lane >> 2);
-                    orow[i] = was.tile * CH_ROWS + rw < was.r.n * a.group
-                                  ? a.out + paged_row_at(a, was.r.first, was.h, was.tile, rw, CH_ROWS, a.os, hb) + 16 * (lane & 3)
-                                  : nullptr;
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        const int rw = r * 128 + (warp & 3) * 32 + 16 * i + (lane >> 1);
+                        orow[i] = done && was.tile * CH_ROWS + rw < was.r.n * a.group
+                                      ? a.out + paged_row_at(a, was.r.first, was.h, was.tile, rw, CH_ROWS, a.os, hb) + 16 * (lane & 1)
+                                      : nullptr;
+                    }
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    float v[32];
-                    if (n > 0) {
-                        ch_ld32(to + 32 * c, o);
-                        ch_wait_ld(o);
-                    }
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        float v[16];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = n > 0 ? __uint_as_float(o[j]) : 0.0f;
-                    if (n > 0 && sm.odd != 0) ch_add_odd(a, was, u0, u1, pos, wlo, 32 * c, v);
-                    if (!done) {
+                        for (int j = 0; j < 16; ++j) o[j] = 0u;
+                        if (n > 0) {
+                            tc_ld16(to + c, o);
+                            tc_wait_ld(o);
+                        }
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) ps[(long)(32 * c + j) * CH_ROWS + prow] = v[j];
-                        continue;
-                    }
+                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(o[j]);
+                        if (odd) ch_add_odd(a, was, u0, u1, pos, wlo, c, v);
+                        if (!done) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = l != 0.0f ? v[j] * inv : 0.0f;
-                    if (a.io != GTN_F16) {
-                        if (live) ch_q8_store(a, was, prow, 32 * c, D, v);
-                        continue;
-                    }
-                    // through shared memory, so that four adjacent lanes write a row's 64 bytes
-                    __syncwarp();
+                            for (int j = 0; j < 16; ++j) ps[(long)(c + j) * CH_ROWS + prow] = v[j];
+                            continue;
+                        }
+                        // through shared memory, so that two adjacent lanes write 16 columns of a row
+                        __syncwarp();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                         stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)),
-                                     "r"(pack_f16(v[8 * j], v[8 * j + 1])), "r"(pack_f16(v[8 * j + 2], v[8 * j + 3])),
-                                     "r"(pack_f16(v[8 * j + 4], v[8 * j + 5])), "r"(pack_f16(v[8 * j + 6], v[8 * j + 7]))
-                                     : "memory");
-                    __syncwarp();
+                        for (int j = 0; j < 2; ++j)
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                             stage + lane * 32 + ((j ^ ((lane >> 2) & 1)) << 4)),
+                                         "r"(pack_f16(v[8 * j] * inv, v[8 * j + 1] * inv)),
+                                         "r"(pack_f16(v[8 * j + 2] * inv, v[8 * j + 3] * inv)),
+                                         "r"(pack_f16(v[8 * j + 4] * inv, v[8 * j + 5] * inv)),
+                                         "r"(pack_f16(v[8 * j + 6] * inv, v[8 * j + 7] * inv))
+                                         : "memory");
+                        __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int lr = 8 * i + (lane >> 2);
-                        const uint4 y = lds16(stage + lr * 64 + (((lane & 3) ^ ((lr >> 1) & 3)) << 4));
-                        if (orow[i]) *reinterpret_cast<uint4*>(orow[i] + 64 * c) = y;
+                        for (int i = 0; i < 2; ++i) {
+                            const int lr = 16 * i + (lane >> 1);
+                            const uint4 y = lds16(stage + lr * 32 + (((lane & 1) ^ ((lr >> 2) & 1)) << 4));
+                            if (orow[i]) *reinterpret_cast<uint4*>(orow[i] + 2 * c) = y;
+                        }
                     }
                 }
                 if (!done && live) {
