@@ -160,7 +160,8 @@ int64_t gtn_paged_page_bytes(int dtype, int page_size, int kv_heads, int d_head)
  *   n_used [1]                   pages taken from the front of free_pages.
  * Requests are served in order. One is not granted when its lengths are negative, its tokens fit
  * neither the table's row nor the `rows` rows, or when it needs pages and those of the requests up to
- * it exceed n_free; the caller plans it again in a later step. The free list itself is not changed. */
+ * it exceed n_free; the caller plans it again in a later step. The free list itself is not changed. The
+ * tensors written must not overlap each other or those read. */
 int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const gtn_tensor* free_pages,
                    const gtn_tensor* n_free, int page_size, gtn_tensor* block_table, gtn_tensor* q_start,
                    gtn_tensor* kv_lens, gtn_tensor* pos, gtn_tensor* slots, gtn_tensor* n_used, void* stream);
@@ -170,7 +171,7 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
  * rows into the pages of slots[r]. q [rows, heads * d_head], k and v [rows, kv_heads * d_head]: fp32, fp16
  * or Q8, one type, row strides as in their descriptors (they may be column ranges of one stacked
  * projection); q_out [rows, heads * d_head]: fp16 or Q8; pos and slots: int32 [rows]. q_out may be q's own
- * memory when type and strides agree. Q8 results use the activation quantizer (gtn_quantize_q8_rows), but
+ * memory when type and strides agree, else it lies apart from q, k and v. Q8 results use the activation quantizer (gtn_quantize_q8_rows), but
  * Q8 value rows go to a Q8 cache unchanged. Rows with pos < 0 are skipped, rows with slot < 0 write no
  * cache row; two rows must not share a slot. */
 int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor* v, const gtn_tensor* pos,
@@ -183,8 +184,10 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
  * j > p - window or j < n_sink. out = sum_j softmax_j(scale q.k_j) v_j; zeros for a row that sees no key
  * (kv_lens[b] = 0: a request that was not granted). Keys that a row does not see never reach it,
  * whatever they hold, and table entries whose page no row of the request sees may be anything.
- *   q, out [rows, heads * d_head]: fp16 (16-byte aligned rows) or Q8, the same type and shape, rows < 2^20;
- *   block_table int32 [n, max_pages], q_start int32 [n + 1], kv_lens int32 [n], n <= 4096;
+ *   q, out [rows, heads * d_head]: fp16 (16-byte aligned rows) or Q8, the same type and shape, rows <= 2^20;
+ *   out may be q's own memory when the strides agree, else it lies apart;
+ *   block_table int32 [n, max_pages], q_start int32 [n + 1], kv_lens int32 [n], n <= 4096, max_pages *
+ *   page_size < 2^30; calls whose rows times keys could exceed 2^31 tiles are refused;
  *   scale: 0 means 1 / sqrt(d_head); max_new: a bound on the new tokens of one request where the caller
  *   knows one (1 for a decode step), else 0: it chooses the kernels, not the result;
  *   workspace: device memory of gtn_paged_attn_workspace(...) bytes, 16-byte aligned; its contents are

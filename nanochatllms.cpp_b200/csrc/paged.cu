@@ -50,6 +50,20 @@ int paged_on_device(const void* const* p, int n, const char* who) {
     return GTN_OK;
 }
 
+PagedSpan paged_span(const gtn_tensor* t) {
+    const uint8_t* p = (const uint8_t*)t->data;
+    const int last = t->ndim - 1;
+    const long rows = t->ndim > 1 ? (long)(t->shape[0] - 1) * bstride(t, 0) : 0;
+    return {p, p + rows + row_bytes(t->dtype, t->shape[last])};
+}
+
+int paged_apart(const gtn_tensor* q, const gtn_tensor* out, const char* who, const char* name) {
+    const bool same = q->data == out->data && q->dtype == out->dtype &&
+                      (q->strides[0] == out->strides[0] || q->shape[0] == 1);
+    GTN_REQUIRE(same || !paged_meet(paged_span(q), paged_span(out)), "%s: %s overlaps an input", who, name);
+    return GTN_OK;
+}
+
 // ---- planner -----------------------------------------------------------------------------------
 // need_b = ceil((ctx + new) / ps) - ceil(ctx / ps) pages, granted while the inclusive prefix of need
 // stays within n_free; q_start = prefix of new. Every CTA runs both prefix sums over all requests itself
@@ -451,6 +465,12 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
     GTN_REQUIRE(pos->shape[0] == slots->shape[0], "%s: pos and slots differ in rows", who);
     GTN_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0, "%s: page_size %d", who,
                 page_size);
+    const gtn_tensor* io[] = {block_table, q_start, kv_lens, pos, slots, n_used, ctx_lens, new_lens, free_pages, n_free};
+    PagedSpan span[10];
+    for (int i = 0; i < 10; ++i) span[i] = paged_span(io[i]);
+    for (int i = 0; i < 6; ++i)
+        for (int j = i + 1; j < 10; ++j)
+            GTN_REQUIRE(!paged_meet(span[i], span[j]), "%s: tensors that are written overlap others", who);
     const void* ptrs[] = {ctx_lens->data, new_lens->data, free_pages->data, n_free->data, block_table->data,
                           q_start->data,  kv_lens->data,  pos->data,        slots->data,  n_used->data};
     GTN_CHECK(paged_on_device(ptrs, 10, who));
@@ -504,16 +524,17 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
         GTN_REQUIRE(t->dtype != GTN_Q8 || t->strides[0] % GTN_QBLK == 0, "%s: Q8 row stride %d", who, t->strides[0]);
         GTN_REQUIRE((uintptr_t)t->data % (t->dtype == GTN_F32 ? 4 : 2) == 0, "%s: row alignment", who);
     }
-    const uint8_t *qb = (const uint8_t*)q->data, *ob = (const uint8_t*)q_out->data;
-    const bool same = qb == ob && q->dtype == q_out->dtype && bstride(q, 0) == bstride(q_out, 0);
-    const long qe = (long)(rows - 1) * bstride(q, 0) + row_bytes(q->dtype, q->shape[1]);
-    const long oe = (long)(rows - 1) * bstride(q_out, 0) + row_bytes(q_out->dtype, q->shape[1]);
-    GTN_REQUIRE(same || ob >= qb + qe || qb >= ob + oe, "%s: q_out overlaps q", who);
+    GTN_CHECK(paged_apart(q, q_out, who, "q_out"));
+    if (q->data != q_out->data) {
+        GTN_CHECK(paged_apart(k, q_out, who, "q_out"));
+        GTN_CHECK(paged_apart(v, q_out, who, "q_out"));
+        GTN_REQUIRE(k->data != q_out->data && v->data != q_out->data, "%s: q_out is k or v", who);
+    }
     GTN_REQUIRE(rope_pct >= 0.0f && rope_pct <= 1.0f, "%s: rope_pct", who);
     GTN_REQUIRE(rope_base > 0.0f && std::isfinite(rope_base), "%s: rope_base", who);
     const void* ptrs[] = {q->data, k->data, v->data, q_out->data, pos->data, slots->data, a.c.k, a.c.v};
     GTN_CHECK(paged_on_device(ptrs, 8, who));
-    a.q = qb;
+    a.q = (const uint8_t*)q->data;
     a.k = (const uint8_t*)k->data;
     a.v = (const uint8_t*)v->data;
     a.out = (uint8_t*)q_out->data;

@@ -41,6 +41,14 @@ int paged_int_arg(const gtn_tensor* t, int ndim, const char* who, const char* na
 // Every pointer lies in memory that the current device owns (or managed memory). Turns a host pointer or
 // another device's tensor into an error before a kernel meets it.
 int paged_on_device(const void* const* p, int n, const char* who);
+// The bytes [data, end) that a tensor's rows span, and whether two tensors' spans meet.
+struct PagedSpan {
+    const uint8_t *data, *end;
+};
+PagedSpan paged_span(const gtn_tensor* t);
+inline bool paged_meet(const PagedSpan& x, const PagedSpan& y) { return x.data < y.end && y.data < x.end; }
+// out may be q's own memory row for row, else it must lie apart from it.
+int paged_apart(const gtn_tensor* q, const gtn_tensor* out, const char* who, const char* name);
 
 // Attributes common to the kernels: nothing is read before the previous kernel in the stream is done.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -107,8 +107,6 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     GTN_REQUIRE(n <= PAGED_MAX_REQ, "%s: %d requests (at most %d)", who, n, PAGED_MAX_REQ);
     GTN_REQUIRE(block_table->shape[0] == n && q_start->shape[0] == n + 1, "%s: shapes do not agree on %d requests", who,
                 n);
-    GTN_REQUIRE((long)block_table->shape[1] * a.c.ps < (1L << 31), "%s: block_table of %d pages a row", who,
-                block_table->shape[1]);
     GTN_REQUIRE(q->ndim == 2 && out->ndim == 2 && shape_eq(q, out), "%s: q and out must be 2-D, of one shape", who);
     GTN_REQUIRE(q->dtype == out->dtype && (q->dtype == GTN_F16 || q->dtype == GTN_Q8), "%s: q / out dtypes %d, %d", who,
                 q->dtype, out->dtype);
@@ -117,10 +115,14 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     GTN_REQUIRE(heads % a.c.kv_heads == 0, "%s: heads %d not a multiple of kv heads %d", who, heads, a.c.kv_heads);
     // what the kernels count in 32 bits: rows by the group (paged_group), units on the line
     const long group = heads / a.c.kv_heads, rows = q->shape[0], cap = (long)block_table->shape[1] * a.c.ps;
-    GTN_REQUIRE(rows * group * group < (1L << 32) && rows * heads < (1L << 31), "%s: %ld rows of %d heads", who, rows, heads);
-    const long few = max_new > 0 && max_new * group <= 16 ? rows * group : 0;  // tiles of the decode kernel beyond one a request
-    GTN_REQUIRE(((few + n) * (cap / 16 + 2)) * a.c.kv_heads < (1L << 31) &&
-                    ((rows * group / CH_ROWS + n) * (cap / CH_KEYS + 2)) * a.c.kv_heads < (1L << 31),
+    GTN_REQUIRE(rows <= (1 << 20) && (rows * group + CH_ROWS) * group < (1L << 32) && rows * heads < (1L << 31),
+                "%s: %ld rows of %d heads", who, rows, heads);
+    GTN_REQUIRE(cap < (1L << 30), "%s: block_table of %d pages a row", who, block_table->shape[1]);
+    const bool small = max_new > 0 && max_new * group <= 16;
+    const long few = small ? rows * group : 0;  // tiles of the decode kernel beyond one a request
+    const long few_units = (few + n) * (cap / 16 + 2) * a.c.kv_heads;
+    const long many_units = (rows * group / CH_ROWS + n) * (cap / CH_KEYS + 2) * a.c.kv_heads;
+    GTN_REQUIRE(few_units < 0x7fffffffL && many_units < 0x7fffffffL,
                 "%s: %ld rows of %d requests over tables of %ld keys are too many for one call", who, rows, n, cap);
     const gtn_tensor* rt[] = {q, out};
     for (const gtn_tensor* t : rt) {
@@ -131,6 +133,7 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
         else
             GTN_REQUIRE((uintptr_t)t->data % 2 == 0 && t->strides[0] % GTN_QBLK == 0, "%s: Q8 row alignment", who);
     }
+    GTN_CHECK(paged_apart(q, out, who, "out"));
     GTN_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "%s: scale", who);
     GTN_REQUIRE(window >= 0 && n_sink >= 0, "%s: window %d, n_sink %d", who, window, n_sink);
     GTN_REQUIRE(max_new >= 0, "%s: max_new", who);
@@ -155,7 +158,8 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     a.group = (int)group;
     a.group_mul = group > 1 ? (unsigned)(((1ull << 32) + group - 1) / group) : 0;
     a.cap = cap;
-    a.window = window;
+    a.most = (unsigned)few_units;
+    a.window = window < cap ? window : 0;  // a window of all keys is none (and positions minus it stay in 32 bits)
     a.n_sink = n_sink;
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)d)) * 1.4426950408889634f;
     a.part = (float*)workspace;
@@ -169,7 +173,7 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     p.cut = a.group <= 8 ? 8 : a.group <= 16 ? 16 : 0;
     const long most = max_new > 0 ? (long)max_new * a.group : 0x7fffffffL;
     cudaError_t e = cudaSuccess;
-    if (most <= 16) {
+    if (small) {
         p.cut = 0x7fffffff;
         if (most == 1 && a.c.dt == GTN_Q8)
             e = d == 64 ? launch_decode<GTN_Q8, 64, 1>(a, p, 1, a, 0, S(stream))
@@ -178,6 +182,7 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
             e = most <= 8 ? decode<8>(a, p, (int)most, a, 0, S(stream)) : decode<16>(a, p, (int)most, a, 0, S(stream));
     } else {
         PagedAttnArgs c = a;
+        c.most = (unsigned)many_units;
         c.part = (float*)((uint8_t*)workspace + decode_ws_bytes(d));
         if (n == 1) p.cut = 0;
         PagedPick rest = p;

@@ -286,10 +286,10 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
     const int me = blockIdx.x;
     if (tid == 0) a.join[me].last = -1;
     tc_fence_before();
-    paged_sched<CH_ROWS, CH_KEYS, CH_THREADS, true>(a, p, me == 0, sm.pre, sm.wsum);
+    const unsigned total = paged_sched<CH_ROWS, CH_KEYS, CH_THREADS, true>(a, p, me == 0, sm.pre, sm.wsum);
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    const unsigned total = sm.pre[CH_THREADS - 1], share = paged_share(total, a.workers_mul);
+    const unsigned share = paged_share(total, a.workers_mul);
     PagedPos x{};
     int left = 0;
     if (share * (unsigned)me < total) {
@@ -733,6 +733,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             const int lrow = lane / CPR, c16 = lane % CPR, w3 = warp - 9;
             PagedPos y = x;  // warp 9: the unit whose bytes are asked for next
             int ahead = left, asked = 0, page = -1;
+            bool k_only = false;  // K of unit `asked` is on its way, V is not
             auto fetch = [&]() {  // K and V of the unit at y
                 const int slot = asked % RSD;
                 const int lo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
@@ -759,6 +760,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     if (page >= 0)
                         ch_bulk(sq + C::RAW0 + (kv * RSD + slot) * C::RAW + dst, (kv ? a.c.v : a.c.k) + off, dl ? D : 16 * D,
                                 &sm.raw_full[kv][slot]);
+                    k_only = kv == 0;
                 }
                 ++asked;
                 if (--ahead > 0 && ++y.u == y.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, y);
@@ -837,8 +839,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             }
             // a wait has run out somewhere: the copies in flight end before the shared memory goes
             if (warp == 9 && sm.abort != 0)
-                for (int i = max(0, asked - RSD); i < asked; ++i)
-                    for (int kv = 0; kv < 2; ++kv) tc_wait(&sm.raw_full[kv][i % RSD], (uint32_t)(i / RSD) & 1u, a.err);
+                for (int i = max(0, asked - RSD); i <= asked; ++i)
+                    for (int kv = 0; kv < 2 && (i < asked || (k_only && kv == 0)); ++kv)
+                        tc_wait(&sm.raw_full[kv][i % RSD], (uint32_t)(i / RSD) & 1u, a.err);
         }
     }
     tc_fence_before();

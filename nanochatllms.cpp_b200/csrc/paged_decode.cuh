@@ -129,8 +129,8 @@ __global__ void __launch_bounds__(32 * PD_WARPS, DecodeCfg<DT, D, ROWS>::OCC) k_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const unsigned me = blockIdx.x * PD_WARPS + warp;
     if (lane == 0) a.join[me].last = -1;
-    paged_sched<ROWS, KEYS, 32 * PD_WARPS, false>(a, p, blockIdx.x == 0, s_pre, s_wsum);
-    const unsigned total = s_pre[32 * PD_WARPS - 1], share = max(PD_SHARE, paged_share(total, a.workers_mul));
+    const unsigned total = paged_sched<ROWS, KEYS, 32 * PD_WARPS, false>(a, p, blockIdx.x == 0, s_pre, s_wsum);
+    const unsigned share = max(PD_SHARE, paged_share(total, a.workers_mul));
     if (share * me >= total) {
         if (p.chained) pdl_wait();
         return;

@@ -37,6 +37,7 @@ struct PagedAttnArgs {
     int n_req, rows, heads, group, window, n_sink;
     unsigned group_mul;  // floor(x / group) = umulhi(x, group_mul) for x < 2^32 / group (0: group is 1)
     long cap;          // keys that a row of the table can hold
+    unsigned most;     // units that a kernel can have for lengths that agree with the tensors
     unsigned workers_mul;  // floor(2^32 / workers) + 1
     float scale_log2;  // scale * log2(e): the softmax runs in base 2
     float* part;       // scratch slots: [worker][2] of ROWS * (D + 2) floats
@@ -45,7 +46,7 @@ struct PagedAttnArgs {
 };
 
 // A request's rows as the kernels take them: row i of [0, n) sits at position base + i; lengths that the
-// table or the row tensor cannot hold are flagged and cut.
+// table cannot hold are flagged and cut; rows behind the tensor's end (a plan's refused requests) are cut.
 struct PagedReq {
     int first;  // row of token 0 in q and out
     int n;      // tokens
@@ -127,12 +128,16 @@ __device__ __forceinline__ unsigned paged_warp_units(const PagedAttnArgs& a, con
 
 // pre[i]: units of the requests of threads 0 .. i of THREADS, thread i holding `per` requests from i * per on.
 // By the whole CTA; ends with a barrier. BIG: requests of many tiles are common (each is summed by a warp).
+// Returns the units of all, or 0 (and flags it) if they are more than valid lengths can give: row ranges that
+// overlap must not become work without end. Sums stop at 2^31 - 1, which a single request's units do not reach
+// (the host refuses such calls).
+__device__ __forceinline__ unsigned paged_add(unsigned x, unsigned y) { return min(x + y, 0x7fffffffu); }
 template <int ROWS, int KEYS, int THREADS, bool BIG>
-__device__ __forceinline__ void paged_sched(const PagedAttnArgs& a, const PagedPick& p, bool flag, unsigned* pre,
+__device__ __forceinline__ unsigned paged_sched(const PagedAttnArgs& a, const PagedPick& p, bool flag, unsigned* pre,
                                             unsigned* wsum) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.n_req + THREADS - 1) / THREADS;
-    unsigned mine = 0;
+    unsigned mine = 0, units;
 #pragma unroll 1
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
@@ -140,6 +145,7 @@ __device__ __forceinline__ void paged_sched(const PagedAttnArgs& a, const PagedP
         r.first = r.n = r.base = 0;
         if (b < a.n_req) r = paged_req(a, b, flag);
         const int nt = paged_tiles<ROWS>(a, p, r);
+        units = 0;
         if (BIG) {
             for (unsigned any = __ballot_sync(0xffffffffu, nt > 0); any; any &= any - 1) {
                 const int src = __ffs(any) - 1;
@@ -148,24 +154,28 @@ __device__ __forceinline__ void paged_sched(const PagedAttnArgs& a, const PagedP
                 q.n = __shfl_sync(0xffffffffu, r.n, src);
                 q.base = __shfl_sync(0xffffffffu, r.base, src);
                 const unsigned one = paged_warp_units<ROWS, KEYS>(a, q, __shfl_sync(0xffffffffu, nt, src));
-                if (lane == src) mine += one;
+                if (lane == src) units = one;
             }
         } else {
 #pragma unroll 1
-            for (int t = 0; t < nt; ++t) mine += paged_tile<ROWS, KEYS>(a, r, t).units;
+            for (int t = 0; t < nt; ++t) units += paged_tile<ROWS, KEYS>(a, r, t).units;
         }
+        mine = paged_add(mine, units * a.c.kv_heads);
     }
-    mine *= a.c.kv_heads;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned y = __shfl_up_sync(0xffffffffu, mine, o);
-        if (lane >= o) mine += y;
+        if (lane >= o) mine = paged_add(mine, y);
     }
     if (lane == 31) wsum[warp] = mine;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) mine += wsum[w];
+    for (int w = 0; w < warp; ++w) mine = paged_add(mine, wsum[w]);
     pre[tid] = mine;
     __syncthreads();
+    const unsigned total = pre[THREADS - 1];
+    if (total <= a.most) return total;
+    if (flag && tid == 0) atomicOr(a.err, GTN_DEVERR_PAGE);
+    return 0;
 }
 // Units per worker, a bit more than total / workers at most (the same for every worker).
 __device__ __forceinline__ unsigned paged_share(unsigned total, unsigned workers_mul) {

@@ -120,3 +120,52 @@ def test_reference_planner_by_hand():
     assert q_start == [0, 2, 7, 8, 9] and kv == [5, 5, 0, 2] and used == 3
     assert pos == [3, 4, 0, 1, 2, 3, 4, 4, 1, -1]
     assert slots == [31, 40, 44, 45, 46, 47, 48, -1, 37, -1]
+
+
+FAR = [P + (i << 20) for i in range(12)]
+
+
+def far_plan(**kw):
+    """A plan whose tensors lie apart."""
+    names = dict(ctx_lens=(3,), new_lens=(3,), free_pages=(9,), n_free=(1,), block_table=(3, 4), q_start=(4,), kv_lens=(3,),
+                 pos=(7,), slots=(7,), n_used=(1,))
+    a = {n: t(G.I32, *shape, buf=at) for (n, shape), at in zip(names.items(), FAR)}
+    a.update({n: t(G.I32, *names[n], buf=FAR[list(names).index(o)] + 4 * at) for n, (o, at) in kw.items()})
+    G.paged_plan(page_size=16, stream=0, **a)
+
+
+@pytest.mark.parametrize("bad", [dict(kv_lens=("ctx_lens", 0)), dict(n_used=("n_free", 0)), dict(slots=("pos", 6)),
+                                 dict(q_start=("new_lens", 2)), dict(block_table=("free_pages", 8)),
+                                 dict(ctx_lens=("block_table", 11)), dict(pos=("kv_lens", 1))], ids=str)
+def test_plan_outputs_lie_apart(bad):
+    with pytest.raises(G.GtenError, match="overlap"):
+        far_plan(**bad)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(out=t(G.F16, 5, 256, buf=P + 512)), dict(out=t(G.F16, 5, 256, strides=(512, 1))),
+    dict(q=t(G.F16, 5, 256, buf=P + 5 * 512 - 16)), dict(q=t(G.Q8, 5, 256, buf=P + 34), out=t(G.Q8, 5, 256))], ids=str)
+def test_attn_output_lies_apart(bad):
+    with pytest.raises(G.GtenError, match="overlap"):
+        attn(**bad)
+
+
+@pytest.mark.parametrize("bad", [dict(k=t(G.F16, 5, 128, buf=P + 65536 + 64)), dict(v=t(G.F16, 5, 128, buf=P + 65536 + 2304)),
+                                 dict(k=t(G.F16, 5, 128, buf=P + 65536, strides=(256, 1)))], ids=str)
+def test_append_output_lies_apart(bad):
+    with pytest.raises(G.GtenError, match="status 1.*q_out"):
+        append(**bad)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(cache=cache(page_stride=1 << 31)), dict(cache=cache(page_stride=(1 << 40) + 16)),
+    dict(q=t(G.F16, (1 << 20) + 1, 256), out=t(G.F16, (1 << 20) + 1, 256)),
+    dict(block_table=t(G.I32, 3, 1 << 26)),                                                     # 2^30 keys a row
+    dict(cache=cache(kv_heads=1024), q=t(G.F16, 1 << 20, 1 << 17), out=t(G.F16, 1 << 20, 1 << 17)),  # rows * heads
+    dict(cache=cache(page_size=256, kv_heads=1, d_head=64), q=t(G.F16, 1 << 20, 2048), out=t(G.F16, 1 << 20, 2048),
+         block_table=t(G.I32, 3, 1 << 15)),                                                     # rows * group units of keys
+    dict(cache=cache(page_size=256, kv_heads=8), q=t(G.F16, 5, 512), out=t(G.F16, 5, 512), block_table=t(G.I32, 4096, 1 << 12),
+         q_start=t(G.I32, 4097), kv_lens=t(G.I32, 4096))], ids=str)
+def test_attn_calls_that_32_bits_cannot_count(bad):
+    with pytest.raises(G.GtenError, match="status 1"):
+        attn(**bad)
