@@ -34,15 +34,17 @@ constexpr float CH_GROW = 8.0f;
 template <int DT, int D>
 struct ChunkCfg {
     static constexpr int TILE = 128 * D * 2;  // bytes of a Q, K or V tile
-    // tiles of K and V in flight; for a Q8 cache also the pages' bytes of RS tiles each (at D = 128 one of K less
-    // makes room for them)
     static constexpr bool Q8 = DT == GTN_Q8;
-    static constexpr int KS = D == 64 ? 3 : Q8 ? 1 : 2, VS = D == 64 ? 3 : 2;
-    static constexpr int RS = Q8 ? (D == 64 ? 2 : 1) : 0;
-    static constexpr int RAW = 128 * (D + D / 16);  // 128 rows of 8-bit values, then their deltas
+    // Stages of K and V in flight. A Q8 element is two fp16 values (rounded product, rest) in two tiles of a stage.
+    static constexpr int KS = D == 64 ? (Q8 ? 2 : 3) : Q8 ? 1 : 2, VS = KS;
+    static constexpr int PARTS = Q8 ? 2 : 1, STG = PARTS * TILE;
+    // Q8 pages' bytes on their way: groups of GH 64-key halves of a unit's four (K, K, V, V), two groups; a half is
+    // 64 rows of 8-bit values, then their deltas
+    static constexpr int GH = D == 64 ? 4 : 1;
+    static constexpr int RAW = 64 * (D + D / 16), RAWS = Q8 ? 2 * GH * RAW : 0;
     static constexpr int STAGE = 32 * 32;  // bytes per softmax warp: 32 rows x 16 fp16 outputs on their way out
-    static constexpr int OUT = (2 + KS + VS) * TILE, RAW0 = OUT + 8 * STAGE;  // offsets
-    static constexpr int SMEM = 1024 + RAW0 + 2 * RS * RAW;
+    static constexpr int OUT = 2 * TILE + (KS + VS) * STG, RAW0 = OUT + 8 * STAGE;  // offsets
+    static constexpr int SMEM = 1024 + RAW0 + RAWS;
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
     // Keys per score product. 64: the next unit's scores of a half start as soon as the half's weights are
     // used, so the softmax does not wait for them. But at N = 64 the operands (Q again for every half) come out
@@ -169,7 +171,7 @@ __device__ __forceinline__ void ch_bulk(uint32_t dst, const void* src, uint32_t 
 
 struct ChunkSmem {
     uint64_t k_full[3], k_empty[3], v_load[3], v_full[3], v_empty[3];
-    uint64_t raw_full[2][2], raw_empty[2][2];  // Q8: K and V, per raw tile
+    uint64_t raw_full[2], raw_empty[2];  // Q8: per group of halves
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain;  // s, p: per tile and 64-key half
     uint32_t tmem;
     volatile int abort;
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ ChunkSmem sm;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sq = base, sk = sq + 2 * C::TILE, sv = sk + C::KS * C::TILE;
+    const uint32_t sq = base, sk = sq + 2 * C::TILE, sv = sk + C::KS * C::STG;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
@@ -272,9 +274,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             mbar_init(&sm.pv_done[r], 1);
             mbar_init(&sm.o_full[r], 1);
         }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&sm.raw_full[i >> 1][i & 1], 1);
-            mbar_init(&sm.raw_empty[i >> 1][i & 1], 3);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.raw_full[i], C::GH);
+            mbar_init(&sm.raw_empty[i], 3);
         }
         mbar_init(&sm.drain, 1);
         sm.abort = 0;
@@ -561,17 +563,19 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             // ---- MMA issue
             const uint32_t leader = ch_elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
             const uint32_t q0 = __shfl_sync(0xffffffffu, sq, 0);
-            const uint32_t k0 = q0 + 2 * C::TILE, v0 = k0 + C::KS * C::TILE;
+            const uint32_t k0 = q0 + 2 * C::TILE, v0 = k0 + C::KS * C::STG;
             int ks = 0, vs = 0;
             uint32_t k_ph = 0, v_ph = 0, q_ph = 0, p_ph = 0;
             bool ok = true;
             // scores of half b of the unit in stage ks, or (b = 0) of both halves; `two`: the second is wanted
             auto qk = [&](int r, int b, bool two) {
-                const uint64_t qd = ch_desc(q0 + r * C::TILE, 16), kd = ch_desc(k0 + ks * C::TILE + b * 8192, 16);
+                const uint64_t qd = ch_desc(q0 + r * C::TILE, 16), kd = ch_desc(k0 + ks * C::STG + b * 8192, 16);
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t off = ((i >> 2) * HALF + (i & 3) * 32) >> 4;
-                    ch_mma_ss(tm + r * 128 + b * 64, qd + off, kd + off, C::IDESC_S, i > 0, leader);
+                for (int i = 0; i < C::PARTS * (D / 16); ++i) {
+                    const int e = i % (D / 16);
+                    const uint32_t off = ((e >> 2) * HALF + (e & 3) * 32) >> 4;
+                    ch_mma_ss(tm + r * 128 + b * 64, qd + off, kd + off + (i >= D / 16 ? C::TILE >> 4 : 0), C::IDESC_S, i > 0,
+                              leader);
                 }
                 ch_commit(&sm.s_full[r][b], leader);
                 if (C::SN == 128 && two) ch_commit(&sm.s_full[r][1], leader);
@@ -604,11 +608,11 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                         if (!(ok = wait(&sm.p_full[r][b], (p_ph >> i) & 1u))) break;
                         p_ph ^= 1u << i;
                         tc_fence_after();
-                        const uint64_t vd = ch_desc(v0 + vs * C::TILE + b * 8192, HALF);
+                        const uint64_t vd = ch_desc(v0 + vs * C::STG + b * 8192, HALF);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            ch_mma_ts(tm + C::COL_O + r * D, tm + r * 128 + b * 64 + j * 8, vd + (j * 2048 >> 4), C::IDESC_O,
-                                      q > 0 || j > 0, leader);
+                        for (int j = 0; j < 4 * C::PARTS; ++j)
+                            ch_mma_ts(tm + C::COL_O + r * D, tm + r * 128 + b * 64 + (j & 3) * 8,
+                                      vd + (((j & 3) * 2048 + (j >> 2) * C::TILE) >> 4), C::IDESC_O, q > 0 || j > 0, leader);
                         ch_commit(&sm.pv_done[r], leader);
                         if (C::SN == 64 ? q + 2 < nr : b == 1 && q + 1 < nr) qk(r, C::SN == 64 ? b : 0, q + 2 < nr);
                         if (q + 1 == nr) ch_commit(&sm.o_full[r], leader);
@@ -649,7 +653,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     __syncwarp();
                     if (lane < pieces)
                         for (int h = 0; h < HALVES; ++h)
-                            tma_load_3d(sk + ks * C::TILE + h * HALF + lane * box * 128, &kmap, 64 * h, yrow, page,
+                            tma_load_3d(sk + ks * C::STG + h * HALF + lane * box * 128, &kmap, 64 * h, yrow, page,
                                         &sm.k_full[ks]);
                     ++k_issued;
                     if (++ks == C::KS) {
@@ -661,7 +665,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     __syncwarp();
                     if (lane < pieces)
                         for (int h = 0; h < HALVES; ++h)
-                            tma_load_3d(sv + vs * C::TILE + h * HALF + lane * box * 128, &vmap, 64 * h, yrow, page,
+                            tma_load_3d(sv + vs * C::STG + h * HALF + lane * box * 128, &vmap, 64 * h, yrow, page,
                                         &sm.v_load[vs]);
                     ++v_issued;
                     if (++vs == C::VS) {
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                         const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
                         for (int i = ct; i < HALVES * 1024; i += 64) {
                             const int key = kb + ((i >> 3) & 127);
-                            const uint32_t at = sv + vs * C::TILE + i * 16;
+                            const uint32_t at = sv + vs * C::STG + i * 16;
                             const bool seen = key <= x.t.phi && (key >= lo || key < a.n_sink);
                             uint4 v = lds16(at);
                             uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -723,109 +727,123 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 next_item(u1 - u0);
             }
         } else {
-            // ---- Q8 pages to fp16 tiles. Warp 9 brings the pages' bytes into shared memory, RS units ahead (bulk
+            // ---- Q8 pages to fp16 tiles. Warp 9 brings the pages' bytes into shared memory, two groups ahead (bulk
             // copies of 16 rows and of their deltas, a lane each); all three convert: a warp takes groups of RPG
             // rows, lane = 16 elements of a row.
             int ks = 0, vs = 0, rs = 0;
             uint32_t k_ph = 1, v_ph = 1, r_ph = 0;
             bool ok = true;
-            constexpr int CPR = D / 16, RPG = 32 / CPR, GROUPS = 128 / RPG, RSD = C::RS > 0 ? C::RS : 1;
-            const int lrow = lane / CPR, c16 = lane % CPR, w3 = warp - 9;
+            constexpr int CPR = D / 16, RPG = 32 / CPR, PASS = C::GH == 4 ? 128 : 64;  // PASS: rows converted in a go
+            const int lrow = lane / CPR, c16 = lane % CPR, w3 = warp == 9 ? 2 : warp - 10;
             PagedPos y = x;  // warp 9: the unit whose bytes are asked for next
-            int ahead = left, asked = 0, page = -1;
-            bool k_only = false;  // K of unit `asked` is on its way, V is not
-            auto fetch = [&]() {  // K and V of the unit at y
-                const int slot = asked % RSD;
+            int ahead = left, asked = 0;
+            auto fetch = [&]() {  // the next group, from the unit at y
+                // lane: half lane / 8 of the group; of its 8, lanes 0-3 copy a 16-key piece's values, 4-7 its deltas
+                const int half = C::GH == 4 ? (lane >> 3) & 3 : asked & 3, piece = 4 * (half & 1) + (lane & 3);
+                const bool mine = lane < 8 * C::GH, dl = lane & 4;
                 const int lo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
-                const int k0 = paged_unit_key<CH_KEYS>(y.t, y.u) + 16 * (lane & 7);
-                // lane i of 8: the 16-key piece i; lanes 0-7 copy the values, 8-15 the deltas
-                page = -1;
-                if (lane < 16 && k0 <= y.t.phi && (k0 + 15 >= lo || k0 < a.n_sink)) {
+                const int k0 = paged_unit_key<CH_KEYS>(y.t, y.u) + 16 * piece;
+                int page = -1;
+                if (mine && k0 <= y.t.phi && (k0 + 15 >= lo || k0 < a.n_sink)) {
                     page = a.table[y.b * a.table_stride + (k0 >> a.c.ps_shift)];
                     if ((unsigned)page >= (unsigned)a.c.n_pages) {
                         page = -1;
                         atomicOr(a.err, GTN_DEVERR_PAGE);
                     }
                 }
-                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0) & 0xffu) * 16 * (D + D / 16);
-                const int cell = y.h * a.c.ps + (k0 & (a.c.ps - 1));  // row among the page's
-                const bool dl = lane >= 8;
-                const long off = (long)max(page, 0) * a.c.page_stride +
-                                 (dl ? (long)a.c.kv_heads * a.c.ps * D + cell * (D / 16) : (long)cell * D);
-                const uint32_t dst = dl ? 128 * D + (lane & 7) * D : (lane & 7) * 16 * D;
-                for (int kv = 0; kv < 2; ++kv) {
-                    if (asked >= C::RS && !(ok = wait(&sm.raw_empty[kv][slot], (uint32_t)(asked / RSD - 1) & 1u))) return;
-                    if (lane == 0) mbar_arrive_expect_tx(&sm.raw_full[kv][slot], bytes);
-                    __syncwarp();
-                    if (page >= 0)
-                        ch_bulk(sq + C::RAW0 + (kv * RSD + slot) * C::RAW + dst, (kv ? a.c.v : a.c.k) + off, dl ? D : 16 * D,
-                                &sm.raw_full[kv][slot]);
-                    k_only = kv == 0;
+                const int slot = asked & 1;
+                if (asked >= 2 && !(ok = wait(&sm.raw_empty[slot], (uint32_t)((asked >> 1) - 1) & 1u))) return;
+                const uint32_t here = __ballot_sync(0xffffffffu, page >= 0) >> (lane & 24) & 0xfu;
+                if (mine && (lane & 7) == 0) mbar_arrive_expect_tx(&sm.raw_full[slot], __popc(here) * 16 * (D + D / 16));
+                __syncwarp();
+                if (page >= 0) {
+                    const int cell = y.h * a.c.ps + (k0 & (a.c.ps - 1));  // row among the page's
+                    const long off = (long)page * a.c.page_stride +
+                                     (dl ? (long)a.c.kv_heads * a.c.ps * D + cell * (D / 16) : (long)cell * D);
+                    ch_bulk(sq + C::RAW0 + (slot * C::GH + (C::GH == 4 ? half : 0)) * C::RAW +
+                                (dl ? 64 * D + (lane & 3) * D : (lane & 3) * 16 * D),
+                            (half & 2 ? a.c.v : a.c.k) + off, dl ? D : 16 * D, &sm.raw_full[slot]);
                 }
                 ++asked;
-                if (--ahead > 0 && ++y.u == y.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, y);
+                if (C::GH == 4 || (asked & 3) == 0)
+                    if (--ahead > 0 && ++y.u == y.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, y);
             };
             if (warp == 9)
-                for (int i = 0; i < C::RS && ahead > 0 && ok; ++i) fetch();
+                for (int i = 0; i < 2 && ahead > 0 && ok; ++i) fetch();
             while (left > 0 && ok) {
                 const int kb = paged_unit_key<CH_KEYS>(x.t, x.u);
                 const bool scan = !seen_whole(kb);
                 const int lo = a.window > 0 ? max(0, x.t.plo - a.window + 1) : 0;
                 const bool all = kb + CH_KEYS - 1 <= x.t.phi && (kb >= lo || kb + CH_KEYS <= a.n_sink);
 #pragma unroll 1
-                for (int kv = 0; kv < 2 && ok; ++kv) {
-                    ok = wait(&sm.raw_full[kv][rs], r_ph) && (kv ? wait(&sm.v_empty[vs], v_ph) : wait(&sm.k_empty[ks], k_ph));
+                for (int q = 0; q < 2 * (128 / PASS) && ok; ++q) {
+                    const int kv = q / (128 / PASS), r0 = PASS == 64 ? 64 * (q & 1) : 0;
+                    const bool first = PASS == 128 || !(q & 1), last = PASS == 128 || (q & 1);
+                    if (C::GH == 1 || q == 0) ok = wait(&sm.raw_full[rs], r_ph);
+                    if (ok && first) ok = kv ? wait(&sm.v_empty[vs], v_ph) : wait(&sm.k_empty[ks], k_ph);
                     if (!ok) break;
-                    const uint32_t raw = sq + C::RAW0 + (kv * RSD + rs) * C::RAW;
-                    const uint32_t tile = kv ? sv + vs * C::TILE : sk + ks * C::TILE;
+                    const uint32_t raw = sq + C::RAW0 + (rs * C::GH + (C::GH == 4 ? 2 * kv : 0)) * C::RAW;
+                    const uint32_t tile = kv ? sv + vs * C::STG : sk + ks * C::STG;
 #pragma unroll 2
-                    for (int grp = w3; grp < GROUPS; grp += 3) {
-                        const int row = grp * RPG + lrow, key = kb + row;
-                        uint4 f = lds16(raw + row * D + c16 * 16);
+                    for (int grp = w3; grp < PASS / RPG; grp += 3) {
+                        const int hrow = (grp * RPG) % 64 + lrow, row = r0 + grp * RPG + lrow, key = kb + row;
+                        const uint32_t src = raw + grp * RPG / 64 * C::RAW;
+                        uint4 f = lds16(src + hrow * D + c16 * 16);
                         uint16_t d1;
-                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(d1) : "r"(raw + 128 * D + (row * (D / 32) + (c16 >> 1)) * 2) : "memory");
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(d1) : "r"(src + 64 * D + (hrow * (D / 32) + (c16 >> 1)) * 2) : "memory");
                         if (!all && (key > x.t.phi || (key < lo && key >= a.n_sink))) {  // nobody sees it: zeros
                             f = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
                             d1 = 0;
                         }
                         const __half2 d2 = __half2half2(__ushort_as_half(d1));
                         const uint32_t in[4] = {f.x, f.y, f.z, f.w};
-                        uint32_t w[8];
+                        uint32_t w[8], rest[8];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint2 q = tc_bytes_to_f16x4(in[j] ^ 0x80808080u, 0x64806480u);
-                            const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&q.x), d2);
-                            const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&q.y), d2);
-                            w[2 * j] = *reinterpret_cast<const uint32_t*>(&h0);
-                            w[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+                        for (int j = 0; j < 8; ++j) {
+                            const uint2 two = tc_bytes_to_f16x4(in[j >> 1] ^ 0x80808080u, 0x64806480u);
+                            const uint32_t one = j & 1 ? two.y : two.x;
+                            const __half2 z = *reinterpret_cast<const __half2*>(&one), h = __hmul2(z, d2), e = __hfma2(z, d2, __hneg2(h));
+                            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                            rest[j] = *reinterpret_cast<const uint32_t*>(&e);
                         }
+                        if ((d1 & 0x7c00u) == 0x7c00u)  // infinity and NaN have no rest
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) rest[j] = 0u;
                         if (kv && scan) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
-                                if ((w[j] & 0x7c00u) == 0x7c00u) { w[j] &= 0xffff0000u; sm.odd = 1; }
-                                if ((w[j] & 0x7c000000u) == 0x7c000000u) { w[j] &= 0x0000ffffu; sm.odd = 1; }
+                                const uint32_t keep = ((w[j] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) |
+                                                      ((w[j] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
+                                if (keep != 0xffffffffu) sm.odd = 1;
+                                w[j] &= keep;
+                                rest[j] &= keep;
                             }
                         }
                         const uint32_t at = tile + (c16 >> 2) * HALF + row * 128;
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                             at + ((((2 * c16 + j) & 7) ^ (row & 7)) << 4)),
-                                         "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
+                        for (int j = 0; j < 2; ++j) {
+                            const uint32_t to = at + ((((2 * c16 + j) & 7) ^ (row & 7)) << 4);
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[4 * j]), "r"(w[4 * j + 1]),
+                                         "r"(w[4 * j + 2]), "r"(w[4 * j + 3])
                                          : "memory");
+                            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + C::TILE), "r"(rest[4 * j]),
+                                         "r"(rest[4 * j + 1]), "r"(rest[4 * j + 2]), "r"(rest[4 * j + 3])
+                                         : "memory");
+                        }
                     }
-                    fence_async_smem();
+                    if (last) fence_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(kv ? &sm.v_full[vs] : &sm.k_full[ks]);
-                        mbar_arrive(&sm.raw_empty[kv][rs]);
+                        if (last) mbar_arrive(kv ? &sm.v_full[vs] : &sm.k_full[ks]);
+                        if (C::GH == 1 || kv) mbar_arrive(&sm.raw_empty[rs]);
+                    }
+                    if (C::GH == 1 || kv) {
+                        rs ^= 1;
+                        r_ph ^= rs == 0;
+                        if (warp == 9 && ahead > 0) fetch();
                     }
                 }
                 if (!ok) break;
-                if (++rs == RSD) {
-                    rs = 0;
-                    r_ph ^= 1u;
-                }
                 if (++ks == C::KS) {
                     ks = 0;
                     k_ph ^= 1u;
@@ -834,14 +852,11 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     vs = 0;
                     v_ph ^= 1u;
                 }
-                if (warp == 9 && ahead > 0) fetch();
                 if (--left > 0 && ++x.u == x.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
             }
             // a wait has run out somewhere: the copies in flight end before the shared memory goes
             if (warp == 9 && sm.abort != 0)
-                for (int i = max(0, asked - RSD); i <= asked; ++i)
-                    for (int kv = 0; kv < 2 && (i < asked || (k_only && kv == 0)); ++kv)
-                        tc_wait(&sm.raw_full[kv][i % RSD], (uint32_t)(i / RSD) & 1u, a.err);
+                for (int i = max(0, asked - 2); i < asked; ++i) tc_wait(&sm.raw_full[i & 1], (uint32_t)(i >> 1) & 1u, a.err);
         }
     }
     tc_fence_before();
