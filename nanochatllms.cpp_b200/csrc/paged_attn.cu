@@ -22,9 +22,12 @@ static int64_t chunk_ws_bytes(int d) {
 template <int D, int ROWS>
 static cudaError_t launch_join(const PagedAttnArgs& dec, const PagedAttnArgs& chunk, int chunk_ctas, int workers, int rows,
                                cudaStream_t st) {
-    const int n = chunk_ctas * (CH_ROWS / 128) * (D / 32);
-    return launch_pdl(k_paged_join<ROWS, CH_ROWS, D>, dim3(n + (workers + 3) / 4 * rows), dim3(128), 0, st, dec, chunk, n,
-                      workers, rows);
+    const int n = chunk_ctas * (CH_ROWS / 32);
+    const int warps = join_threads(n > 0) / 32;
+    const dim3 grid(n + (workers + warps - 1) / warps * rows), block(32 * warps);
+    if (n == 0) return launch_pdl(k_paged_join<ROWS, 0, D>, grid, block, 0, st, dec, chunk, n, workers, rows);
+    if constexpr (ROWS > 1) return launch_pdl(k_paged_join<ROWS, CH_ROWS, D>, grid, block, 0, st, dec, chunk, n, workers, rows);
+    return cudaErrorInvalidValue;
 }
 
 template <int DT, int D, int ROWS>

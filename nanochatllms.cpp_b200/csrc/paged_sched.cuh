@@ -364,50 +364,69 @@ __device__ __forceinline__ void paged_join_rows(const PagedAttnArgs& a, int w, i
     }
 }
 
-// The same for workers that are CTAs: 128 rows of the item and columns c0 .. c0 + 31, by a CTA of a thread per row.
+__host__ __device__ constexpr int join_threads(bool chunk) { return chunk ? 256 : 128; }
+
+// The same for workers that are CTAs: rows row0 .. row0 + 31 of the item, by a CTA: lane = row, a warp D / 8 columns;
+// through shared memory, so that rows leave whole.
 template <int ROWS, int D>
-__device__ __forceinline__ void paged_join_cols(const PagedAttnArgs& a, int w, int half, int c0) {
-    const int row = half * 128 + threadIdx.x;
+__device__ __forceinline__ void paged_join_cols(const PagedAttnArgs& a, int w, int row0) {
+    constexpr int N = D / 8, L = D / 4;  // columns per thread; lanes that write a row
+    __shared__ float tile[32][D + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = row0 + lane;
     const PagedJoin x = a.join[w];
-    if (x.last < 0 || half * 128 >= x.nrow) return;
+    if (x.last < 0 || row0 >= x.nrow) return;
     const long S = paged_slot<ROWS, D>();
-    const float* part = a.part + 2L * w * S;
+    const float* part = a.part + 2L * w * S + row;
     const int n = x.last - w + 1;
     auto slot = [&](int i) { return part + (i == 0 ? S : 2L * i * S); };
     float m = -INFINITY;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, slot(i)[ROWS * D + row]);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) m = fmaxf(m, slot(i)[ROWS * D]);
     const float mm = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, y[32];
+    float l = 0.0f, y[N];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] = 0.0f;
+    for (int j = 0; j < N; ++j) y[j] = 0.0f;
+#pragma unroll 2
     for (int i = 0; i < n; ++i) {
         const float* ps = slot(i);
-        const float f = ex2(ps[ROWS * D + row] - mm);
-        l = fmaf(ps[ROWS * (D + 1) + row], f, l);
+        const float f = ex2(ps[ROWS * D] - mm);
+        l = fmaf(ps[ROWS * (D + 1)], f, l);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) y[j] = fmaf(ps[(c0 + j) * ROWS + row], f, y[j]);
+        for (int j = 0; j < N; ++j) y[j] = fmaf(ps[(warp * N + j) * ROWS], f, y[j]);
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) y[j] = l != 0.0f ? y[j] * inv : 0.0f;
-    const bool live = row < x.nrow;
-    paged_store<32>(a.out + (live ? paged_row_at(a, x.first, x.h, x.tile, row, ROWS, a.os, row_bytes(a.io, D)) : 0), a.io,
-                    c0, y, live);
+    for (int j = 0; j < N; ++j) tile[lane][warp * N + j] = l != 0.0f ? y[j] * inv : 0.0f;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = warp * 4; i < warp * 4 + 4; i += 32 / L) {
+        const int r = i + lane / L, c0 = lane % L * 4;
+        const bool live = row0 + r < x.nrow;
+        float z[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[j] = tile[r][c0 + j];
+        paged_store<4>(a.out + (live ? paged_row_at(a, x.first, x.h, x.tile, row0 + r, ROWS, a.os, row_bytes(a.io, D)) : 0), a.io,
+                       c0, z, live);
+    }
 }
 
-// What both kernels of a call have left: the first `chunk_ctas` CTAs join the chunk kernel's items, the others the
-// decode kernel's, four workers (of `workers`) and one row (of row_step) each.
+// What both kernels of a call have left: the first `chunk_ctas` CTAs join the chunk kernel's items, 32 rows each, the
+// others the decode kernel's: a warp takes one row (of row_step) of one worker (of `workers`), so that an item's rows,
+// which read the most where a sequence is spread over the whole GPU, fall to different SMs. CROWS = 0: there is no
+// chunk kernel; without its part the code has the registers to keep eight parts in flight (TinyLlama at 1,990 keys:
+// 12.3 us against 13.0).
 template <int ROWS, int CROWS, int D>
-__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs dec, PagedAttnArgs chunk, int chunk_ctas, int workers,
-                                                    int row_step) {
+__global__ void __launch_bounds__(join_threads(CROWS > 0), CROWS > 0 ? 4 : 1) k_paged_join(PagedAttnArgs dec, PagedAttnArgs chunk, int chunk_ctas,
+                                                                int workers, int row_step) {
     pdl_wait();
-    constexpr int PER = CROWS / 128 * (D / 32);  // CTAs of a worker's item
+    constexpr int WARPS = join_threads(CROWS > 0) / 32;
     const int i = blockIdx.x;
-    if (i < chunk_ctas) {
-        paged_join_cols<CROWS, D>(chunk, i / PER, i % (CROWS / 128), i % PER / (CROWS / 128) * 32);
-        return;
-    }
-    const int w = (i - chunk_ctas) / row_step * 4 + (threadIdx.x >> 5);
+    if constexpr (CROWS > 0)
+        if (i < chunk_ctas) {
+            paged_join_cols<CROWS, D>(chunk, i / (CROWS / 32), i % (CROWS / 32) * 32);
+            return;
+        }
+    const int w = (i - chunk_ctas) / row_step * WARPS + (threadIdx.x >> 5);
     if (w < workers) paged_join_rows<ROWS, D>(dec, w, (i - chunk_ctas) % row_step, row_step);
 }
 
