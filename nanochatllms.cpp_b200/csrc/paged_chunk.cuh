@@ -734,30 +734,31 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
             uint32_t k_ph = 1, v_ph = 1, r_ph = 0;
             bool ok = true;
             constexpr int CPR = D / 16, RPG = 32 / CPR, PASS = C::GH == 4 ? 128 : 64;  // PASS: rows converted in a go
-            const int lrow = lane / CPR, c16 = lane % CPR, w3 = warp == 9 ? 2 : warp - 10;
+            const int lrow = lane / CPR, c16 = lane % CPR, g0 = warp == 9 ? 12 : (warp - 10) * 6, g1 = warp == 9 ? 16 : g0 + 6;
             PagedPos y = x;  // warp 9: the unit whose bytes are asked for next
-            int ahead = left, asked = 0;
-            auto fetch = [&]() {  // the next group, from the unit at y
-                // lane: half lane / 8 of the group; of its 8, lanes 0-3 copy a 16-key piece's values, 4-7 its deltas
-                const int half = C::GH == 4 ? (lane >> 3) & 3 : asked & 3, piece = 4 * (half & 1) + (lane & 3);
-                const bool mine = lane < 8 * C::GH, dl = lane & 4;
+            int ahead = left, asked = 0, page = -1, cell = 0;
+            // lane: half lane / 8 of a group; of its 8, lanes 0-3 copy a 16-key piece's values, 4-7 its deltas
+            const bool mine = lane < 8 * C::GH, dl = lane & 4;
+            auto half_of = [&]() { return C::GH == 4 ? (lane >> 3) & 3 : asked & 3; };
+            auto find_page = [&]() {  // of the next group; looked up a group ahead of its use
                 const int lo = a.window > 0 ? max(0, y.t.plo - a.window + 1) : 0;
-                const int k0 = paged_unit_key<CH_KEYS>(y.t, y.u) + 16 * piece;
-                int page = -1;
-                if (mine && k0 <= y.t.phi && (k0 + 15 >= lo || k0 < a.n_sink)) {
-                    page = a.table[y.b * a.table_stride + (k0 >> a.c.ps_shift)];
-                    if ((unsigned)page >= (unsigned)a.c.n_pages) {
-                        page = -1;
-                        atomicOr(a.err, GTN_DEVERR_PAGE);
-                    }
-                }
-                const int slot = asked & 1;
+                const int k0 = paged_unit_key<CH_KEYS>(y.t, y.u) + 64 * (half_of() & 1) + 16 * (lane & 3);
+                page = -1;
+                cell = y.h * a.c.ps + (k0 & (a.c.ps - 1));  // row among the page's
+                if (mine && k0 <= y.t.phi && (k0 + 15 >= lo || k0 < a.n_sink))
+                    page = a.table[y.b * a.table_stride + (k0 >> a.c.ps_shift)] & 0x7fffffff;  // (a bad one stays bad)
+            };
+            auto fetch = [&]() {  // the next group
+                const int slot = asked & 1, half = half_of();
                 if (asked >= 2 && !(ok = wait(&sm.raw_empty[slot], (uint32_t)((asked >> 1) - 1) & 1u))) return;
+                if (page >= a.c.n_pages) {
+                    page = -1;
+                    atomicOr(a.err, GTN_DEVERR_PAGE);
+                }
                 const uint32_t here = __ballot_sync(0xffffffffu, page >= 0) >> (lane & 24) & 0xfu;
                 if (mine && (lane & 7) == 0) mbar_arrive_expect_tx(&sm.raw_full[slot], __popc(here) * 16 * (D + D / 16));
                 __syncwarp();
                 if (page >= 0) {
-                    const int cell = y.h * a.c.ps + (k0 & (a.c.ps - 1));  // row among the page's
                     const long off = (long)page * a.c.page_stride +
                                      (dl ? (long)a.c.kv_heads * a.c.ps * D + cell * (D / 16) : (long)cell * D);
                     ch_bulk(sq + C::RAW0 + (slot * C::GH + (C::GH == 4 ? half : 0)) * C::RAW +
@@ -767,7 +768,9 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 ++asked;
                 if (C::GH == 4 || (asked & 3) == 0)
                     if (--ahead > 0 && ++y.u == y.t.units) paged_next<CH_ROWS, CH_KEYS>(a, p, y);
+                if (ahead > 0) find_page();
             };
+            if (warp == 9 && ahead > 0) find_page();
             if (warp == 9)
                 for (int i = 0; i < 2 && ahead > 0 && ok; ++i) fetch();
             while (left > 0 && ok) {
@@ -784,8 +787,8 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     if (!ok) break;
                     const uint32_t raw = sq + C::RAW0 + (rs * C::GH + (C::GH == 4 ? 2 * kv : 0)) * C::RAW;
                     const uint32_t tile = kv ? sv + vs * C::STG : sk + ks * C::STG;
-#pragma unroll 2
-                    for (int grp = w3; grp < PASS / RPG; grp += 3) {
+#pragma unroll 1
+                    for (int grp = g0; grp < g1; ++grp) {
                         const int hrow = (grp * RPG) % 64 + lrow, row = r0 + grp * RPG + lrow, key = kb + row;
                         const uint32_t src = raw + grp * RPG / 64 * C::RAW;
                         uint4 f = lds16(src + hrow * D + c16 * 16);
