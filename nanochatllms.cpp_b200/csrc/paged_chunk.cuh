@@ -48,10 +48,10 @@ struct ChunkCfg {
     static constexpr int COL_O = 256;  // TMEM columns: S0, S1 at 0 and 128; O0, O1 at 256 and 256 + D
     // Keys per score product. 64: the next unit's scores of a half start as soon as the half's weights are
     // used, so the softmax does not wait for them. But at N = 64 the operands (Q again for every half) come out
-    // of shared memory slower than the product runs, which costs where the products are the bound: at D = 128
-    // one product over both halves (30,000-key chunk: 1144 us against 1284 us with halves; at D = 64 halves win,
-    // window chunks 164 us against 181 us).
-    static constexpr int SN = D == 64 ? 64 : 128;
+    // of shared memory slower than the product runs, which costs where the products or the shared memory are the
+    // bound: one product over both halves at D = 128 (30,000-key chunk: 1144 us against 1284 with halves) and for
+    // Q8 pages (prompts 117 us against 119); halves for fp16 at D = 64 (window chunks 164 us against 181).
+    static constexpr int SN = D == 64 && !Q8 ? 64 : 128;
     // kind::f16, A = B = fp16, D = fp32; scores: both K-major, N = SN; output: B (V) MN-major, N = D
     static constexpr uint32_t IDESC_S = (1u << 4) | (((uint32_t)SN >> 3) << 17) | ((128u >> 4) << 24);
     static constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
