@@ -167,9 +167,13 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)d)) * 1.4426950408889634f;
     a.part = (float*)workspace;
     a.err = device_error_word();
-    // Requests of at most `cut` rows per kv head (tokens x query heads of it) go to the decode kernel, the
-    // others to the chunk kernel. With a bound on the new tokens that says so, only the one is launched; so
-    // is it for a single request, where the other's empty launch would cost more than its choice gives.
+    // Requests of at most `cut` rows per kv head (tokens x query heads of it) go to the decode kernel, whose tiles are
+    // 8 or 16 rows high, the others to the chunk kernel (16 requests of two tokens x 8 heads over 500 to 1,900 keys:
+    // 20.5 us against 26.6). With a bound on the new tokens that says so, only the decode kernel is launched (single
+    // tokens behind a window of 4,096 keys: 58.6 us, 65.5 without the bound). A single request without a bound runs on the
+    // chunk kernel alone: the other's empty launch would cost more than its choice gives (one token of TinyLlama at
+    // 1,990 keys: 12.3 us on the decode kernel, 20.3 on this way). Single rows over a Q8 cache have a kernel
+    // of their own (paged_decode.cuh: 61.5 us against 76.1).
     PagedPick p;
     p.below = true;
     p.chained = false;

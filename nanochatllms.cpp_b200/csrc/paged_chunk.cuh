@@ -2,24 +2,37 @@
 //
 // A worker (paged_sched.cuh) is a CTA, one per SM; an item is 256 query rows (two tiles of 128, the rows of
 // one kv head's query heads packed token by token, so that K and V are read once for all of them), a unit 128
-// keys. S = Q K^T and O += P V run on tcgen05 with S (128 columns per tile), P (fp16, in S's place) and O in
-// TMEM; one thread owns a query row, so that the softmax needs no exchange between threads. The two tiles
-// alternate: while one tile's scores are turned into weights, the tensor cores work for the other.
+// keys, taken in halves of 64. S = Q K^T and O += P V run on tcgen05 with S (128 fp32 columns per tile), P (fp16, in
+// S's place) and O in TMEM; one thread owns a query row, so that the softmax needs no exchange between threads. Four
+// softmaxes are on their way (two tiles, two halves): while one half's scores are turned into weights, the tensor
+// cores work for the others.
 //
 // Roles, which meet only at mbarriers:
 //   warps 0-3, 4-7  softmax of tile 0, 1: read S, running maximum and sum, write P; rescale O when the maximum
 //                   has grown by more than 2^CH_GROW (until then the old one serves, the weights stay below
-//                   2^(CH_BIAS + CH_GROW) < 65504); load Q before an item and write O behind it;
-//   warp 8          issues the MMAs (one thread): P V of unit u, then Q K^T of unit u + 1, tile by tile;
+//                   2^(CH_BIAS + CH_GROW) < 65504); load Q before an item and write O behind it. Weights round to fp16
+//                   once (2^-11 relative), their sum is taken before that, in fp32;
+//   warp 8          issues the MMAs: P V of unit u half by half, behind each the next scores that may go in its place;
 //   warps 9-11      K and V. fp16 cache: warp 9 fetches pages with TMA (128-byte swizzle), warps 10 and 11
-//                   look at the V tiles that not every row sees whole (below). Q8 cache: all three read the
-//                   pages' 8-bit values and write the tiles as fp16, q * delta rounded once (2^-11
-//                   relative, like the weights).
+//                   look at the V tiles that not every row sees whole (below). Q8 cache: warp 9 copies the pages'
+//                   bytes into shared memory, two groups ahead, and all three write the tiles as fp16: an element
+//                   value * delta has up to 18 bits, so it is two fp16 values, the rounded product and the rest, each
+//                   in a tile of its own, and every product runs over both. (Rounded once instead, K and V each add as
+//                   much error as the output's own rounding: 5.2e-4 in all against 2.8e-4, for 106 us against 117.)
 // Keys that a row does not see get weight 0, but 0 times NaN or infinity would reach the row all the same. So
 // in the tiles that not every row sees whole, values that no row sees are zeroed in shared memory, and
 // non-finite ones that some row sees are too, with a flag on which the epilogue adds them, read from the
 // pages again, to the rows that see them.
 // Every wait is bounded as in gemm_tc.cuh.
+//
+// Measured (graph replay, B200): 2,048 tokens over 29,999 keys, 32/8 heads of 128, fp16: 1,100 us, 945 TFLOP/s, 57% of
+// the library product's rate: the exponentials take 66% of their unit, the rest goes where softmax and products wait
+// for each other in turns. Window chunks (D = 64): 126 us, 330 TFLOP/s, bound by the exponentials (half the
+// products per exponential of D = 128). Q8 prompts: 117 us, bound by the conversion of the pages (some 350 cycles per
+// 512 elements and warp, next to two softmax warps per scheduler). A call of a few units per CTA is bound by the
+// code's first run: 7,500 cycles to the first product, 5,500 behind an item.
+// One query row per thread and 384 threads leave 168 registers each; four softmax warpgroups (two threads a row) spilled
+// and were slower, as were more CTAs with smaller tiles.
 #pragma once
 #include "paged_decode.cuh"
 
