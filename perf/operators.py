@@ -250,18 +250,13 @@ def _q8_pages(pool, c):
 
 
 # ---- the framework's calls
-_gten = None
-
-
 def _lib():
-    """The library's module, imported once as a program does."""
-    global _gten
-    if _gten is None:
-        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-        sys.path.insert(0, os.path.join(root, "nanochatllms.cpp_b200"))
-        import gten_b200
-        _gten = gten_b200
-    return _gten
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    pkg = os.path.join(root, "nanochatllms.cpp_b200")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import gten_b200
+    return gten_b200
 
 
 def _handles(s):
