@@ -160,8 +160,10 @@ int64_t gtn_paged_page_bytes(int dtype, int page_size, int kv_heads, int d_head)
  *   n_used [1]                   pages taken from the front of free_pages.
  * Requests are served in order. One is not granted when its lengths are negative, its tokens fit
  * neither the table's row nor the `rows` rows, or when it needs pages and those of the requests up to
- * it exceed n_free; the caller plans it again in a later step. The free list itself is not changed. The
- * tensors written must not overlap each other or those read. */
+ * it exceed n_free; the caller plans it again in a later step. The free list itself is not changed. A page
+ * id of a granted row that no pool can hold (negative, or id * page_size beyond 31 bits) raises GTN_ERR_DEVICE
+ * at the next gtn_check and gives the row slot -1. max_pages * page_size < 2^30. The tensors written must not
+ * overlap each other or those read. */
 int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const gtn_tensor* free_pages,
                    const gtn_tensor* n_free, int page_size, gtn_tensor* block_table, gtn_tensor* q_start,
                    gtn_tensor* kv_lens, gtn_tensor* pos, gtn_tensor* slots, gtn_tensor* n_used, void* stream);

@@ -79,6 +79,7 @@ struct PlanArgs {
     int32_t *table, *q_start, *kv_lens, *pos, *slots, *n_used;
     long table_stride;
     int n, n_cap, max_pages, rows, ps_shift;
+    unsigned int* err;
 };
 
 // Exclusive prefix over the CTA's threads of one value each; *total receives the sum. red: 17 values of
@@ -189,7 +190,9 @@ static __global__ void __launch_bounds__(PLAN_THREADS) k_paged_plan(PlanArgs a) 
             if (o >= 0) {
                 const int have = (c + psm) >> a.ps_shift, col = pos >> a.ps_shift;
                 const int page = col < have ? a.table[lo * a.table_stride + col] : a.free_pages[o + col - have];
-                slot = page < 0 ? -1 : (page << a.ps_shift) + (pos & psm);
+                // an id that no pool can hold has no slot: its cells would not fit 31 bits and come out as another page's
+                if ((unsigned)page <= 0x7fffffffu >> a.ps_shift) slot = (page << a.ps_shift) + (pos & psm);
+                else atomicOr(a.err, GTN_DEVERR_PAGE);
             }
         }
         a.pos[t] = pos;
@@ -470,6 +473,9 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
     GTN_REQUIRE(pos->shape[0] == slots->shape[0], "%s: pos and slots differ in rows", who);
     GTN_REQUIRE(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0, "%s: page_size %d", who,
                 page_size);
+    // (lengths of granted requests then fit 31 bits; paged_attn has the same limit)
+    GTN_REQUIRE((long)block_table->shape[1] * page_size < (1L << 30), "%s: block_table of %d pages a row", who,
+                block_table->shape[1]);
     const gtn_tensor* io[] = {block_table, q_start, kv_lens, pos, slots, n_used, ctx_lens, new_lens, free_pages, n_free};
     PagedSpan span[10];
     for (int i = 0; i < 10; ++i) span[i] = paged_span(io[i]);
@@ -496,6 +502,7 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
     a.max_pages = block_table->shape[1];
     a.rows = pos->shape[0];
     a.ps_shift = __builtin_ctz((unsigned)page_size);
+    a.err = device_error_word();
     return cuda_status(launch_pdl(k_paged_plan, dim3((a.rows + PLAN_ROWS - 1) / PLAN_ROWS), dim3(PLAN_THREADS), 0,
                                   S(stream), a),
                        who);

@@ -1,0 +1,75 @@
+"""Bad page ids and other input of the paged serving operators that must raise, and calls on which a kernel could
+go wrong without a wrong index. Bounds as in test_gpu_paged.py."""
+import pytest
+import torch
+
+import gten_b200 as G
+from paged_ref import F16, gt, i32, ref_plan
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- planner --------------------------------------------------------------------------------------------
+def plan(gpu, ctx, new, free, table, rows, ps):
+    n = len(ctx)
+    t = {"ctx": i32(ctx, gpu), "new": i32(new, gpu), "free": i32(free, gpu), "n_free": i32([len(free)], gpu),
+         "table": i32(table, gpu), "q_start": i32([7] * (n + 1), gpu), "kv": i32([7] * n, gpu), "pos": i32([7] * rows, gpu),
+         "slots": i32([7] * rows, gpu), "used": i32([7], gpu)}
+    G.paged_plan(gt(t["ctx"]), gt(t["new"]), gt(t["free"]), gt(t["n_free"]), ps, gt(t["table"]), gt(t["q_start"]),
+                 gt(t["kv"]), gt(t["pos"]), gt(t["slots"]), gt(t["used"]))
+    return t
+
+
+@pytest.mark.parametrize("ps", [16, 64, 256])
+@pytest.mark.parametrize("where", ["free", "table"])
+@pytest.mark.parametrize("bad", ["first_too_large", "wraps_to_3", "tagged", "minus_one", "lowest", "largest"])
+def test_plan_raises_for_page_ids_that_no_pool_holds(gpu, ps, where, bad):
+    """Slots are page * page_size + offset in 32 bits: an id beyond them must not become another page's slot."""
+    page = {"first_too_large": 2 ** 31 // ps, "wraps_to_3": 2 ** 32 // ps + 3,
+            "tagged": -2 ** 31 + 3, "minus_one": -1, "lowest": -2 ** 31, "largest": 2 ** 31 - 1}[bad]
+    assert page * ps >= 2 ** 31 or page < 0
+    # request 0 goes on in its first page and takes a new one, request 1 is sound
+    ctx, new, table, free = [5, 0], [ps, 3], [[4, -1], [-1, -1]], [6, 8]
+    if where == "free":
+        free[0] = page
+    else:
+        table[0][0] = page
+    G.check()
+    t = plan(gpu, ctx, new, free, table, ps + 4, ps)
+    with pytest.raises(G.GtenError, match="status 5"):
+        G.check()
+    G.check()
+    lost = range(ps - 5, ps) if where == "free" else range(0, ps - 5)  # the rows in the bad page
+    sound = ([1, 8], [[4, -1], [-1, -1]]) if where == "free" else ([6, 8], [[1, -1], [-1, -1]])
+    want = ref_plan(ctx, new, sound[0], 2, ps, sound[1], ps + 4)
+    slots = [-1 if i in lost else s for i, s in enumerate(want[4])]
+    assert t["slots"].tolist() == slots and t["pos"].tolist() == want[3]
+    assert t["kv"].tolist() == want[2] and t["q_start"].tolist() == want[1] and t["used"].item() == 2
+
+
+@pytest.mark.parametrize("ps", [16, 256])
+def test_plan_takes_the_largest_page_id(gpu, ps):
+    page = 2 ** 31 // ps - 1
+    t = plan(gpu, [0], [ps], [page], [[-1]], ps, ps)
+    G.check()
+    assert t["slots"].tolist() == [page * ps + i for i in range(ps)]
+
+
+def test_plan_ignores_bad_ids_that_it_does_not_use(gpu):
+    """Free entries behind those taken, and the pages of requests that are not granted."""
+    t = plan(gpu, [16, 16], [1, 40], [5, -1, 2 ** 30], [[2, -1], [2 ** 31 - 1, -1]], 41, 16)
+    G.check()
+    assert t["slots"].tolist() == [80] + [-1] * 40 and t["kv"].tolist() == [17, 0] and t["used"].item() == 1
+
+
+def test_plan_then_append_leaves_other_pages_alone(gpu):
+    """A wrapped id reaches no cell of another request."""
+    ps, kvh, d = 16, 1, 64
+    t = plan(gpu, [0], [3], [2 ** 28 + 2], [[-1]], 3, ps)
+    pool = torch.zeros(4, ps * kvh * d * 2, dtype=torch.uint8, device=gpu)
+    x = torch.ones(3, d, dtype=torch.float16, device=gpu)
+    cache = G.PagedCache(pool, pool.clone(), F16, 4, ps, kvh, d)
+    G.paged_append(gt(x, F16), gt(x, F16), gt(x, F16), gt(t["pos"]), gt(t["slots"]), cache, gt(torch.empty_like(x), F16))
+    with pytest.raises(G.GtenError, match="status 5"):
+        G.check()
+    assert not bool(pool.any())
