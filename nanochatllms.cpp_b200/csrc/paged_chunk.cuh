@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 page = -1;
                 cell = y.h * a.c.ps + (k0 & (a.c.ps - 1));  // row among the page's
                 if (mine && k0 <= y.t.phi && (k0 + 15 >= lo || k0 < a.n_sink))
-                    page = a.table[y.b * a.table_stride + (k0 >> a.c.ps_shift)] & 0x7fffffff;  // (a bad one stays bad)
+                    page = (int)min((unsigned)a.table[y.b * a.table_stride + (k0 >> a.c.ps_shift)], 0x7fffffffu);  // negative: too large
             };
             auto fetch = [&]() {  // the next group
                 const int slot = asked & 1, half = half_of();

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import gten_b200 as G
-from paged_ref import F16, gt, i32, ref_plan
+from paged_ref import F16, Q8, attn_bound, gt, i32, ref_attn, ref_plan
+from test_gpu_paged import Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +74,27 @@ def test_plan_then_append_leaves_other_pages_alone(gpu):
     with pytest.raises(G.GtenError, match="status 5"):
         G.check()
     assert not bool(pool.any())
+
+
+# ---- attention: table entries ---------------------------------------------------------------------------
+#: every kernel: single rows over Q8, tiles of 8 and of 16 rows, chunks
+KERNELS = [(2, 2, 1, 1), (4, 2, 1, 1), (16, 1, 1, 1), (4, 2, 40, 0), (32, 1, 9, 0)]
+
+
+@pytest.mark.parametrize("cache,d", [(F16, 64), (F16, 128), (Q8, 64), (Q8, 128)])
+@pytest.mark.parametrize("heads,kvh,n,max_new", KERNELS)
+@pytest.mark.parametrize("entry", ["tagged", "minus_one", "n_pages", "largest"])
+def test_bad_table_entries_raise(gpu, cache, d, heads, kvh, n, max_new, entry):
+    """An entry whose low 31 bits name a page is as bad as any: no page of another request is read for it."""
+    b = Batch(gpu, 90, [(200, n), (70, n)], heads, kvh, d, 16, cache, F16)
+    pages = b.k.raw.shape[0]
+    for col in (0, 5):
+        b.table[0][col] = {"tagged": b.table[1][1] - 2 ** 31, "minus_one": -1, "n_pages": pages, "largest": 2 ** 31 - 1}[entry]
+        G.check()
+        b.run(max_new=max_new)
+        with pytest.raises(G.GtenError, match="status 5"):
+            G.check()
+        # the other request is whole
+        got = b.out.view(-1, heads, d).double()[n:2 * n]
+        want, A, S = ref_attn(b.qv[n:2 * n], b.keys[1], b.values[1], 70 - n, d ** -0.5, 0, 0)
+        assert bool(((got - want).abs() <= attn_bound(want, A, S, cache, F16)).all())
