@@ -275,15 +275,13 @@ static __global__ void __launch_bounds__(APP_THREADS, 5) k_paged_append(AppendAr
     uint2 raw[2];
     uint16_t dl[2];
     auto load = [&](int hh) {
-        if (hh < heads) {
-            const uint8_t* src = hh < a.heads         ? a.q + (long)t * a.qs + hh * hb
-                                 : hh < a.heads + kvh ? a.k + (long)t * a.ks + (hh - a.heads) * hb
-                                                      : a.v + (long)t * a.vs + (hh - a.heads - kvh) * hb;
-            app_load8<SDT>(src, 8 * g0, x[0], &raw[0], &dl[0]);
-            app_load8<SDT>(src, 8 * g1, x[1], &raw[1], &dl[1]);
-        }
+        const uint8_t* src = hh < a.heads         ? a.q + (long)t * a.qs + hh * hb
+                             : hh < a.heads + kvh ? a.k + (long)t * a.ks + (hh - a.heads) * hb
+                                                  : a.v + (long)t * a.vs + (hh - a.heads - kvh) * hb;
+        app_load8<SDT>(src, 8 * g0, x[0], &raw[0], &dl[0]);
+        app_load8<SDT>(src, 8 * g1, x[1], &raw[1], &dl[1]);
     };
-    load(tid / TPH);  // on its way while the position and the angles are found
+    if (tid / TPH < heads) load(tid / TPH);  // on its way while the position and the angles are found
     const int pos = a.pos[t], slot = a.slots[t];
     if (pos < 0) return;
     if (tid < a.half) cs[tid] = rope_cs(pos, fr.f[tid]);
@@ -291,11 +289,12 @@ static __global__ void __launch_bounds__(APP_THREADS, 5) k_paged_append(AppendAr
     const bool store = slot >= 0 && page < a.c.n_pages;
     if (slot >= 0 && !store && tid == 0 && a.err) atomicOr(a.err, GTN_DEVERR_PAGE);
     __syncthreads();
-    for (int turn = 0; turn < heads; turn += APP_THREADS / TPH) {  // (the whole CTA takes every turn)
-        const int hh = turn + tid / TPH;
-        if (turn > 0) load(hh);
+    // a head's lanes go the same way, the heads of a warp need not (types, turns): shuffles name the head's lanes alone
+    const unsigned mates = ((1u << TPH) - 1) << (tid & 31 & ~(TPH - 1));
+    for (int hh = tid / TPH; hh < heads; hh += APP_THREADS / TPH) {
+        if (hh >= APP_THREADS / TPH) load(hh);
         const int part = hh < a.heads ? 0 : hh < a.heads + kvh ? 1 : 2, h = hh - (part == 0 ? 0 : part == 1 ? a.heads : a.heads + kvh);
-        const bool live = hh < heads && (part == 0 || store);
+        const bool live = part == 0 || store;
         if (part != 2 && i < hg) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -330,7 +329,7 @@ static __global__ void __launch_bounds__(APP_THREADS, 5) k_paged_append(AppendAr
         for (int b = 0; b < NB; ++b) {
             float m = fmaxf(g0 >> 2 == b ? mx[0] : 0.0f, g1 >> 2 == b ? mx[1] : 0.0f);
 #pragma unroll
-            for (int o = 1; o < TPH; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int o = 1; o < TPH; o <<= 1) m = fmaxf(m, __shfl_xor_sync(mates, m, o));
             if (g0 >> 2 == b) m0 = m;
             if (g1 >> 2 == b) m1 = m;
         }

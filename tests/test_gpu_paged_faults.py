@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import gten_b200 as G
-from paged_ref import F16, Q8, attn_bound, gt, i32, ref_attn, ref_plan
+import test_gpu_paged as tp
+from paged_ref import F16, F32, Q8, attn_bound, gt, i32, ref_attn, ref_plan
 from test_gpu_paged import Batch
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +99,14 @@ def test_bad_table_entries_raise(gpu, cache, d, heads, kvh, n, max_new, entry):
         got = b.out.view(-1, heads, d).double()[n:2 * n]
         want, A, S = ref_attn(b.qv[n:2 * n], b.keys[1], b.values[1], 70 - n, d ** -0.5, 0, 0)
         assert bool(((got - want).abs() <= attn_bound(want, A, S, cache, F16)).all())
+
+
+# ---- append: heads of several types in a warp ----------------------------------------------------------
+@pytest.mark.parametrize("src", [F16, F32, Q8])
+@pytest.mark.parametrize("cache,qdt", [(Q8, F16), (F16, Q8), (Q8, Q8), (F16, F16)])
+@pytest.mark.parametrize("heads,kvh,d,rope_pct", [(36, 36, 64, 1.0), (28, 7, 64, 0.25), (16, 16, 128, 1.0), (20, 3, 128, 0.5),
+                                                  (65, 1, 64, 1.0), (1, 1, 128, 1.0), (33, 33, 128, 0.0)])
+def test_append_with_many_heads(gpu, src, cache, qdt, heads, kvh, d, rope_pct):
+    """Rows of several turns of a CTA, and the border between queries, keys and values inside a warp, where some
+    lanes quantize and others do not."""
+    tp.test_append_matches(gpu, src, cache, qdt, heads, kvh, d, 16, rope_pct, 10000.0, 5000, False)
