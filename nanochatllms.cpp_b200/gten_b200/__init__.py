@@ -147,18 +147,27 @@ def _stream(stream):
     return C.c_void_p(_raw_stream())
 
 
+class _Described:
+    """A class whose ``desc()`` describes its fields to the C library. ``_d`` keeps the descriptor with the object
+    until a field is set; copies and pickles leave it behind."""
+    _ref = None
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_ref", None)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_ref"}
+
+
 @dataclass
-class GT:
+class GT(_Described):
     """A gten tensor view: device buffer + dtype + logical shape (elements), contiguous rows unless
     ``strides`` (elements, one per dim) says otherwise."""
     buf: object
     dtype: int
     shape: tuple
     strides: tuple | None = None
-
-    def __setattr__(self, name, value):
-        object.__setattr__(self, name, value)
-        object.__setattr__(self, "_ref", None)  # a kept descriptor does not outlive a field
 
     def desc(self) -> gtn_tensor:
         t = gtn_tensor()
@@ -176,14 +185,27 @@ class GT:
         return t
 
 
+def _place(t):
+    """What a kept descriptor of a GT or PagedCache depends on besides its fields: the buffers' addresses. None: its
+    descriptor is not kept (another class, or fields that can change in place)."""
+    if type(t) is GT:
+        if isinstance(t.shape, tuple) and (t.strides is None or isinstance(t.strides, tuple)):
+            return _ptr(t.buf)
+    elif type(t) is PagedCache:
+        return _ptr(t.k), _ptr(t.v)
+    return None
+
+
 def _d(t):
-    """The descriptor by reference: kept with a GT, and made anew when the buffer's address has changed."""
+    """The descriptor by reference: kept with the object, and made anew when a field or a buffer's address has changed."""
     if t is None:
         return None
+    at = _place(t)
+    if at is None:
+        return C.byref(t.desc())
     r = t._ref
-    if r is None or r[1] != _ptr(t.buf):
-        c = t.desc()
-        r = (C.byref(c), c.data)
+    if r is None or r[1] != at:
+        r = (C.byref(t.desc()), at)
         object.__setattr__(t, "_ref", r)
     return r[0]
 
@@ -243,15 +265,18 @@ def token_embed(weight: GT, tokens: GT, out: GT, start_pos: int = 0, stream=None
 
 
 # ---- paged serving operators ----------------------------------------------------------------
-class PagedCache:
+@dataclass(eq=False)
+class PagedCache(_Described):
     """A paged K/V cache: two pools of ``n_pages`` pages of ``page_size`` tokens (gtn_paged_cache has the
     page layout; ``page_bytes`` the bytes of one page). k, v: device buffers (torch tensors or pointers)."""
-
-    def __init__(self, k, v, dtype: int, n_pages: int, page_size: int, kv_heads: int, d_head: int, page_stride: int = 0):
-        self.k, self.v = k, v  # keeps the buffers alive
-        self.d_head, self.kv_heads = d_head, kv_heads
-        self._desc = gtn_paged_cache(_ptr(k), _ptr(v), dtype, n_pages, page_size, kv_heads, d_head, page_stride)
-        self._by_ref = C.byref(self._desc)
+    k: object
+    v: object
+    dtype: int
+    n_pages: int
+    page_size: int
+    kv_heads: int
+    d_head: int
+    page_stride: int = 0
 
     @staticmethod
     def page_bytes(dtype: int, page_size: int, kv_heads: int, d_head: int) -> int:
@@ -261,7 +286,8 @@ class PagedCache:
         return n
 
     def desc(self) -> gtn_paged_cache:
-        return self._desc
+        return gtn_paged_cache(_ptr(self.k), _ptr(self.v), self.dtype, self.n_pages, self.page_size, self.kv_heads,
+                               self.d_head, self.page_stride)
 
 
 def paged_plan(ctx_lens: GT, new_lens: GT, free_pages: GT, n_free: GT, page_size: int, block_table: GT, q_start: GT,
@@ -275,7 +301,7 @@ def paged_plan(ctx_lens: GT, new_lens: GT, free_pages: GT, n_free: GT, page_size
 def paged_append(q: GT, k: GT, v: GT, pos: GT, slots: GT, cache: PagedCache, q_out: GT, rope_pct: float = 1.0,
                  rope_base: float = 10000.0, stream=None):
     """Rotary at each row's own position, K and V rows into their pages, rotated queries to q_out."""
-    _check(lib().gtn_paged_append(_d(q), _d(k), _d(v), _d(pos), _d(slots), cache._by_ref, _d(q_out), rope_pct, rope_base,
+    _check(lib().gtn_paged_append(_d(q), _d(k), _d(v), _d(pos), _d(slots), _d(cache), _d(q_out), rope_pct, rope_base,
                                   _stream(stream)), "paged_append")
 
 
@@ -307,7 +333,7 @@ def paged_attn(q: GT, cache: PagedCache, block_table: GT, q_start: GT, kv_lens: 
     one, a tensor is taken from torch's allocator for this call, on the call's stream."""
     if workspace is None:
         workspace = _scratch(q.shape[-1] // cache.d_head, cache.d_head, stream)
-    _check(lib().gtn_paged_attn(_d(q), cache._by_ref, _d(block_table), _d(q_start), _d(kv_lens), _d(out), scale, window,
+    _check(lib().gtn_paged_attn(_d(q), _d(cache), _d(block_table), _d(q_start), _d(kv_lens), _d(out), scale, window,
                                 n_sink, max_new, _ptr(workspace), workspace.numel(), _stream(stream)), "paged_attn")
 
 
