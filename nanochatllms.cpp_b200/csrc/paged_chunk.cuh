@@ -21,8 +21,8 @@
 //                   much error as the output's own rounding: 5.2e-4 in all against 2.8e-4, for 106 us against 117.)
 // Keys that a row does not see get weight 0, but 0 times NaN or infinity would reach the row all the same. So
 // in the tiles that not every row sees whole, values that no row sees are zeroed in shared memory, and
-// non-finite ones that some row sees are too, with a flag on which the epilogue adds them, read from the
-// pages again, to the rows that see them.
+// non-finite ones that some row sees are too, with a note of the item on which its epilogue adds them, read from the
+// pages again, to the rows that see them (some milliseconds at most, far below the waits' bound).
 // Every wait is bounded as in gemm_tc.cuh.
 //
 // Measured (graph replay, B200): 2,048 tokens over 29,999 keys, 32/8 heads of 128, fp16: 1,100 us, 945 TFLOP/s, 57% of
@@ -188,15 +188,24 @@ struct ChunkSmem {
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain;  // s, p: per tile and 64-key half
     uint32_t tmem;
     volatile int abort;
-    volatile int odd;  // a non-finite value was set aside (stays set)
+    unsigned odd;  // 1 + the start (on the line) of the last item of which a non-finite value was set aside; 0: none
     unsigned pre[CH_THREADS], wsum[CH_THREADS / 32];
 };
 
-// Adds the values that were set aside (non-finite) to a row's columns c0 .. c0 + 15, as far as it sees them.
+// Keys [kb, kb + nk) that every row of the positions plo .. phi sees.
+__device__ __forceinline__ bool ch_whole(const PagedAttnArgs& a, int kb, int nk, int plo, int phi) {
+    const int lo = a.window > 0 ? max(0, phi - a.window + 1) : 0;
+    return kb + nk - 1 <= plo && (kb >= lo || kb + nk <= a.n_sink);
+}
+
+// Adds the values that were set aside (non-finite) to a row's columns c0 .. c0 + 15, as far as it sees them: those of
+// the units that not every row sees whole, at most some 256 + 2 * 128 keys at each end of the window and the first
+// tokens' last unit, however long the item is.
 static __device__ __noinline__ void ch_add_odd(const PagedAttnArgs& a, const PagedPos& x, int u0, int u1, int pos, int wlo,
                                                int c0, float (&v)[16]) {
     for (int u = u0; u < u1; ++u) {
         const int kb = paged_unit_key<CH_KEYS>(x.t, u);
+        if (ch_whole(a, kb, CH_KEYS, x.t.plo, x.t.phi)) continue;  // (nothing of it was set aside)
         for (int key = kb; key < kb + CH_KEYS && key <= pos; ++key) {
             if (key < wlo && key >= a.n_sink) continue;
             const int page = a.table[x.b * a.table_stride + (key >> a.c.ps_shift)];
@@ -335,12 +344,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
         }
         return true;
     };
-    // keys [kb, kb + nk) that every row of the positions plo .. phi sees
-    auto whole_for = [&](int kb, int nk, int plo, int phi) {
-        const int lo = a.window > 0 ? max(0, phi - a.window + 1) : 0;
-        return kb + nk - 1 <= plo && (kb >= lo || kb + nk <= a.n_sink);
-    };
-    auto seen_whole = [&](int kb) { return whole_for(kb, CH_KEYS, x.t.plo, x.t.phi); };
+    auto seen_whole = [&](int kb) { return ch_whole(a, kb, CH_KEYS, x.t.plo, x.t.phi); };
     auto next_item = [&](int done) {
         left -= done;
         if (left > 0) paged_next<CH_ROWS, CH_KEYS>(a, p, x);
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 uint32_t v[2][32];
                 ch_ld32(tb, v[0]);
                 ch_ld32(tb + 32, v[1]);
-                const bool whole = whole_for(kb, 64, tlo, thi);
+                const bool whole = ch_whole(a, kb, 64, tlo, thi);
                 // the keys of chunk i (32) that this row sees, as bits
                 auto seen_bits = [&](int i) -> uint32_t {
                     const int k0 = kb + 32 * i;
@@ -512,7 +516,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                 const int prow = r * 128 + row;
                 float* ps = a.part + (2L * me + (u0 == 0)) * paged_slot<CH_ROWS, D>();
                 const uint32_t stage = sq + C::OUT + warp * C::STAGE;
-                const bool odd = n > 0 && sm.odd != 0;
+                const bool odd = n > 0 && sm.odd > was.start;  // of this item, or of one that the copies are ahead at
                 if (done && a.io != GTN_F16) {
                     ch_q8_rows<D>(a, was, prow, live, n > 0, odd, to, inv, u0, u1, pos, wlo);
                 } else {
@@ -726,7 +730,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                                 asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]),
                                              "r"(w[2]), "r"(w[3])
                                              : "memory");
-                            if (bad) sm.odd = 1;
+                            if (bad) atomicMax(&sm.odd, x.start + 1);
                         }
                         fence_async_smem();
                     }
@@ -830,7 +834,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                             for (int j = 0; j < 8; ++j) {
                                 const uint32_t keep = ((w[j] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) |
                                                       ((w[j] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
-                                if (keep != 0xffffffffu) sm.odd = 1;
+                                if (keep != 0xffffffffu) atomicMax(&sm.odd, x.start + 1);
                                 w[j] &= keep;
                                 rest[j] &= keep;
                             }

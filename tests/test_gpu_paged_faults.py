@@ -6,6 +6,7 @@ import torch
 import gten_b200 as G
 import test_gpu_paged as tp
 from paged_ref import F16, F32, Q8, attn_bound, gt, i32, ref_attn, ref_plan
+from paged_long import LongBatch
 from test_gpu_paged import Batch
 
 pytestmark = pytest.mark.gpu
@@ -110,3 +111,39 @@ def test_append_with_many_heads(gpu, src, cache, qdt, heads, kvh, d, rope_pct):
     """Rows of several turns of a CTA, and the border between queries, keys and values inside a warp, where some
     lanes quantize and others do not."""
     tp.test_append_matches(gpu, src, cache, qdt, heads, kvh, d, 16, rope_pct, 10000.0, 5000, False)
+
+
+# ---- attention: values that are not finite, in long chunks --------------------------------------------
+@pytest.mark.parametrize("d,heads,kvh", [(128, 32, 8), (64, 8, 8)])
+@pytest.mark.parametrize("window,n_sink", [(0, 0), (9000, 5)])
+def test_infinity_at_the_end_of_a_long_chunk(gpu, d, heads, kvh, window, n_sink):
+    """An infinity that only the last token sees, in calls whose workers take many items: its row gets it, the others
+    and other requests' are right, and looking for it costs milliseconds, not a walk over every key per item."""
+    lens = [(30000, 1024), (700, 700), (29000, 300)]
+    b = LongBatch(gpu, 91, lens, heads, kvh, d, 64, F16)
+    kw = dict(window=window, n_sink=n_sink)
+    keys, values = ([b.cells(p, i) for i in range(3)] for p in (b.k, b.v))
+
+    def timed():
+        G.check()
+        e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        e[0].record()
+        b.run(**kw)
+        e[1].record()
+        G.check()
+        return e[0].elapsed_time(e[1])
+
+    clean = min(timed() for _ in range(3))
+    b.set_row(b.v, 0, 29999, float("inf"))
+    spoilt = timed()
+    for r, i in [(0, 0), (0, 511), (0, 1022), (1, 0), (1, 300), (1, 699), (2, 0), (2, 299)]:
+        want, A, S = b.want(r, i, keys[r], values[r], **kw)
+        assert bool(((b.row(r, i) - want[0]).abs() <= long_bound(want, A, S)[0]).all()), (r, i)
+    assert bool((b.row(0, 1023) == float("inf")).all())
+    assert spoilt < clean + 20.0, (clean, spoilt)
+
+
+def long_bound(want, A, S):
+    """attn_bound for up to 30,000 keys: fp32 sums of n terms are off by at most n 2^-24 of the sum of magnitudes, here
+    2^-9; the workers' shares of a few thousand keys at a time stay far below it."""
+    return attn_bound(want, A, S, F16, F16) + A * 2.0 ** -9
