@@ -121,10 +121,14 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     GTN_REQUIRE(rows <= (1 << 20) && (rows * group + CH_ROWS) * group < (1L << 32) && rows * heads < (1L << 31),
                 "%s: %ld rows of %d heads", who, rows, heads);
     GTN_REQUIRE(cap < (1L << 30), "%s: block_table of %d pages a row", who, block_table->shape[1]);
-    const bool small = max_new > 0 && max_new * group <= 16;
-    const long few = small ? rows * group : 0;  // tiles of the decode kernel beyond one a request
-    const long few_units = (few + n) * (cap / 16 + 2) * a.c.kv_heads;
-    const long many_units = (rows * group / CH_ROWS + n) * (cap / CH_KEYS + 2) * a.c.kv_heads;
+    // With a bound on the new tokens that a decode tile holds, the decode kernel takes every request, in tiles as high as
+    // the bound: rows / height tiles and one more a request, unless a call could then have more units than 32 bits count.
+    const long most = max_new > 0 ? max_new * group : 0x7fffffffL, per_tile = (cap / 16 + 2) * a.c.kv_heads;
+    const int height = most == 1 && a.c.dt == GTN_Q8 ? 1 : most <= 8 ? 8 : 16;
+    const long all_units = (rows * group / height + (height > 1 ? n : 0)) * per_tile;
+    const bool small = most <= 16 && all_units < 0x7fffffffL;
+    const long few_units = small ? all_units : n * per_tile;  // else one tile a request
+    const long many_units = small ? 0 : (rows * group / CH_ROWS + n) * (cap / CH_KEYS + 2) * a.c.kv_heads;
     GTN_REQUIRE(few_units < 0x7fffffffL && many_units < 0x7fffffffL,
                 "%s: %ld rows of %d requests over tables of %ld keys are too many for one call", who, rows, n, cap);
     const gtn_tensor* rt[] = {q, out};
@@ -178,15 +182,14 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     p.below = true;
     p.chained = false;
     p.cut = a.group <= 8 ? 8 : a.group <= 16 ? 16 : 0;
-    const long most = max_new > 0 ? (long)max_new * a.group : 0x7fffffffL;
     cudaError_t e = cudaSuccess;
     if (small) {
         p.cut = 0x7fffffff;
-        if (most == 1 && a.c.dt == GTN_Q8)
+        if (height == 1)
             e = d == 64 ? launch_decode<GTN_Q8, 64, 1>(a, p, 1, a, 0, S(stream))
                         : launch_decode<GTN_Q8, 128, 1>(a, p, 1, a, 0, S(stream));
         else
-            e = most <= 8 ? decode<8>(a, p, (int)most, a, 0, S(stream)) : decode<16>(a, p, (int)most, a, 0, S(stream));
+            e = height == 8 ? decode<8>(a, p, (int)most, a, 0, S(stream)) : decode<16>(a, p, (int)most, a, 0, S(stream));
     } else {
         PagedAttnArgs c = a;
         c.most = (unsigned)many_units;

@@ -147,3 +147,21 @@ def long_bound(want, A, S):
     """attn_bound for up to 30,000 keys: fp32 sums of n terms are off by at most n 2^-24 of the sum of magnitudes, here
     2^-9; the workers' shares of a few thousand keys at a time stay far below it."""
     return attn_bound(want, A, S, F16, F16) + A * 2.0 ** -9
+
+
+# ---- attention: bounds on the new tokens over wide tables ---------------------------------------------
+@pytest.mark.parametrize("heads,kvh,cache,pad", [(64, 8, F16, 0), (36, 36, Q8, 3072)])
+def test_decode_steps_over_wide_tables(gpu, heads, kvh, cache, pad):
+    """Single tokens of 1,024 requests whose tables have room for 2^19 keys: the bound on the new tokens chooses the
+    kernels, not whether the call is taken."""
+    n = 1024
+    b = Batch(gpu, 92, [(1 + i % 2, 1) for i in range(n)], heads, kvh, 64, 16, cache, F16, pad=pad)
+    table = torch.full((n, 1 << 15), -1, dtype=torch.int32, device=gpu)
+    table[:, :b.mp] = i32(b.table, gpu)
+    q, cache_, _, q_start, kv_lens, out = b.tensors()
+    outs = []
+    for max_new in (1, 0):
+        b.out.fill_(3.0)
+        G.paged_attn(q, cache_, gt(table), q_start, kv_lens, out, max_new=max_new)
+        G.check()
+        b.compare()

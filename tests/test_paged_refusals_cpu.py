@@ -6,7 +6,7 @@ import pytest
 import gten_b200 as G
 
 MB = 1 << 20
-AT = [(64 + 64 * i) * MB for i in range(16)]  # buffers that lie apart
+AT = [(i + 1) << 40 for i in range(16)]  # buffers that lie apart
 
 
 def t(at, *shape, dtype=G.I32, strides=None):
@@ -43,9 +43,52 @@ def test_plan_base_call_passes_the_checks():
 @pytest.mark.parametrize("page_size,max_pages", [(16, 1 << 26), (256, 1 << 22), (16, 2 ** 31 - 1), (64, 1 << 25)])
 def test_plan_refuses_tables_of_2_30_keys(page_size, max_pages):
     """Lengths that such a row could hold would not fit 32 bits beside the new tokens."""
-    msg = refusal(G.paged_plan, plan_args(page_size=page_size, block_table=t(1 << 40, 3, max_pages)))
+    msg = refusal(G.paged_plan, plan_args(page_size=page_size, block_table=t(AT[4], 3, max_pages)))
     assert "status 1" in msg and "block_table of" in msg
 
 
 def test_plan_takes_tables_just_below_2_30_keys():
-    assert passed(refusal(G.paged_plan, plan_args(block_table=t(1 << 40, 3, (1 << 26) - 1))))
+    assert passed(refusal(G.paged_plan, plan_args(block_table=t(AT[4], 3, (1 << 26) - 1))))
+
+
+def attn_args(n=3, rows=5, heads=4, max_pages=4, page_size=16, kvh=2, dtype=G.F16, **kw):
+    a = dict(q=t(AT[0], rows, heads * 64, dtype=G.F16), cache=G.PagedCache(AT[1], AT[2], dtype, 8, page_size, kvh, 64),
+             block_table=t(AT[3], n, max_pages), q_start=t(AT[4], n + 1), kv_lens=t(AT[5], n),
+             out=t(AT[6], rows, heads * 64, dtype=G.F16), workspace=Ws(AT[8], 64 * MB), stream=0)
+    a.update(kw)
+    return a
+
+
+class Ws:
+    def __init__(self, at, n):
+        self.at, self.n = at, n
+
+    def data_ptr(self):
+        return self.at
+
+    def numel(self):
+        return self.n
+
+
+def test_attn_base_call_passes_the_checks():
+    assert passed(refusal(G.paged_attn, attn_args()))
+
+
+#: calls whose tiles of 16 rows fit 32 bits of units and whose single rows do not
+WIDE = [dict(n=1024, rows=1024, heads=64, kvh=8, max_pages=1 << 15),               # 8 query heads per kv head, 2^19 keys
+        dict(n=1024, rows=1024, heads=128, kvh=8, max_pages=1 << 15),
+        dict(n=1024, rows=4096, heads=36, kvh=36, max_pages=1 << 15, dtype=G.Q8),  # many more rows than requests
+        dict(n=2, rows=1 << 20, heads=16, kvh=16, max_pages=1 << 13)]
+
+
+@pytest.mark.parametrize("wide", WIDE, ids=str)
+@pytest.mark.parametrize("max_new", [0, 1, 2, 8, 16, 17, 2 ** 31 - 1])
+def test_attn_takes_with_a_bound_what_it_takes_without(wide, max_new):
+    """max_new chooses the kernels, not whether a call is taken."""
+    assert passed(refusal(G.paged_attn, attn_args(max_new=max_new, **wide)))
+
+
+@pytest.mark.parametrize("max_new", [0, 1, 5])
+def test_attn_refuses_units_beyond_32_bits(max_new):
+    msg = refusal(G.paged_attn, attn_args(n=4096, rows=4096, heads=8, kvh=8, max_pages=1 << 16, max_new=max_new))
+    assert "status 1" in msg and "too many for one call" in msg
