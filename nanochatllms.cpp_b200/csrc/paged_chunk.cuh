@@ -804,6 +804,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                     if (!ok) break;
                     const uint32_t raw = sq + C::RAW0 + (rs * C::GH + (C::GH == 4 ? 2 * kv : 0)) * C::RAW;
                     const uint32_t tile = kv ? sv + vs * C::STG : sk + ks * C::STG;
+                    bool bad = false;
 #pragma unroll 1
                     for (int grp = g0; grp < g1; ++grp) {
                         const int hrow = (grp * RPG) % 64 + lrow, row = r0 + grp * RPG + lrow, key = kb + row;
@@ -834,7 +835,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                             for (int j = 0; j < 8; ++j) {
                                 const uint32_t keep = ((w[j] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) |
                                                       ((w[j] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
-                                if (keep != 0xffffffffu) atomicMax(&sm.odd, x.start + 1);
+                                bad |= keep != 0xffffffffu;
                                 w[j] &= keep;
                                 rest[j] &= keep;
                             }
@@ -851,6 +852,7 @@ __global__ void __launch_bounds__(CH_THREADS, 1)
                                          : "memory");
                         }
                     }
+                    if (bad) atomicMax(&sm.odd, x.start + 1);
                     if (last) fence_async_smem();
                     __syncwarp();
                     if (lane == 0) {
