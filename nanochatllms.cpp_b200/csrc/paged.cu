@@ -562,7 +562,7 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
     a.half = rd / 2;
     a.err = device_error_word();
     RopeFreq fr;
-    for (int j = 0; j < 64; ++j) fr.f[j] = j < a.half ? std::pow((double)rope_base, -2.0 * j / (2 * a.half)) : 0.0;
+    for (int j = 0; j < 64; ++j) fr.f[j] = j < a.half ? std::pow((double)rope_base, -2.0 * j / rd) : 0.0;  // (rd may be odd)
     bool aligned = a.half % 8 == 0;
     for (const gtn_tensor* t : rt)
         aligned = aligned && (t->dtype == GTN_Q8 || ((uintptr_t)t->data % 16 == 0 && bstride(t, 0) % 16 == 0));

@@ -165,3 +165,28 @@ def test_decode_steps_over_wide_tables(gpu, heads, kvh, cache, pad):
         G.paged_attn(q, cache_, gt(table), q_start, kv_lens, out, max_new=max_new)
         G.check()
         b.compare()
+
+
+# ---- append and gtn_rotary_emb --------------------------------------------------------------------------
+@pytest.mark.parametrize("d,rope_pct", [(64, 1.0), (64, 0.25), (64, 0.8), (64, 0.05), (128, 0.7), (128, 0.3), (128, 0.0),
+                                        (64, 0.02)])
+def test_append_rotates_as_rotary_emb(gpu, d, rope_pct):
+    """The same rows at positions 0, 1, ... through both operators, rotated widths that are odd among them (0.8 of 64 is
+    51: pairs 25 apart, exponents -2j / 51). rotary_emb forms its angle in fp32: the exponent 2j / rd is off by 2^-24 of
+    itself and the power by some 2^-23, which ln(10000) < 10 and the position multiply; both cosines are then right to
+    p * 12 * 2^-23 + 2^-22."""
+    rows, heads, kvh = 40, 3, 1
+    gen = torch.Generator(device=gpu).manual_seed(d)
+    x = torch.randn(rows, heads * d, generator=gen, device=gpu)
+    kv = torch.zeros(rows, kvh * d, device=gpu)
+    pool = torch.zeros(3, 16 * kvh * d * 2, dtype=torch.uint8, device=gpu)
+    cache = G.PagedCache(pool, pool.clone(), F16, 3, 16, kvh, d)
+    out, want = torch.empty(rows, heads * d, dtype=torch.float16, device=gpu), torch.empty_like(x)
+    G.rotary_emb(gt(x, F32), gt(want, F32), d, rope_pct)
+    G.paged_append(gt(x, F32), gt(kv, F32), gt(kv, F32), gt(i32(range(rows), gpu)), gt(i32(range(rows), gpu)), cache, gt(out, F16),
+                   rope_pct)
+    G.check()
+    p = torch.arange(rows, device=gpu, dtype=torch.float64)[:, None]
+    mag = x.double().view(rows, heads, d).abs().amax(-1, keepdim=True).expand(-1, -1, d).reshape(rows, -1)
+    err = 2 * mag * (p * 12 * 2.0 ** -23 + 2.0 ** -22)
+    assert bool(((out.double() - want.double()).abs() <= err + (want.double().abs() + err) * 2.0 ** -11 + 2.0 ** -25).all())
