@@ -33,6 +33,7 @@ int paged_cache_args(const gtn_paged_cache* c, const char* who, PagedCache* out)
 int paged_int_arg(const gtn_tensor* t, int ndim, const char* who, const char* name) {
     GTN_CHECK(check_tensor(t, name));
     GTN_REQUIRE(t->dtype == GTN_I32 && t->ndim == ndim, "%s: %s must be int32, %d-D", who, name, ndim);
+    GTN_REQUIRE((uintptr_t)t->data % 4 == 0, "%s: %s must be 4-byte aligned", who, name);
     GTN_REQUIRE(t->shape[ndim - 1] == 1 || t->strides[ndim - 1] == 1, "%s: %s must be contiguous", who, name);
     GTN_REQUIRE(ndim == 1 || t->strides[0] >= t->shape[1], "%s: %s rows overlap", who, name);
     return GTN_OK;

@@ -92,3 +92,30 @@ def test_attn_takes_with_a_bound_what_it_takes_without(wide, max_new):
 def test_attn_refuses_units_beyond_32_bits(max_new):
     msg = refusal(G.paged_attn, attn_args(n=4096, rows=4096, heads=8, kvh=8, max_pages=1 << 16, max_new=max_new))
     assert "status 1" in msg and "too many for one call" in msg
+
+
+def append_args(**kw):
+    a = dict(q=t(AT[0], 5, 256, dtype=G.F16), k=t(AT[1], 5, 128, dtype=G.F16), v=t(AT[2], 5, 128, dtype=G.F16), pos=t(AT[3], 5),
+             slots=t(AT[4], 5), cache=G.PagedCache(AT[5], AT[6], G.F16, 8, 16, 2, 64), q_out=t(AT[7], 5, 256, dtype=G.F16), stream=0)
+    a.update(kw)
+    return a
+
+
+def test_append_base_call_passes_the_checks():
+    assert passed(refusal(G.paged_append, append_args()))
+
+
+INTS = [(G.paged_plan, plan_args, n) for n in ("ctx_lens", "new_lens", "free_pages", "n_free", "block_table", "q_start", "kv_lens",
+                                               "pos", "slots", "n_used")]
+INTS += [(G.paged_append, append_args, n) for n in ("pos", "slots")]
+INTS += [(G.paged_attn, attn_args, n) for n in ("block_table", "q_start", "kv_lens")]
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("call,args,name", INTS, ids=lambda x: x if isinstance(x, str) else "")
+def test_int_tensors_are_aligned(call, args, name, off):
+    """A 4-byte load from another address faults."""
+    a = args()
+    a[name].buf += off
+    msg = refusal(call, a)
+    assert "status 1" in msg and f"{name} must be 4-byte aligned" in msg
