@@ -53,9 +53,23 @@ int paged_on_device(const void* const* p, int n, const char* who) {
 
 PagedSpan paged_span(const gtn_tensor* t) {
     const uint8_t* p = (const uint8_t*)t->data;
-    const int last = t->ndim - 1;
-    const long rows = t->ndim > 1 ? (long)(t->shape[0] - 1) * bstride(t, 0) : 0;
-    return {p, p + rows + row_bytes(t->dtype, t->shape[last])};
+    const long width = row_bytes(t->dtype, t->shape[t->ndim - 1]);
+    const long rows = t->ndim > 1 ? t->shape[0] : 1, stride = rows > 1 ? bstride(t, 0) : 0;
+    return {p, p + (rows - 1) * stride + width, width, stride};
+}
+
+PagedSpan paged_pool_span(const PagedCache& c, const uint8_t* pool) {
+    const long width = paged_page_bytes(c.dt, c.ps, c.kv_heads, c.d);
+    return {pool, pool + (c.n_pages - 1) * c.page_stride + width, width, c.n_pages > 1 ? c.page_stride : 0};
+}
+
+bool paged_meet(const PagedSpan& x, const PagedSpan& y) {
+    if (x.data >= y.end || y.data >= x.end) return false;
+    const long stride = x.stride ? x.stride : y.stride;
+    if (stride == 0 || (y.stride && y.stride != stride)) return true;
+    long off = (y.data - x.data) % stride;  // of y's columns behind x's
+    if (off < 0) off += stride;
+    return off < x.width || off + y.width > stride;
 }
 
 int paged_apart(const gtn_tensor* q, const gtn_tensor* out, const char* who, const char* name) {
@@ -537,11 +551,15 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
         GTN_REQUIRE((uintptr_t)t->data % (t->dtype == GTN_F32 ? 4 : 2) == 0, "%s: row alignment", who);
     }
     GTN_CHECK(paged_apart(q, q_out, who, "q_out"));
-    if (q->data != q_out->data) {
-        GTN_CHECK(paged_apart(k, q_out, who, "q_out"));
-        GTN_CHECK(paged_apart(v, q_out, who, "q_out"));
-        GTN_REQUIRE(k->data != q_out->data && v->data != q_out->data, "%s: q_out is k or v", who);
-    }
+    // what is written lies apart from what is read: k and v too where q_out is q's own memory (as column ranges beside it)
+    const PagedSpan qo = paged_span(q_out), kp = paged_pool_span(a.c, a.c.k), vp = paged_pool_span(a.c, a.c.v);
+    GTN_REQUIRE(!paged_meet(paged_span(k), qo) && !paged_meet(paged_span(v), qo), "%s: q_out overlaps k or v", who);
+    GTN_REQUIRE(!paged_meet(kp, vp), "%s: the pools of the cache overlap", who);
+    GTN_REQUIRE(!paged_meet(qo, kp) && !paged_meet(qo, vp), "%s: q_out overlaps the cache", who);
+    const gtn_tensor* in[] = {q, k, v, pos, slots};
+    for (const gtn_tensor* t : in)
+        GTN_REQUIRE(!paged_meet(paged_span(t), kp) && !paged_meet(paged_span(t), vp), "%s: the cache overlaps an input", who);
+    GTN_REQUIRE(!paged_meet(paged_span(pos), qo) && !paged_meet(paged_span(slots), qo), "%s: q_out overlaps pos or slots", who);
     GTN_REQUIRE(rope_pct >= 0.0f && rope_pct <= 1.0f, "%s: rope_pct", who);
     GTN_REQUIRE(rope_base > 0.0f && std::isfinite(rope_base), "%s: rope_base", who);
     const void* ptrs[] = {q->data, k->data, v->data, q_out->data, pos->data, slots->data, a.c.k, a.c.v};

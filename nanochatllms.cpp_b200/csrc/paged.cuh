@@ -41,12 +41,17 @@ int paged_int_arg(const gtn_tensor* t, int ndim, const char* who, const char* na
 // Every pointer lies in memory that the current device owns (or managed memory). Turns a host pointer or
 // another device's tensor into an error before a kernel meets it.
 int paged_on_device(const void* const* p, int n, const char* who);
-// The bytes [data, end) that a tensor's rows span, and whether two tensors' spans meet.
+// The rows of a tensor (or the pages of a pool): `width` bytes every `stride` bytes (0: one row), in [data, end).
 struct PagedSpan {
     const uint8_t *data, *end;
+    long width, stride;
 };
 PagedSpan paged_span(const gtn_tensor* t);
-inline bool paged_meet(const PagedSpan& x, const PagedSpan& y) { return x.data < y.end && y.data < x.end; }
+PagedSpan paged_pool_span(const PagedCache& c, const uint8_t* pool);
+inline PagedSpan paged_bytes_span(const void* p, long n) { return {(const uint8_t*)p, (const uint8_t*)p + n, n, 0}; }
+// Whether two of them may share bytes. Exact for rows of one stride (column ranges of one buffer); rows of different
+// strides count as meeting when their ranges do.
+bool paged_meet(const PagedSpan& x, const PagedSpan& y);
 // out may be q's own memory row for row, else it must lie apart from it.
 int paged_apart(const gtn_tensor* q, const gtn_tensor* out, const char* who, const char* name);
 

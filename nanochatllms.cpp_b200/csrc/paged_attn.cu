@@ -148,6 +148,15 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     GTN_REQUIRE(workspace && ((uintptr_t)workspace & 15) == 0, "%s: workspace must be 16-byte aligned device memory", who);
     GTN_REQUIRE(workspace_bytes >= ws_need, "%s: workspace of %ld bytes, %ld needed", who, (long)workspace_bytes,
                 (long)ws_need);
+    // what is written lies apart from what is read (the pools are only read and may be one)
+    const PagedSpan io[] = {paged_span(out),         paged_bytes_span(workspace, ws_need), paged_span(block_table),
+                            paged_span(q_start),     paged_span(kv_lens),                  paged_pool_span(a.c, a.c.k),
+                            paged_pool_span(a.c, a.c.v)};
+    for (int i = 0; i < 2; ++i)
+        for (int j = i + 1; j < 7; ++j)
+            GTN_REQUIRE(!paged_meet(io[i], io[j]), "%s: %s overlaps %s", who, i ? "workspace" : "out",
+                        j == 1 ? "workspace" : j < 5 ? "the lengths or the table" : "the cache");
+    GTN_REQUIRE(!paged_meet(io[1], paged_span(q)), "%s: workspace overlaps q", who);
     const void* ptrs[] = {q->data, out->data, a.c.k, a.c.v, block_table->data, q_start->data, kv_lens->data, workspace};
     GTN_CHECK(paged_on_device(ptrs, 8, who));
     a.q = (const uint8_t*)q->data;

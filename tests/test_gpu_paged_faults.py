@@ -5,7 +5,7 @@ import torch
 
 import gten_b200 as G
 import test_gpu_paged as tp
-from paged_ref import F16, F32, Q8, attn_bound, gt, i32, ref_attn, ref_plan
+from paged_ref import F16, F32, Q8, attn_bound, cache_of, gt, i32, new_pool, ref_attn, ref_plan
 from paged_long import LongBatch
 from test_gpu_paged import Batch
 
@@ -190,3 +190,33 @@ def test_append_rotates_as_rotary_emb(gpu, d, rope_pct):
     mag = x.double().view(rows, heads, d).abs().amax(-1, keepdim=True).expand(-1, -1, d).reshape(rows, -1)
     err = 2 * mag * (p * 12 * 2.0 ** -23 + 2.0 ** -22)
     assert bool(((out.double() - want.double()).abs() <= err + (want.double().abs() + err) * 2.0 ** -11 + 2.0 ** -25).all())
+
+
+# ---- column ranges of one buffer ------------------------------------------------------------------------
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("cache", [F16, Q8])
+def test_rows_side_by_side(gpu, cache, in_place):
+    """Queries, keys, values, rotated queries and outputs as columns of one buffer give what separate ones give."""
+    heads, kvh, d, rows = 4, 2, 64, 37
+    gen = torch.Generator(device=gpu).manual_seed(93)
+    hd, kd = heads * d, kvh * d
+    wide = torch.randn(rows, 3 * hd + 2 * kd, generator=gen, device=gpu).to(torch.float16)
+    cuts = [0, hd, hd + kd, hd + 2 * kd, 2 * hd + 2 * kd, 3 * hd + 2 * kd]
+    part = lambda w, i: gt(w[:, cuts[i]:cuts[i + 1]], F16, (rows, cuts[i + 1] - cuts[i]), (wide.shape[1], 1))  # noqa: E731
+    own = [wide[:, a:b].contiguous() for a, b in zip(cuts, cuts[1:])]
+    pos, lens, starts, table = i32(range(rows), gpu), i32([rows], gpu), i32([0, rows], gpu), i32([[2, 0, 1]], gpu)
+    slots = i32([[2, 0, 1][t // 16] * 16 + t % 16 for t in range(rows)], gpu)
+    got = []
+    for q, k, v, qr, out in ([part(wide, i) for i in range(5)], [gt(x, F16) for x in own]):
+        if in_place:
+            qr = q
+        kp, vp = (new_pool(cache, 3, 16, kvh, d, gpu) for _ in range(2))
+        c = cache_of(kp, vp)
+        G.paged_append(q, k, v, gt(pos), gt(slots), c, qr)
+        G.paged_attn(qr, c, gt(table), gt(starts), gt(lens), out)
+        G.check()
+        got.append((kp.raw, vp.raw))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    for i, x in enumerate(own):
+        assert torch.equal(wide[:, cuts[i]:cuts[i + 1]], x), i

@@ -119,3 +119,72 @@ def test_int_tensors_are_aligned(call, args, name, off):
     a[name].buf += off
     msg = refusal(call, a)
     assert "status 1" in msg and f"{name} must be 4-byte aligned" in msg
+
+
+# ---- overlaps -------------------------------------------------------------------------------------------
+def f16(at, rows, cols, stride=None):
+    return t(at, rows, cols, dtype=G.F16, strides=(stride, 1) if stride else None)
+
+
+def pools(k=AT[5], v=AT[6], stride=0, n_pages=8):
+    return G.PagedCache(k, v, G.F16, n_pages, 16, 2, 64, stride)  # pages of 4,096 bytes
+
+
+@pytest.mark.parametrize("bad,what", [
+    (dict(pos=t(AT[7] + 8, 5)), "q_out overlaps pos or slots"), (dict(slots=t(AT[7] + 2556, 5)), "q_out overlaps pos or slots"),
+    (dict(cache=pools(AT[7])), "q_out overlaps the cache"), (dict(cache=pools(v=AT[7] - 7 * 4096)), "q_out overlaps the cache"),
+    (dict(cache=pools(v=AT[5])), "pools of the cache overlap"), (dict(cache=pools(v=AT[5] + 7 * 4096)), "pools of the cache overlap"),
+    (dict(cache=pools(v=AT[5] + 4080, stride=8192)), "pools of the cache overlap"),
+    (dict(cache=pools(AT[0])), "cache overlaps an input"), (dict(cache=pools(v=AT[2] + 1264)), "cache overlaps an input"),
+    (dict(pos=t(AT[6] + 8 * 4096 - 4, 5)), "cache overlaps an input"), (dict(slots=t(AT[5], 5)), "cache overlaps an input"),
+    # in the queries' place, with keys or values that share rows with them
+    (dict(q_out=f16(AT[0], 5, 256), k=f16(AT[0] + 256, 5, 128)), "q_out overlaps k or v"),
+    (dict(q_out=f16(AT[0], 5, 256), v=f16(AT[0], 5, 128, 256)), "q_out overlaps k or v"),
+    (dict(q=f16(AT[0], 5, 256, 512), q_out=f16(AT[0], 5, 256, 512), k=f16(AT[0] + 500, 5, 128, 512)), "q_out overlaps k or v"),
+    (dict(q=f16(AT[0], 5, 256, 512), q_out=f16(AT[0], 5, 256, 512), k=f16(AT[0] + 512, 5, 128, 384)), "q_out overlaps k or v")],
+    ids=str)
+def test_append_refuses_overlaps(bad, what):
+    msg = refusal(G.paged_append, append_args(**bad))
+    assert "status 1" in msg and what in msg
+
+
+@pytest.mark.parametrize("good", [
+    dict(k=f16(AT[1], 5, 128), v=f16(AT[1], 5, 128)),                                     # read twice
+    dict(cache=pools(v=AT[5] + 4096, stride=8192)),                                       # K and V pages in turns
+    dict(cache=pools(v=AT[5] + 8192, stride=3 * 4096)), dict(cache=pools(n_pages=1, v=AT[5] + 4096)),
+    dict(q_out=f16(AT[0], 5, 256)),                                                       # in the queries' place
+    # column ranges of one buffer of 1,024 elements a row
+    dict(q=f16(AT[0], 5, 256, 1024), k=f16(AT[0] + 512, 5, 128, 1024), v=f16(AT[0] + 768, 5, 128, 1024),
+         q_out=f16(AT[0], 5, 256, 1024)),
+    dict(q=f16(AT[0], 5, 256, 1024), k=f16(AT[0] + 512, 5, 128, 1024), v=f16(AT[0] + 768, 5, 128, 1024),
+         q_out=f16(AT[0] + 1024, 5, 256, 1024)),
+    dict(q=f16(AT[0] + 1024, 5, 256, 1024), q_out=f16(AT[0] + 512, 5, 256, 1024)),
+    dict(q=f16(AT[0], 1, 256), k=f16(AT[0] + 512, 1, 128), v=f16(AT[0] + 768, 1, 128), q_out=f16(AT[0], 1, 256), pos=t(AT[3], 1),
+         slots=t(AT[4], 1))], ids=str)
+def test_append_takes_neighbours(good):
+    assert passed(refusal(G.paged_append, append_args(**good)))
+
+
+@pytest.mark.parametrize("bad,what", [
+    (dict(block_table=t(AT[6] + 2556, 3, 4)), "out overlaps the lengths or the table"),
+    (dict(q_start=t(AT[6], 4)), "out overlaps the lengths or the table"), (dict(kv_lens=t(AT[6] - 8, 3)), "out overlaps the lengths"),
+    (dict(cache=pools(AT[6])), "out overlaps the cache"), (dict(cache=pools(v=AT[6] - 16)), "out overlaps the cache"),
+    (dict(workspace=Ws(AT[6] + 16, 64 * MB)), "out overlaps workspace"),
+    (dict(workspace=Ws(AT[0] - 64, 64 * MB)), "workspace overlaps q"),
+    (dict(workspace=Ws(AT[3], 64 * MB)), "workspace overlaps the lengths or the table"),
+    (dict(workspace=Ws(AT[4] - 1024, 64 * MB)), "workspace overlaps the lengths or the table"),
+    (dict(workspace=Ws(AT[5] - 1024, 64 * MB)), "workspace overlaps the lengths or the table"),
+    (dict(workspace=Ws(AT[1] + 4096, 64 * MB)), "workspace overlaps the cache"),
+    (dict(workspace=Ws(AT[2] - 1024, 64 * MB)), "workspace overlaps the cache")], ids=str)
+def test_attn_refuses_overlaps(bad, what):
+    msg = refusal(G.paged_attn, attn_args(**bad))
+    assert "status 1" in msg and what in msg
+
+
+@pytest.mark.parametrize("good", [
+    dict(out=f16(AT[0], 5, 256)), dict(q=f16(AT[0], 5, 256, 640), out=f16(AT[0] + 512, 5, 256, 640)),
+    dict(q=f16(AT[0] + 1000 * 1280, 5, 256, 640), out=f16(AT[0] + 640, 5, 256, 640)),
+    dict(cache=pools(AT[1], AT[1])), dict(cache=pools(AT[1], AT[1] + 4096, stride=8192)),
+    dict(q=f16(AT[0], 1, 256), out=f16(AT[0] + 512, 1, 256))], ids=str)
+def test_attn_takes_neighbours(good):
+    assert passed(refusal(G.paged_attn, attn_args(**good)))
