@@ -49,9 +49,8 @@ unsigned int* device_error_word() {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev != dev_cached) {
-        p = nullptr;
-        if (cudaGetSymbolAddress((void**)&p, g_dev_err) != cudaSuccess) p = nullptr;
-        dev_cached = dev;
+        dev_cached = cudaGetSymbolAddress((void**)&p, g_dev_err) == cudaSuccess ? dev : -1;  // a failure is not kept
+        if (dev_cached < 0) p = nullptr;
     }
     return p;
 }

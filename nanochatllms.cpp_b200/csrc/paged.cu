@@ -51,6 +51,11 @@ int paged_on_device(const void* const* p, int n, const char* who) {
     return GTN_OK;
 }
 
+int paged_error_word(unsigned int** out, const char* who) {
+    *out = device_error_word();
+    return *out ? GTN_OK : fail(GTN_ERR_CUDA, "%s: the current device has no error word", who);
+}
+
 PagedSpan paged_span(const gtn_tensor* t) {
     const uint8_t* p = (const uint8_t*)t->data;
     const long width = row_bytes(t->dtype, t->shape[t->ndim - 1]);
@@ -302,7 +307,7 @@ static __global__ void __launch_bounds__(APP_THREADS, 5) k_paged_append(AppendAr
     if (tid < a.half) cs[tid] = rope_cs(pos, fr.f[tid]);
     const int page = slot >> a.c.ps_shift, r = slot & (a.c.ps - 1);
     const bool store = slot >= 0 && page < a.c.n_pages;
-    if (slot >= 0 && !store && tid == 0 && a.err) atomicOr(a.err, GTN_DEVERR_PAGE);
+    if (slot >= 0 && !store && tid == 0) atomicOr(a.err, GTN_DEVERR_PAGE);
     __syncthreads();
     // a head's lanes go the same way, the heads of a warp need not (types, turns): shuffles name the head's lanes alone
     const unsigned mates = ((1u << TPH) - 1) << (tid & 31 & ~(TPH - 1));
@@ -392,7 +397,7 @@ static __global__ void __launch_bounds__(APP_THREADS) k_paged_append_any(AppendA
     __syncthreads();
     const int kvh = a.c.kv_heads, page = slot >> a.c.ps_shift, r = slot & (a.c.ps - 1);
     const bool store = slot >= 0 && page < a.c.n_pages;
-    if (slot >= 0 && !store && tid == 0 && a.err) atomicOr(a.err, GTN_DEVERR_PAGE);
+    if (slot >= 0 && !store && tid == 0) atomicOr(a.err, GTN_DEVERR_PAGE);
     const long hb = row_bytes(a.sdt, D);
     for (int hh = warp; hh < a.heads + 2 * kvh; hh += APP_THREADS / 32) {
         const bool is_q = hh < a.heads, is_k = !is_q && hh < a.heads + kvh;
@@ -498,8 +503,9 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
             GTN_REQUIRE(!paged_meet(span[i], span[j]), "%s: tensors that are written overlap others", who);
     const void* ptrs[] = {ctx_lens->data, new_lens->data, free_pages->data, n_free->data, block_table->data,
                           q_start->data,  kv_lens->data,  pos->data,        slots->data,  n_used->data};
-    GTN_CHECK(paged_on_device(ptrs, 10, who));
     PlanArgs a;
+    GTN_CHECK(paged_error_word(&a.err, who));
+    GTN_CHECK(paged_on_device(ptrs, 10, who));
     a.ctx = (const int32_t*)ctx_lens->data;
     a.nw = (const int32_t*)new_lens->data;
     a.free_pages = (const int32_t*)free_pages->data;
@@ -516,7 +522,6 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
     a.max_pages = block_table->shape[1];
     a.rows = pos->shape[0];
     a.ps_shift = __builtin_ctz((unsigned)page_size);
-    a.err = device_error_word();
     return cuda_status(launch_pdl(k_paged_plan, dim3((a.rows + PLAN_ROWS - 1) / PLAN_ROWS), dim3(PLAN_THREADS), 0,
                                   S(stream), a),
                        who);
@@ -563,6 +568,7 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
     GTN_REQUIRE(rope_pct >= 0.0f && rope_pct <= 1.0f, "%s: rope_pct", who);
     GTN_REQUIRE(rope_base > 0.0f && std::isfinite(rope_base), "%s: rope_base", who);
     const void* ptrs[] = {q->data, k->data, v->data, q_out->data, pos->data, slots->data, a.c.k, a.c.v};
+    GTN_CHECK(paged_error_word(&a.err, who));
     GTN_CHECK(paged_on_device(ptrs, 8, who));
     a.q = (const uint8_t*)q->data;
     a.k = (const uint8_t*)k->data;
@@ -579,7 +585,6 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
     a.odt = q_out->dtype;
     const int rd = (int)((float)d * rope_pct);
     a.half = rd / 2;
-    a.err = device_error_word();
     RopeFreq fr;
     for (int j = 0; j < 64; ++j) fr.f[j] = j < a.half ? std::pow((double)rope_base, -2.0 * j / rd) : 0.0;  // (rd may be odd)
     bool aligned = a.half % 8 == 0;

@@ -41,6 +41,8 @@ int paged_int_arg(const gtn_tensor* t, int ndim, const char* who, const char* na
 // Every pointer lies in memory that the current device owns (or managed memory). Turns a host pointer or
 // another device's tensor into an error before a kernel meets it.
 int paged_on_device(const void* const* p, int n, const char* who);
+// The device error word, which the kernels write without asking whether there is one.
+int paged_error_word(unsigned int** out, const char* who);
 // The rows of a tensor (or the pages of a pool): `width` bytes every `stride` bytes (0: one row), in [data, end).
 struct PagedSpan {
     const uint8_t *data, *end;

@@ -158,6 +158,7 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
                         j == 1 ? "workspace" : j < 5 ? "the lengths or the table" : "the cache");
     GTN_REQUIRE(!paged_meet(io[1], paged_span(q)), "%s: workspace overlaps q", who);
     const void* ptrs[] = {q->data, out->data, a.c.k, a.c.v, block_table->data, q_start->data, kv_lens->data, workspace};
+    GTN_CHECK(paged_error_word(&a.err, who));
     GTN_CHECK(paged_on_device(ptrs, 8, who));
     a.q = (const uint8_t*)q->data;
     a.out = (uint8_t*)out->data;
@@ -179,7 +180,6 @@ int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_
     a.n_sink = n_sink;
     a.scale_log2 = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)d)) * 1.4426950408889634f;
     a.part = (float*)workspace;
-    a.err = device_error_word();
     // Requests of at most `cut` rows per kv head (tokens x query heads of it) go to the decode kernel, whose tiles are
     // 8 or 16 rows high, the others to the chunk kernel (16 requests of two tokens x 8 heads over 500 to 1,900 keys:
     // 20.5 us against 26.6). With a bound on the new tokens that says so, only the decode kernel is launched (single

@@ -188,3 +188,16 @@ def test_attn_refuses_overlaps(bad, what):
     dict(q=f16(AT[0], 1, 256), out=f16(AT[0] + 512, 1, 256))], ids=str)
 def test_attn_takes_neighbours(good):
     assert passed(refusal(G.paged_attn, attn_args(**good)))
+
+
+# ---- the device -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("call,args", [(G.paged_plan, plan_args), (G.paged_append, append_args), (G.paged_attn, attn_args)],
+                         ids=["plan", "append", "attn"])
+def test_without_an_error_word_nothing_is_launched(call, args):
+    """The kernels write the device's error word without asking whether there is one."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("there is one")
+    for _ in range(2):
+        msg = refusal(call, args())
+        assert "status 2" in msg and "no error word" in msg
