@@ -150,7 +150,7 @@ int64_t gtn_paged_page_bytes(int dtype, int page_size, int kv_heads, int d_head)
 
 /* Plans one step for n requests (1 to 4096). All tensors int32 on the device:
  *   ctx_lens [n], new_lens [n]   tokens already in the cache, tokens of this step (0 allowed);
- *   free_pages [f], n_free [1]   page ids to hand out, in order; how many of them are free (<= f);
+ *   free_pages [f], n_free [1]   page ids to hand out, in order (f may be 0); how many of them are free (<= f);
  *   block_table [n, max_pages]   in and out: the first ceil(ctx / page_size) entries of a row are its
  *                                pages; the pages for the new tokens are written behind them;
  *   q_start [n + 1]              prefix sum of new_lens;

@@ -476,7 +476,9 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
     const char* who = "paged_plan";
     GTN_CHECK(paged_int_arg(ctx_lens, 1, who, "ctx_lens"));
     GTN_CHECK(paged_int_arg(new_lens, 1, who, "new_lens"));
-    GTN_CHECK(paged_int_arg(free_pages, 1, who, "free_pages"));
+    // a list that has run out may be empty (then without memory): requests that need no page go on
+    const bool none = free_pages && free_pages->dtype == GTN_I32 && free_pages->ndim == 1 && free_pages->shape[0] == 0;
+    if (!none) GTN_CHECK(paged_int_arg(free_pages, 1, who, "free_pages"));
     GTN_CHECK(paged_int_arg(n_free, 1, who, "n_free"));
     GTN_CHECK(paged_int_arg(block_table, 2, who, "block_table"));
     GTN_CHECK(paged_int_arg(q_start, 1, who, "q_start"));
@@ -497,11 +499,11 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
                 block_table->shape[1]);
     const gtn_tensor* io[] = {block_table, q_start, kv_lens, pos, slots, n_used, ctx_lens, new_lens, free_pages, n_free};
     PagedSpan span[10];
-    for (int i = 0; i < 10; ++i) span[i] = paged_span(io[i]);
+    for (int i = 0; i < 10; ++i) span[i] = none && io[i] == free_pages ? paged_bytes_span(nullptr, 0) : paged_span(io[i]);
     for (int i = 0; i < 6; ++i)
         for (int j = i + 1; j < 10; ++j)
             GTN_REQUIRE(!paged_meet(span[i], span[j]), "%s: tensors that are written overlap others", who);
-    const void* ptrs[] = {ctx_lens->data, new_lens->data, free_pages->data, n_free->data, block_table->data,
+    const void* ptrs[] = {ctx_lens->data, new_lens->data, none ? n_free->data : free_pages->data, n_free->data, block_table->data,
                           q_start->data,  kv_lens->data,  pos->data,        slots->data,  n_used->data};
     PlanArgs a;
     GTN_CHECK(paged_error_word(&a.err, who));

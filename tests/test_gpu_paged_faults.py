@@ -220,3 +220,11 @@ def test_rows_side_by_side(gpu, cache, in_place):
         assert torch.equal(a, b)
     for i, x in enumerate(own):
         assert torch.equal(wide[:, cuts[i]:cuts[i + 1]], x), i
+
+
+def test_plan_with_an_empty_free_list(gpu):
+    """A server whose pages are all handed out goes on with the requests that need none."""
+    t = plan(gpu, [5, 16, 31], [3, 1, 1], [], [[2, -1], [4, -1], [1, 3]], 6, 16)
+    G.check()
+    assert t["kv"].tolist() == [8, 0, 32] and t["used"].item() == 0 and t["q_start"].tolist() == [0, 3, 4, 5]
+    assert t["slots"].tolist() == [37, 38, 39, -1, 63, -1] and t["table"].tolist() == [[2, -1], [4, -1], [1, 3]]

@@ -201,3 +201,10 @@ def test_without_an_error_word_nothing_is_launched(call, args):
     for _ in range(2):
         msg = refusal(call, args())
         assert "status 2" in msg and "no error word" in msg
+
+
+def test_plan_takes_an_empty_free_list():
+    assert passed(refusal(G.paged_plan, plan_args(free_pages=t(0, 0))))
+    assert passed(refusal(G.paged_plan, plan_args(free_pages=t(AT[2], 0))))
+    for bad in (t(0, 9), t(0, 0, dtype=G.F32), t(0, 0, 1), t(AT[2], -1)):
+        assert "status 1" in refusal(G.paged_plan, plan_args(free_pages=bad))
