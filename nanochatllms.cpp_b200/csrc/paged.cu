@@ -68,8 +68,7 @@ PagedSpan paged_pool_span(const PagedCache& c, const uint8_t* pool) {
     return {pool, pool + (c.n_pages - 1) * c.page_stride + width, width, c.n_pages > 1 ? c.page_stride : 0};
 }
 
-bool paged_meet(const PagedSpan& x, const PagedSpan& y) {
-    if (x.data >= y.end || y.data >= x.end) return false;
+bool paged_meet_rows(const PagedSpan& x, const PagedSpan& y) {
     const long stride = x.stride ? x.stride : y.stride;
     if (stride == 0 || (y.stride && y.stride != stride)) return true;
     long off = (y.data - x.data) % stride;  // of y's columns behind x's

@@ -53,7 +53,10 @@ PagedSpan paged_pool_span(const PagedCache& c, const uint8_t* pool);
 inline PagedSpan paged_bytes_span(const void* p, long n) { return {(const uint8_t*)p, (const uint8_t*)p + n, n, 0}; }
 // Whether two of them may share bytes. Exact for rows of one stride (column ranges of one buffer); rows of different
 // strides count as meeting when their ranges do.
-bool paged_meet(const PagedSpan& x, const PagedSpan& y);
+bool paged_meet_rows(const PagedSpan& x, const PagedSpan& y);
+inline bool paged_meet(const PagedSpan& x, const PagedSpan& y) {
+    return x.data < y.end && y.data < x.end && paged_meet_rows(x, y);
+}
 // out may be q's own memory row for row, else it must lie apart from it.
 int paged_apart(const gtn_tensor* q, const gtn_tensor* out, const char* who, const char* name);
 

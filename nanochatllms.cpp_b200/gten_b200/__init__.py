@@ -185,29 +185,24 @@ class GT(_Described):
         return t
 
 
-def _place(t):
-    """What a kept descriptor of a GT or PagedCache depends on besides its fields: the buffers' addresses. None: its
-    descriptor is not kept (another class, or fields that can change in place)."""
-    if type(t) is GT:
-        if isinstance(t.shape, tuple) and (t.strides is None or isinstance(t.strides, tuple)):
-            return _ptr(t.buf)
-    elif type(t) is PagedCache:
-        return _ptr(t.k), _ptr(t.v)
-    return None
-
-
 def _d(t):
-    """The descriptor by reference: kept with the object, and made anew when a field or a buffer's address has changed."""
+    """The descriptor by reference: kept with a GT or PagedCache, and made anew when a field or a buffer's address has
+    changed. Not kept for other classes, and for fields that can change in place (lists)."""
     if t is None:
         return None
-    at = _place(t)
-    if at is None:
-        return C.byref(t.desc())
-    r = t._ref
-    if r is None or r[1] != at:
-        r = (C.byref(t.desc()), at)
-        object.__setattr__(t, "_ref", r)
-    return r[0]
+    r = getattr(t, "_ref", None)
+    if r is not None and _ptr(r[2]) == r[1] and (r[3] is None or _ptr(r[4]) == r[3]):
+        return r[0]
+    c = t.desc()
+    ref = C.byref(c)
+    if type(t) is PagedCache:
+        r = (ref, c.k or 0, t.k, c.v or 0, t.v)
+    elif type(t) is GT and isinstance(t.shape, tuple) and (t.strides is None or isinstance(t.strides, tuple)):
+        r = (ref, c.data or 0, t.buf, None, None)
+    else:
+        return ref
+    object.__setattr__(t, "_ref", r)
+    return ref
 
 
 # ---- gten::ops (src/gten/ops.h) -------------------------------------------------------------
