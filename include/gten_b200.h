@@ -173,7 +173,8 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
  * rows into the pages of slots[r]. q [rows, heads * d_head], k and v [rows, kv_heads * d_head]: fp32, fp16
  * or Q8, one type, row strides as in their descriptors (they may be column ranges of one stacked
  * projection); q_out [rows, heads * d_head]: fp16 or Q8; pos and slots: int32 [rows]. q_out may be q's own
- * memory when type and strides agree, else it lies apart from q, k and v. Q8 results use the activation quantizer (gtn_quantize_q8_rows), but
+ * memory when type and strides agree, else it lies apart from q; it lies apart from k, v, pos, slots and the
+ * pools, and these from each other (k and v may be one, column ranges of one buffer with one stride are apart). Q8 results use the activation quantizer (gtn_quantize_q8_rows), but
  * Q8 value rows go to a Q8 cache unchanged. Rows with pos < 0 are skipped, rows with slot < 0 write no
  * cache row; two rows must not share a slot. */
 int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor* v, const gtn_tensor* pos,
@@ -187,14 +188,18 @@ int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor*
  * (kv_lens[b] = 0: a request that was not granted). Keys that a row does not see never reach it,
  * whatever they hold, and table entries whose page no row of the request sees may be anything.
  *   q, out [rows, heads * d_head]: fp16 (16-byte aligned rows) or Q8, the same type and shape, rows <= 2^20;
- *   out may be q's own memory when the strides agree, else it lies apart;
+ *   out may be q's own memory when the strides agree, else it lies apart from it (column ranges of one buffer, with
+ *   one stride, are apart), and from all else that is read in any case;
  *   block_table int32 [n, max_pages], q_start int32 [n + 1], kv_lens int32 [n], n <= 4096, max_pages *
  *   page_size < 2^30; calls whose rows times keys could exceed 2^31 tiles are refused;
  *   scale: 0 means 1 / sqrt(d_head); max_new: a bound on the new tokens of one request where the caller
- *   knows one (1 for a decode step), else 0: it chooses the kernels, not the result;
+ *   knows one (1 for a decode step), else 0: it chooses the kernels, not the result or whether a call is taken;
  *   workspace: device memory of gtn_paged_attn_workspace(...) bytes, 16-byte aligned; its contents are
- *   scratch, and calls that may run at the same time need one each.
- * Q8 caches and activations enter the products as fp16, so |value| must stay below 65504. */
+ *   scratch, and calls that may run at the same time need one each. It lies apart from all other arguments.
+ * Numerics: scores, maxima, sums and joins in fp32; weights round to fp16 (2^-11 relative, over Q8 pages behind their product
+ * with the value's delta). Values of a Q8 cache (int8 * delta) enter the products exactly, to 2^-25 absolute, as long as
+ * they stay below 65504 in magnitude; Q8 queries round to fp16, single fp16 query rows over a Q8 cache to 16 bits of their
+ * block's largest element. */
 int64_t gtn_paged_attn_workspace(int heads, int d_head);
 int gtn_paged_attn(const gtn_tensor* q, const gtn_paged_cache* cache, const gtn_tensor* block_table,
                    const gtn_tensor* q_start, const gtn_tensor* kv_lens, gtn_tensor* out, float scale, int window,

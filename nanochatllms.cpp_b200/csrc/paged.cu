@@ -88,7 +88,7 @@ int paged_apart(const gtn_tensor* q, const gtn_tensor* out, const char* who, con
 // stays within n_free; q_start = prefix of new. Every CTA runs both prefix sums over all requests itself
 // (at most 8 requests a thread; a second kernel for them would cost more than the few microseconds of
 // one CTA) and then writes its share of the table entries and of the rows.
-// Bound by latency, not by its bytes: 64 decoding requests 6.4 us, 1,000 requests with some 26,000 rows 8.2 us (graph replay,
+// Bound by latency, not by its bytes: 64 decoding requests 7.5 us, 1,000 requests with some 26,000 rows 8.2 us (graph replay,
 // B200), of which the launch is some 3 and the two scans, with their dependent loads, the rest.
 constexpr int PLAN_THREADS = 512;
 constexpr int PLAN_ROWS = 1024;  // rows per CTA
@@ -275,11 +275,11 @@ __device__ __forceinline__ void app_load8(const uint8_t* head, int e0, float (&x
 
 // One CTA per row; a thread takes two groups of eight elements of a head: those that rotate into each other (i
 // and i + half / 8, for i < half / 8), or two neighbours of the rest. D / 16 adjacent lanes hold a head, so the
-// absmax of a 32-element block is a few shuffles. Bound by its loads and stores, 16 bytes each (fp16): 1,948 rows of
-// Zephyr 16.5 us over changing inputs, 2.9 TB/s (12.3 us where they stay in L2); MiniCPM's 1,879 rows from fp32 into Q8 28.7
-// us, bound by the quantizer's instructions. 16 rows: 4.1 us, a launch. Five CTAs per SM (registers) were the best.
-// For rows that are 16-byte aligned and a rotated width of whole groups; k_paged_append_any takes the others (the same
-// rows 26.8 us, 38.9 us and 6.2 us there, against 12.3, 24.3 and 4.1 here).
+// absmax of a 32-element block is a few shuffles. 1,948 rows of Zephyr, fp16, over changing inputs: 16.4 us, 2.9 TB/s;
+// MiniCPM's 1,879 rows from fp32 into Q8: 20.2 us, 3.5 TB/s; 16 rows: 4.1 us, a launch. Of what must be moved that is 44%
+// and 53% of a copy's rate: a row's second turn is partly empty and loads only when the first has stored. Five CTAs per SM
+// (registers) were the best. For rows that are 16-byte aligned and a rotated width of whole groups; k_paged_append_any takes
+// the others (the same rows, back to back in L2: 25.8 us, 37.7 us and 4.5 us there, against 10.7, 14.6 and 2.5 here).
 template <int D, int SDT>
 static __global__ void __launch_bounds__(APP_THREADS, 5) k_paged_append(AppendArgs a, const __grid_constant__ RopeFreq fr) {
     constexpr int TPH = D / 16, NB = D / GTN_QBLK;  // threads and blocks of a head

@@ -26,11 +26,13 @@
 // Every wait is bounded as in gemm_tc.cuh.
 //
 // Measured (graph replay, B200): 2,048 tokens over 29,999 keys, 32/8 heads of 128, fp16: 1,100 us, 945 TFLOP/s, 57% of
-// the library product's rate: the exponentials take 66% of their unit, the rest goes where softmax and products wait
-// for each other in turns. Window chunks (D = 64): 126 us, 330 TFLOP/s, bound by the exponentials (half the
-// products per exponential of D = 128). Q8 prompts: 117 us, bound by the conversion of the pages (some 350 cycles per
-// 512 elements and warp, next to two softmax warps per scheduler). A call of a few units per CTA is bound by the
-// code's first run: 7,500 cycles to the first product, 5,500 behind an item.
+// the library product's rate: tensor cores and exponentials are both active 56% of the time, in turns, so that neither is
+// the bound by itself. Window chunks (D = 64): 126 us, 330 TFLOP/s; the visible pairs' exponentials are some 36 us of it (16 per
+// cycle and SM), keys that units hold and rows do not see come on top (halves end at the causal limit, but begin at
+// the unit in which the window does, and a few first tokens cost a unit); what the rest waits for is not separated yet. Q8
+// prompts: 117 us; the conversion of the pages (some 350 cycles per 512 elements and warp: 3,700 a unit, against 2,048 of
+// exponentials) is less than half of it, and the rest is not separated either. A call of a few units per CTA is bound by
+// the code's first run: 7,500 cycles to the first product, 5,500 behind an item.
 // One query row per thread and 384 threads leave 168 registers each; four softmax warpgroups (two threads a row) spilled
 // and were slower, as were more CTAs with smaller tiles.
 #pragma once
@@ -42,6 +44,8 @@ constexpr int CH_THREADS = 384;
 constexpr int CH_ROWS = 256;
 constexpr int CH_KEYS = 128;
 constexpr float CH_BIAS = 7.0f;
+// Rescaling only when the maximum has grown past a threshold, instead of at every new one, is a published method of
+// fused attention for this GPU generation; the threshold is set by the weights' type: 2^(CH_BIAS + CH_GROW) < 65504.
 constexpr float CH_GROW = 8.0f;
 
 template <int DT, int D>

@@ -16,7 +16,7 @@
 // Q8 caches keep their 8-bit values exact in fp16; the deltas are applied in fp32, to the scores per
 // 32-element block of K and to the weights per 32-column block of V before these round to fp16.
 //
-// One query row per kv head over a Q8 cache (no grouping, single tokens) is bound by instructions on that way: 7
+// One query row per kv head over a Q8 cache (no grouping, single tokens) wastes instructions on that way: 7
 // of 8 rows of every fragment are empty. There (ROWS = 1) a lane owns whole keys: scores are 8-bit dot products
 // (dp4a) of the key with the query, itself split into two bytes per element (q = scale (256 hi + lo), 2^-16 of
 // the block's largest; Q8 queries are their own byte, exactly), softmax runs on one or two scores per lane, and
@@ -25,7 +25,8 @@
 //
 // Measured (graph replay, B200): 16 sequences of 32/8 heads of 128 behind a window of 4,096 keys, fp16: 59 us, 4.56 TB/s,
 // 69% of a copy's rate; the kernel alone reads 269 MB (what it must) in 53 us. MiniCPM's batch of 64, Q8: 63 us, 3.8
-// TB/s: half the issue slots are taken, 910 instructions per 64 keys. One TinyLlama sequence of 1,990 keys: 12.3 us, all
+// TB/s: 910 instructions per 64 keys take half the issue slots, with three warps per scheduler: what bounds it is the
+// latency between dependent instructions rather than their number. One TinyLlama sequence of 1,990 keys: 12.3 us, all
 // latency: the schedule and its first run of code 3 us, two steps of keys, and the join behind a second launch.
 // Fewer stages with more CTAs per SM (F16: 2 stages, 3 CTAs), and more CTAs than are resident, measured the same or
 // slower.
