@@ -174,9 +174,9 @@ int gtn_paged_plan(const gtn_tensor* ctx_lens, const gtn_tensor* new_lens, const
  * or Q8, one type, row strides as in their descriptors (they may be column ranges of one stacked
  * projection); q_out [rows, heads * d_head]: fp16 or Q8; pos and slots: int32 [rows]. q_out may be q's own
  * memory when type and strides agree, else it lies apart from q; it lies apart from k, v, pos, slots and the
- * pools, and these from each other (k and v may be one, column ranges of one buffer with one stride are apart). Q8 results use the activation quantizer (gtn_quantize_q8_rows), but
- * Q8 value rows go to a Q8 cache unchanged. Rows with pos < 0 are skipped, rows with slot < 0 write no
- * cache row; two rows must not share a slot. */
+ * pools, and the pools from each other and from all that is read (column ranges of one buffer, with one stride,
+ * are apart). Q8 results use the activation quantizer (gtn_quantize_q8_rows), but Q8 value rows go to a Q8 cache
+ * unchanged. Rows with pos < 0 are skipped, rows with slot < 0 write no cache row; two rows must not share a slot. */
 int gtn_paged_append(const gtn_tensor* q, const gtn_tensor* k, const gtn_tensor* v, const gtn_tensor* pos,
                      const gtn_tensor* slots, const gtn_paged_cache* cache, gtn_tensor* q_out, float rope_pct,
                      float rope_base, void* stream);
